@@ -1,6 +1,7 @@
-"""Builds libafc_env.so (HIP kernels + C ABI) in-tree for gfx950.
+"""Builds libafc_env.so (the environment: HIP kernels + C ABI) and libafc_ops.so (the learner's sequence and gradient
+operators) in-tree for gfx950.
 
-    python -m rlfluidcontrol_amd.build [--force]
+    python -m rlfluidcontrol_amd.build [--force] [--ops]     (--ops: only libafc_ops.so)
 
 hipcc cross-compiles without a GPU.  -ffp-contract=off: the reference (Java) never fuses
 multiply-add, and parity with the oracle is checked at the bit level wherever the
@@ -31,46 +32,80 @@ FLAGS = (os.environ.get("AFC_EXTRA_FLAGS", "").split()) + ["-O3", "-std=c++17", 
 
 STAMP = os.path.join(HERE, "build", "flags.stamp")
 
+# libafc_ops.so (include/afc_ops.h).  Scalar float arithmetic only: its kernels fuse multiply-adds where the source says so
+# (__builtin_fmaf), and the packed forms, which the compiler would make of them by itself, are switched off.
+OPS_LIB = os.path.join(HERE, "libafc_ops.so")
+OPS_CSRC = os.path.join(CSRC, "ops")
+OPS_SOURCES = ["conv.hip", "scan.hip", "clip.hip"]
+OPS_STAMP = os.path.join(HERE, "build", "ops_flags.stamp")
+OPS_FLAGS = FLAGS + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
-def _flag_string():
-    """the effective compile + link flags: a library built with other flags (AFC_EXTRA_FLAGS) is not reused silently"""
-    return " ".join(FLAGS) + " | HIPCC=" + os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+
+def _ops_deps():
+    d = [os.path.join(OPS_CSRC, f) for f in os.listdir(OPS_CSRC)]
+    return d + [os.path.join(HERE, "..", "include", f) for f in ("afc_ops.h", "afc_env.h")]
+
+
+class _Library:
+    def __init__(self, path, csrc, sources, deps, flags, stamp):
+        self.path, self.csrc, self.sources, self.deps, self.flags, self.stamp = path, csrc, sources, deps, flags, stamp
+
+    def flag_string(self):
+        """the effective compile + link flags: a library built with other flags (AFC_EXTRA_FLAGS) is not reused silently"""
+        return " ".join(self.flags) + " | HIPCC=" + os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+
+    def needs_build(self):
+        if not os.path.exists(self.path):
+            return True
+        t = os.path.getmtime(self.path)
+        if any(os.path.getmtime(d) > t for d in self.deps()):
+            return True
+        if os.environ.get("AFC_EXTRA_FLAGS") or os.path.exists(self.stamp):
+            # a stamp exists only next to a library this module built: compare the flags it was built with
+            try:
+                return open(self.stamp).read() != self.flag_string()
+            except OSError:
+                return True
+        return False
+
+
+ENV = _Library(LIB, CSRC, SOURCES, _deps, FLAGS, STAMP)
+OPS = _Library(OPS_LIB, OPS_CSRC, OPS_SOURCES, _ops_deps, OPS_FLAGS, OPS_STAMP)
 
 
 def needs_build():
-    if not os.path.exists(LIB):
-        return True
-    t = os.path.getmtime(LIB)
-    if any(os.path.getmtime(d) > t for d in _deps()):
-        return True
-    if os.environ.get("AFC_EXTRA_FLAGS") or os.path.exists(STAMP):
-        # a stamp exists only next to a library this module built: compare the flags it was built with
-        try:
-            return open(STAMP).read() != _flag_string()
-        except OSError:
-            return True
-    return False
+    return ENV.needs_build()
 
 
 def build(force=False, verbose=False):
-    if not force and not needs_build():
-        return LIB
+    """Both libraries; returns the environment's."""
+    build_ops(force, verbose)
+    return _build(ENV, force, verbose)
+
+
+def build_ops(force=False, verbose=False):
+    return _build(OPS, force, verbose)
+
+
+def _build(lib, force, verbose):
+    if not force and not lib.needs_build():
+        return lib.path
     import fcntl
     # several ranks of one node may get here together (torchrun): serialise, re-check, build to a
     # temporary name and rename so that nobody ever loads a half-written library
     with open(os.path.join(HERE, ".build.lock"), "w") as lk:
         fcntl.flock(lk, fcntl.LOCK_EX)
         try:
-            if force or needs_build():
+            if force or lib.needs_build():
                 hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-                tmp = LIB + ".tmp.%d" % os.getpid()
+                tmp = lib.path + ".tmp.%d" % os.getpid()
                 objdir = os.path.join(HERE, "build")
                 os.makedirs(objdir, exist_ok=True)
                 jobs = []
                 try:
-                    for src in SOURCES:
+                    for src in lib.sources:
                         obj = os.path.join(objdir, os.path.splitext(src)[0] + ".%d.o" % os.getpid())
-                        cmd = [hipcc] + FLAGS + ["-c", "-o", obj, os.path.join(CSRC, src)]
+                        cmd = [hipcc] + lib.flags + ["-c", "-o", obj, os.path.join(lib.csrc, src)]
                         if verbose:
                             print(" ".join(cmd))
                         jobs.append((obj, cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
@@ -89,9 +124,9 @@ def build(force=False, verbose=False):
                     extra = os.environ.get("AFC_EXTRA_FLAGS", "").split()
                     subprocess.check_call([hipcc] + extra + ["-shared", "-fPIC", "--offload-arch=gfx950", "-o", tmp] +
                                           [j[0] for j in jobs])
-                    os.replace(tmp, LIB)
-                    with open(STAMP, "w") as f:
-                        f.write(_flag_string())
+                    os.replace(tmp, lib.path)
+                    with open(lib.stamp, "w") as f:
+                        f.write(lib.flag_string())
                 finally:  # object files never outlive the call, whether a translation unit failed or not
                     for obj, _, pr in jobs:
                         if pr.poll() is None:
@@ -102,8 +137,8 @@ def build(force=False, verbose=False):
                         os.remove(tmp)
         finally:
             fcntl.flock(lk, fcntl.LOCK_UN)
-    return LIB
+    return lib.path
 
 
 if __name__ == "__main__":
-    print(build(force="--force" in sys.argv, verbose=True))
+    print((build_ops if "--ops" in sys.argv else build)(force="--force" in sys.argv, verbose=True))

@@ -1,0 +1,386 @@
+// conv.hip -- short causal convolution along the sequence (afc_conv, afc_conv_grad, afc_conv_step)
+#include <stdexcept>
+
+#include "ops_common.h"
+
+namespace afc_ops {
+
+template <int DT, int V>
+using Vec = Elem<DT> __attribute__((ext_vector_type(V)));
+
+template <int DT, int V>
+__device__ inline void load(float (&f)[V], const Elem<DT> *p) {
+  if constexpr (V == 1) {
+    f[0] = (float)*p;
+  } else {
+    const Vec<DT, V> v = *reinterpret_cast<const Vec<DT, V> *>(p);
+    for (int i = 0; i < V; ++i) f[i] = (float)v[i];
+  }
+}
+template <int DT, int V>
+__device__ inline void store(Elem<DT> *p, const float (&f)[V]) {
+  if constexpr (V == 1) {
+    *p = (Elem<DT>)f[0];
+  } else {
+    Vec<DT, V> v;
+    for (int i = 0; i < V; ++i) v[i] = (Elem<DT>)f[i];
+    *reinterpret_cast<Vec<DT, V> *>(p) = v;
+  }
+}
+
+struct Tiling {
+  int log_cx;          // lanes side by side along the channels (the others: positions)
+  int run;             // positions of a thread
+  int64_t tiles_c, tiles_l;
+};
+
+constexpr int kRun = 8;  // positions of a forward thread
+
+template <int DT, int V, int K, bool SILU>
+__global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
+  typedef Elem<DT> E;
+  int64_t blk = blockIdx.x;
+  const int64_t ct = blk % T.tiles_c;
+  blk /= T.tiles_c;
+  const int64_t lt = blk % T.tiles_l, b = blk / T.tiles_l;
+  const int cx = 1 << T.log_cx;
+  const int64_t c = (ct * cx + (threadIdx.x & (cx - 1))) * V;
+  if (c >= P.width) return;
+  const int64_t l0 = (lt * (256 >> T.log_cx) + (threadIdx.x >> T.log_cx)) * kRun;
+  const int len = row_length(P.lengths, b, P.length);
+  const E *x = (const E *)P.x.data + b * P.x.stride_batch + c;
+  const E *s0 = P.initial_state ? (const E *)P.initial_state + b * (K - 1) * P.width + c : nullptr;
+  if (l0 == 0 && P.final_state) {
+    for (int j = 0; j < K - 1; ++j) {
+      const int64_t p = (int64_t)len - (K - 1) + j;
+      float v[V] = {};
+      if (p >= 0)
+        load<DT, V>(v, x + p * P.x.stride_length);
+      else if (s0)
+        load<DT, V>(v, s0 + (p + K - 1) * P.width);
+      store<DT, V>((E *)P.final_state + (b * (K - 1) + j) * P.width + c, v);
+    }
+  }
+  if (l0 >= P.length) return;
+  float w[K][V], bias[V] = {}, win[K - 1 + kRun][V];
+  for (int i = 0; i < V; ++i) {
+    for (int k = 0; k < K; ++k) w[k][i] = P.weight[(c + i) * K + k];
+    if (P.bias) bias[i] = P.bias[c + i];
+  }
+#pragma unroll
+  for (int j = 0; j < K - 1 + kRun; ++j) {
+    const int64_t p = l0 + j - (K - 1);
+    for (int i = 0; i < V; ++i) win[j][i] = 0.f;
+    if (p < 0) {
+      if (s0) load<DT, V>(win[j], s0 + (p + K - 1) * P.width);
+    } else if (p < len) {
+      load<DT, V>(win[j], x + p * P.x.stride_length);
+    }
+  }
+  E *y = (E *)P.y.data + b * P.y.stride_batch + c;
+#pragma unroll
+  for (int j = 0; j < kRun; ++j) {
+    const int64_t l = l0 + j;
+    if (l >= P.length) break;
+    float v[V];
+    for (int i = 0; i < V; ++i) {
+      float a = bias[i];
+      for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], win[j + k][i], a);
+      v[i] = l < len ? (SILU ? silu(a) : a) : 0.f;
+    }
+    store<DT, V>(y + l * P.y.stride_length, v);
+  }
+}
+
+template <int DT, int V, int K, bool SILU>
+__global__ __launch_bounds__(256) void k_conv_step(afc_conv_args P) {
+  typedef Elem<DT> E;
+  const int64_t per = P.width / V, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= P.batch * per) return;
+  const int64_t b = t / per, c = (t - b * per) * V;
+  E *st = (E *)P.final_state + b * (K - 1) * P.width + c;
+  float win[K][V];
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) load<DT, V>(win[j], st + j * P.width);
+  load<DT, V>(win[K - 1], (const E *)P.x.data + b * P.x.stride_batch + c);
+  float v[V];
+  for (int i = 0; i < V; ++i) {
+    float a = P.bias ? P.bias[c + i] : 0.f;
+    for (int k = 0; k < K; ++k) a = __builtin_fmaf(P.weight[(c + i) * K + k], win[k][i], a);
+    v[i] = SILU ? silu(a) : a;
+  }
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) store<DT, V>(st + j * P.width, win[j + 1]);
+  store<DT, V>((E *)P.y.data + b * P.y.stride_batch + c, v);
+}
+
+// A thread takes T.run positions [s, e) of V channels.  It walks over the positions q = s .. e + K - 2 whose outputs its dx
+// depend on, with windows of the last K inputs and of the last K dp = dy f'(pre) in registers; dx[q - K + 1] is complete
+// when dp[q] is known.  dweight and dbias: sums of the thread, then of the block, one partial row for each block.
+template <int DT, int V, int K, bool SILU>
+__global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, float *part) {
+  typedef Elem<DT> E;
+  __shared__ float red[256 * V];
+  int64_t blk = blockIdx.x;
+  const int64_t ct = blk % T.tiles_c;
+  blk /= T.tiles_c;
+  const int64_t lt = blk % T.tiles_l, b = blk / T.tiles_l;
+  const int cx = 1 << T.log_cx, ty = 256 >> T.log_cx;
+  const int lane_c = threadIdx.x & (cx - 1), lane_l = threadIdx.x >> T.log_cx;
+  const int64_t c = (ct * cx + lane_c) * V;
+  const int64_t s = (lt * ty + lane_l) * (int64_t)T.run;
+  const int len = row_length(P.lengths, b, P.length);
+  float dw[K + 1][V];
+  for (int k = 0; k <= K; ++k)
+    for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
+  if (c < P.width && (s < P.length || s == 0)) {
+    const int64_t e = s + T.run < P.length ? s + T.run : P.length;
+    const E *x = (const E *)P.x.data + b * P.x.stride_batch + c;
+    const E *dy = (const E *)P.dy.data + b * P.dy.stride_batch + c;
+    E *dx = (E *)P.dx.data + b * P.dx.stride_batch + c;
+    const E *s0 = P.initial_state ? (const E *)P.initial_state + b * (K - 1) * P.width + c : nullptr;
+    const E *df = P.dfinal_state ? (const E *)P.dfinal_state + b * (K - 1) * P.width + c : nullptr;
+    E *ds = P.dinitial_state ? (E *)P.dinitial_state + b * (K - 1) * P.width + c : nullptr;
+    float w[K][V], bias[V] = {}, xw[K][V], dp[K][V];
+    for (int i = 0; i < V; ++i) {
+      for (int k = 0; k < K; ++k) w[k][i] = P.weight[(c + i) * K + k];
+      if (P.bias) bias[i] = P.bias[c + i];
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      for (int i = 0; i < V; ++i) xw[j][i] = dp[j][i] = 0.f;
+      const int64_t p = s + j - K;  // xw[1..K-1]: positions s-K+1 .. s-1 (moved down by one at the first step)
+      if (j > 0 && p < 0) {
+        if (s0) load<DT, V>(xw[j], s0 + (p + K - 1) * P.width);
+      } else if (j > 0 && p < len) {
+        load<DT, V>(xw[j], x + p * P.x.stride_length);
+      }
+    }
+    for (int64_t q = s; q < e + K - 1; ++q) {
+      float xn[V] = {}, dn[V] = {};
+      const bool live = q < len;
+      if (live) {
+        load<DT, V>(xn, x + q * P.x.stride_length);
+        load<DT, V>(dn, dy + q * P.dy.stride_length);
+      }
+      for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k + 1 < K; ++k) {
+          xw[k][i] = xw[k + 1][i];
+          dp[k][i] = dp[k + 1][i];
+        }
+        xw[K - 1][i] = xn[i];
+        float d = dn[i];
+        if (SILU) {
+          float a = bias[i];
+          for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], xw[k][i], a);
+          d *= silu_slope(a, sigmoid(a));
+        }
+        d = live ? d : 0.f;
+        dp[K - 1][i] = d;
+        if (q < e) {
+          for (int k = 0; k < K; ++k) dw[k][i] = __builtin_fmaf(d, xw[k][i], dw[k][i]);
+          dw[K][i] += d;
+        }
+      }
+      const int64_t l = q - (K - 1);
+      if (l < s && (l >= 0 || s > 0)) continue;
+      float v[V];
+      const int64_t jf = l - len + K - 1;
+      float add[V] = {};
+      if (df && jf >= 0 && jf < K - 1) load<DT, V>(add, df + jf * P.width);
+      for (int i = 0; i < V; ++i) {
+        float a = add[i];
+        for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], dp[K - 1 - k][i], a);
+        v[i] = l < len ? a : 0.f;
+      }
+      if (l < 0) {
+        if (ds) store<DT, V>(ds + (l + K - 1) * P.width, v);
+      } else {
+        store<DT, V>(dx + l * P.dx.stride_length, v);
+      }
+    }
+  }
+  if (!part) return;
+  const int64_t row = b * T.tiles_l + lt;
+#pragma unroll
+  for (int k = 0; k <= K; ++k) {
+    __syncthreads();
+    for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = dw[k][i];
+    __syncthreads();
+    if (lane_l == 0 && c < P.width) {
+      for (int i = 0; i < V; ++i) {
+        float a = 0.f;
+        for (int r = 0; r < ty; ++r) a += red[((r << T.log_cx) + lane_c) * V + i];
+        part[(row * (K + 1) + k) * P.width + c + i] = a;
+      }
+    }
+  }
+}
+
+// dweight, dbias: the partial rows summed in their order
+__global__ __launch_bounds__(256) void k_conv_params(const float *part, int64_t rows, int64_t width, int taps, float *dweight,
+                                                     float *dbias) {
+  __shared__ float red[256];
+  const int64_t cols = (taps + 1) * width, col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  float a = 0.f;
+  if (col < cols)
+    for (int64_t r = threadIdx.x >> 6; r < rows; r += 4) a += part[r * cols + col];
+  red[threadIdx.x] = a;
+  __syncthreads();
+  if (threadIdx.x >= 64 || col >= cols) return;
+  a = (red[threadIdx.x] + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]);
+  const int64_t k = col / width, w = col - k * width;
+  if (k < taps) {
+    if (dweight) dweight[w * taps + k] = a;
+  } else if (dbias) {
+    dbias[w] = a;
+  }
+}
+
+namespace {
+
+int elem_bytes(int dtype) { return dtype == AFC_F32 ? 4 : 2; }
+
+void check(const afc_conv_args *p, bool grad, bool step) {
+  want(p != nullptr, "null arguments");
+  want(p->dtype >= AFC_F32 && p->dtype <= AFC_F16, "dtype must be AFC_F32, AFC_BF16 or AFC_F16");
+  want(p->taps >= 2 && p->taps <= 4, "taps must be 2, 3 or 4");
+  want(p->batch >= 0 && p->length >= 0 && p->width >= 1, "batch, length or width");
+  want(p->length < (int64_t)1 << 31 && p->width < (int64_t)1 << 31 && p->batch < (int64_t)1 << 31, "an axis of 2^31 or more");
+  want(p->weight != nullptr, "weight is missing");
+  if (step) want(p->length == 1 && !p->lengths && p->final_state && p->final_state == p->initial_state, "a step takes length 1, no lengths, and its state as initial_state and final_state");
+  if (p->batch == 0 || p->length == 0) return;
+  check_seq(p->x, p->batch, p->length, 0, "x");
+  if (!grad) check_seq(p->y, p->batch, p->length, 0, "y");
+  if (grad) {
+    check_seq(p->dy, p->batch, p->length, 0, "dy");
+    check_seq(p->dx, p->batch, p->length, 0, "dx");
+  }
+}
+
+// vectors of 16 bytes along the channels where every row starts on one
+bool vectors(const afc_conv_args *p, std::initializer_list<const afc_seq *> seqs, std::initializer_list<const void *> states) {
+  const int e = elem_bytes(p->dtype), v = 16 / e;
+  if (p->width % v) return false;
+  for (const afc_seq *s : seqs)
+    if ((uintptr_t)s->data % 16 || s->stride_batch % v || s->stride_length % v) return false;
+  for (const void *s : states)
+    if ((uintptr_t)s % 16) return false;
+  return true;
+}
+
+Tiling tiling(const afc_conv_args *p, int v, int run) {
+  Tiling t;
+  const int64_t lanes = ceil_div(p->width, v);
+  t.log_cx = 0;
+  while (t.log_cx < 6 && (1 << t.log_cx) < lanes) ++t.log_cx;
+  t.run = run;
+  t.tiles_c = ceil_div(lanes, 1 << t.log_cx);
+  t.tiles_l = ceil_div(p->length > 0 ? p->length : 1, (int64_t)run * (256 >> t.log_cx));
+  return t;
+}
+int64_t blocks(const afc_conv_args *p, const Tiling &t) {
+  const int64_t n = p->batch * t.tiles_l * t.tiles_c;
+  want(n < (int64_t)1 << 31, "too many blocks");
+  return n;
+}
+// positions of a gradient thread: long runs save partial rows and the K - 1 positions that neighbours both compute, short
+// ones give the chip enough threads
+Tiling grad_tiling(const afc_conv_args *p, int v) {
+  int run = 64;
+  Tiling t = tiling(p, v, run);
+  while (run > 8 && p->batch * t.tiles_l * t.tiles_c < 1024) t = tiling(p, v, run /= 2);
+  return t;
+}
+uint64_t grad_bytes(const afc_conv_args *p) {
+  uint64_t most = 0;
+  for (int v : {1, 16 / elem_bytes(p->dtype)}) {
+    const Tiling t = grad_tiling(p, v);
+    const uint64_t n = up256((uint64_t)p->batch * t.tiles_l * (p->taps + 1) * p->width * 4);
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+#define CONV_SILU(DT, V, K, ...) (p->silu ? CONV_GO(DT, V, K, true, __VA_ARGS__) : CONV_GO(DT, V, K, false, __VA_ARGS__))
+#define CONV_TAPS(DT, V, ...) \
+  (p->taps == 2 ? CONV_SILU(DT, V, 2, __VA_ARGS__) : p->taps == 3 ? CONV_SILU(DT, V, 3, __VA_ARGS__) : CONV_SILU(DT, V, 4, __VA_ARGS__))
+#define CONV_TYPES(wide, ...)                                                                              \
+  (p->dtype == AFC_F32 ? (wide ? CONV_TAPS(AFC_F32, 4, __VA_ARGS__) : CONV_TAPS(AFC_F32, 1, __VA_ARGS__))  \
+   : p->dtype == AFC_BF16 ? (wide ? CONV_TAPS(AFC_BF16, 8, __VA_ARGS__) : CONV_TAPS(AFC_BF16, 1, __VA_ARGS__)) \
+                          : (wide ? CONV_TAPS(AFC_F16, 8, __VA_ARGS__) : CONV_TAPS(AFC_F16, 1, __VA_ARGS__)))
+
+}  // namespace
+
+static void conv(const afc_conv_args *p, hipStream_t st) {
+  check(p, false, false);
+  OnDevice on(p->device);
+  if (p->batch == 0 || (p->length == 0 && !p->final_state)) return;
+  const bool wide = vectors(p, {&p->x, &p->y}, {p->initial_state, p->final_state});
+  const Tiling t = tiling(p, wide ? 16 / elem_bytes(p->dtype) : 1, kRun);
+  const dim3 grid((unsigned)blocks(p, t));
+#define CONV_GO(DT, V, K, S, ...) (k_conv<DT, V, K, S><<<grid, 256, 0, st>>>(*p, t), 0)
+  (void)CONV_TYPES(wide, 0);
+#undef CONV_GO
+  launched("k_conv");
+}
+
+static void conv_step(const afc_conv_args *p, hipStream_t st) {
+  check(p, false, true);
+  OnDevice on(p->device);
+  if (p->batch == 0) return;
+  const bool wide = vectors(p, {&p->x, &p->y}, {p->final_state});
+  const int64_t n = ceil_div(p->batch * (p->width / (wide ? 16 / elem_bytes(p->dtype) : 1)), 256);
+  want(n < (int64_t)1 << 31, "too many blocks");
+  const dim3 grid((unsigned)n);
+#define CONV_GO(DT, V, K, S, ...) (k_conv_step<DT, V, K, S><<<grid, 256, 0, st>>>(*p), 0)
+  (void)CONV_TYPES(wide, 0);
+#undef CONV_GO
+  launched("k_conv_step");
+}
+
+static void conv_grad(const afc_conv_args *p, hipStream_t st) {
+  check(p, true, false);
+  OnDevice on(p->device);
+  const bool params = p->dweight || p->dbias;
+  const bool wide = vectors(p, {&p->x, &p->dy, &p->dx}, {p->initial_state, p->dfinal_state, p->dinitial_state});
+  const Tiling t = grad_tiling(p, wide ? 16 / elem_bytes(p->dtype) : 1);
+  float *part = params ? (float *)p->workspace : nullptr;
+  const int64_t rows = p->batch * t.tiles_l;
+  if (params)
+    want(p->batch == 0 || (part && p->workspace_bytes >= grad_bytes(p) && (uintptr_t)part % 256 == 0), "workspace is missing, too small or not 256-byte aligned");
+  if (p->batch > 0) {
+    const dim3 grid((unsigned)blocks(p, t));
+#define CONV_GO(DT, V, K, S, ...) (k_conv_grad<DT, V, K, S><<<grid, 256, 0, st>>>(*p, t, part), 0)
+    (void)CONV_TYPES(wide, 0);
+#undef CONV_GO
+    launched("k_conv_grad");
+  }
+  if (params) {
+    const dim3 grid((unsigned)ceil_div((p->taps + 1) * p->width, 64));
+    k_conv_params<<<grid, 256, 0, st>>>(part, rows, p->width, p->taps, p->dweight, p->dbias);
+    launched("k_conv_params");
+  }
+}
+
+}  // namespace afc_ops
+
+extern "C" {
+int afc_conv(const afc_conv_args *args, void *hip_stream) {
+  return afc_ops::entry("afc_conv", [&] { afc_ops::conv(args, (hipStream_t)hip_stream); });
+}
+int afc_conv_step(const afc_conv_args *args, void *hip_stream) {
+  return afc_ops::entry("afc_conv_step", [&] { afc_ops::conv_step(args, (hipStream_t)hip_stream); });
+}
+int afc_conv_grad(const afc_conv_args *args, void *hip_stream) {
+  return afc_ops::entry("afc_conv_grad", [&] { afc_ops::conv_grad(args, (hipStream_t)hip_stream); });
+}
+int afc_conv_workspace(const afc_conv_args *args, uint64_t *bytes) {
+  return afc_ops::entry("afc_conv_workspace", [&] {
+    afc_ops::check(args, false, false);
+    afc_ops::want(bytes != nullptr, "null argument");
+    *bytes = afc_ops::grad_bytes(args);
+  });
+}
+}

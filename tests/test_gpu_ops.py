@@ -1,0 +1,439 @@
+"""The kernels of rlfluidcontrol_amd.ops against the operators written out in 64 bits (ops_reference)."""
+import pytest
+import torch
+
+from rlfluidcontrol_amd import ops
+from tests import ops_reference as ref
+from tests.test_ops import check_conv, check_scan, conv_case, scan_case
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def on_gpu(c, **kw):
+    return {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+
+
+# ---- convolution ----
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,L,W,K,lengths", [
+    (1, 1, 1, 2, None), (2, 1, 8, 4, None), (1, 2, 5, 3, None), (3, 3, 64, 4, [3, 0, 1]), (2, 7, 16, 2, [7, 5]), (2, 8, 24, 3, None), (1, 9, 256, 4, None),
+    (4, 64, 65, 4, [64, 63, 1, 0]), (2, 130, 520, 4, [130, 77]), (1, 257, 100, 3, None), (2, 517, 40, 4, [517, 512]), (70, 5, 8, 4, None)])
+def test_conv(dtype, B, L, W, K, lengths):
+    check_conv(conv_case(B + L + W, B, L, W, K, dtype, DEV, lengths), True)
+
+
+@pytest.mark.parametrize("silu", [True, False])
+@pytest.mark.parametrize("state,bias", [(False, True), (True, False), (False, False)])
+def test_conv_without_what_is_optional(silu, state, bias):
+    c = conv_case(3, 2, 19, 24, 4, BF16, DEV, state=state, bias=bias)
+    check_conv(c, silu)
+    check_conv(c, silu, dlast=False)
+    check_conv(c, silu, dy=False)
+
+
+def test_conv_of_no_length_and_no_rows():
+    c = conv_case(3, 2, 0, 8, 4, F32, DEV)
+    check_conv(c, True)
+    y, last = ops.causal_conv(c["x"], c["weight"], c["bias"], initial_state=c["state"], return_final_state=True)
+    assert y.shape == (2, 0, 8) and torch.equal(last, c["state"])
+    x, w = torch.zeros(0, 5, 8, device=DEV, requires_grad=True), c["weight"].clone().requires_grad_()
+    y = ops.causal_conv(x, w)
+    dw, = torch.autograd.grad(y, [w], torch.zeros_like(y))
+    assert y.shape == (0, 5, 8) and torch.equal(dw, torch.zeros_like(dw))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_conv_strides_and_alignment(dtype):
+    base = conv_case(5, 3, 21, 32, 4, dtype, DEV, [21, 4, 0])
+    flat = check_conv(base, True)
+    wide = torch.randn(3, 21, 70, device=DEV).to(dtype)
+    for cut in (slice(0, 32), slice(1, 33), slice(37, 69)):  # a slice of a projection: aligned, and starting inside a vector
+        wide[..., cut] = base["x"]
+        got = check_conv(dict(base, x=wide[..., cut]), True)
+        assert all(torch.equal(got[k], flat[k]) for k in flat)
+    got = check_conv(dict(base, x=base["x"].transpose(0, 1).contiguous().transpose(0, 1)), True)  # time-major records
+    assert all(torch.equal(got[k], flat[k]) for k in flat)
+    check_conv(dict(base, dy=torch.ones((), device=DEV, dtype=dtype).expand(3, 21, 32)), True)  # what sum() hands back
+    check_conv(dict(base, x=base["x"][:1].expand(3, 21, 32)), True)
+    check_conv(dict(base, x=base["x"][:, :1].expand(3, 21, 32)), True)
+
+
+def test_conv_ignores_what_is_behind_a_row():
+    c = conv_case(7, 3, 12, 16, 4, F32, DEV, [5, 0, 12])
+    want = check_conv(c, True)
+    for bad in (float("nan"), float("inf"), -torch.finfo(F32).max):
+        x, dy = c["x"].clone(), c["dy"].clone()
+        for t in (x, dy):
+            t[0, 5:] = bad
+            t[1] = bad
+        leaf = x.requires_grad_()
+        y, last = ops.causal_conv(leaf, c["weight"], c["bias"], True, c["state"], c["lengths"], return_final_state=True)
+        dx, = torch.autograd.grad([y, last], [leaf], [dy, c["dlast"]])
+        assert torch.equal(y, want["y"]) and torch.equal(last, want["last"]) and torch.equal(dx, want["dx"])
+    far = dict(c, lengths=torch.tensor([5, -3, 99], dtype=torch.int32, device=DEV))  # beyond either end: the nearer end
+    assert torch.equal(check_conv(dict(far, lengths=c["lengths"]), True)["y"], ops.causal_conv(c["x"], c["weight"], c["bias"], True, c["state"], far["lengths"]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,W,K", [(1, 1, 2), (3, 64, 4), (5, 37, 3), (1024, 256, 4)])
+def test_conv_step_continues_a_sequence(dtype, B, W, K):
+    c = conv_case(B + W, B, 5, W, K, dtype, DEV)
+    y, last = ops.causal_conv(c["x"], c["weight"], c["bias"], True, c["state"], return_final_state=True)
+    s = c["state"].clone()
+    wide = torch.empty(B, 5, W + 3, device=DEV, dtype=dtype)
+    wide[..., :W] = c["x"]
+    for l in range(5):
+        assert torch.equal(ops.causal_conv_step(wide[:, l, :W], s, c["weight"], c["bias"], True), y[:, l])
+    assert torch.equal(s, last)
+
+
+# ---- scan ----
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,L,W,N,G,lengths", [
+    (1, 1, 1, 1, 1, None), (2, 1, 5, 16, 1, None), (1, 2, 64, 4, 1, None), (3, 15, 17, 3, 1, [15, 0, 1]), (2, 16, 65, 16, 1, [16, 15]), (2, 17, 66, 8, 2, None),
+    (1, 33, 30, 13, 5, None), (2, 31, 12, 64, 3, [31, 17]), (1, 64, 130, 32, 1, None), (2, 50, 9, 33, 1, [1, 50]), (1, 47, 128, 16, 2, None), (3, 96, 40, 2, 4, [0, 96, 33])])
+def test_scan(dtype, B, L, W, N, G, lengths):
+    check_scan(scan_case(B + L + W + N, B, L, W, N, G, dtype, DEV, lengths), True)
+
+
+@pytest.mark.parametrize("N", list(range(1, 10)) + [12, 15, 17, 24, 31, 48, 49, 63])
+def test_scan_every_kind_of_state(N):
+    check_scan(scan_case(N, 2, 19, 20, N, 2, F32, DEV, [19, 7]), True)
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("off", [dict(D=False), dict(z=False), dict(bias=False), dict(state=False), dict(D=False, z=False, bias=False, state=False)])
+def test_scan_without_what_is_optional(softplus, off):
+    c = scan_case(3, 2, 21, 18, 5, 1, BF16, DEV, **off)
+    if not softplus:
+        c["dt"], c["dt_bias"] = c["dt"].abs() * 0.1, c["dt_bias"].abs() * 0.1 if c["dt_bias"] is not None else None
+    check_scan(c, softplus)
+    check_scan(c, softplus, dlast=False)
+    check_scan(c, softplus, dy=False)
+
+
+@pytest.mark.parametrize("B,L,W,N,G,lengths", [(1, 2999, 6, 16, 1, None), (2, 1500, 20, 4, 2, [1500, 801]), (1, 1025, 70, 8, 1, [1024]), (3, 700, 16, 64, 1, [700, 0, 699])])
+def test_scan_long(B, L, W, N, G, lengths):
+    check_scan(scan_case(L, B, L, W, N, G, F32, DEV, lengths), True)
+
+
+def test_scan_of_no_length_and_no_rows():
+    c = scan_case(3, 2, 0, 8, 4, 1, F32, DEV)
+    r = check_scan(c, True)
+    assert torch.equal(r["last"], c["state"]) and torch.equal(r["dstate"], c["dlast"]) and torch.equal(r["dA"], torch.zeros_like(c["A"]))
+    c = scan_case(3, 0, 5, 8, 4, 1, F32, DEV)
+    r = check_scan(c, True)
+    assert r["y"].shape == (0, 5, 8) and torch.equal(r["dD"], torch.zeros_like(c["D"]))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scan_strides_and_alignment(dtype):
+    base = scan_case(5, 3, 21, 64, 16, 2, dtype, DEV, [21, 4, 0])
+    flat = check_scan(base, True)
+    same = lambda got: all(torch.equal(got[k], flat[k]) for k in flat)  # noqa: E731
+    for at in (0, 1, 8):
+        proj = torch.randn(3, 21, at + 3 * 64 + 64, device=DEV).to(dtype)  # x, dt, z, B and C as slices of one projection
+        c, o = dict(base), at
+        for k in ("x", "dt", "z"):
+            proj[..., o:o + 64] = base[k]
+            c[k] = proj[..., o:o + 64]
+            o += 64
+        for k in ("B", "C"):
+            proj[..., o:o + 32] = base[k].flatten(2)
+            c[k] = proj[..., o:o + 32].unflatten(-1, (2, 16))
+            o += 32
+        assert same(check_scan(c, True))
+    major = {k: base[k].transpose(0, 1).contiguous().transpose(0, 1) for k in ("x", "dt", "z", "B", "C", "dy")}
+    assert same(check_scan(dict(base, **major), True))
+    major = {k: base[k].transpose(1, 2).contiguous().transpose(1, 2) for k in ("B", "C")}  # groups outside of the positions
+    assert same(check_scan(dict(base, **major), True))
+    check_scan(dict(base, dy=torch.ones((), device=DEV, dtype=dtype).expand(3, 21, 64)), True)
+    check_scan(dict(base, B=base["B"][:1].expand(3, 21, 2, 16), x=base["x"][:, :1].expand(3, 21, 64)), True)
+    one = scan_case(6, 3, 21, 64, 16, 1, dtype, DEV)
+    y = ops.selective_scan(one["x"], one["dt"], one["A"], one["B"][:, :, 0], one["C"][:, :, 0], softplus=True)  # no axis of groups
+    assert torch.equal(y, ops.selective_scan(one["x"], one["dt"], one["A"], one["B"], one["C"], softplus=True))
+
+
+def test_scan_ignores_what_is_behind_a_row():
+    c = scan_case(7, 3, 40, 16, 8, 1, F32, DEV, [18, 0, 40])
+    want = check_scan(c, True)
+    for bad in (float("nan"), float("inf"), -torch.finfo(F32).max):
+        leaves = {}
+        for k in ("x", "dt", "B", "C", "z", "dy"):
+            t = c[k].detach().clone()
+            t[0, 18:] = bad
+            t[1] = bad
+            leaves[k] = t.requires_grad_(k != "dy")
+        y, last = ops.selective_scan(leaves["x"], leaves["dt"], c["A"], leaves["B"], leaves["C"], c["D"], leaves["z"], c["dt_bias"], True, c["state"], c["lengths"],
+                                     return_final_state=True)
+        names = ("x", "dt", "B", "C", "z")
+        grads = torch.autograd.grad([y, last], [leaves[k] for k in names], [leaves["dy"], c["dlast"]])
+        assert torch.equal(y, want["y"]) and torch.equal(last, want["last"])
+        assert all(torch.equal(g, want["d" + k]) for k, g in zip(names, grads))
+    far = torch.tensor([18, -3, 99], dtype=torch.int32, device=DEV)
+    with torch.no_grad():
+        a, b = (ops.selective_scan(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], n, return_final_state=True)
+                for n in (far, c["lengths"]))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_scan_extreme_step_sizes():
+    """very large steps wipe the state (decay 0), very small ones keep it (decay 1): neither overflows nor loses the small one"""
+    c = scan_case(9, 2, 24, 16, 4, 1, F32, DEV, z=False)
+    c["dt"][0] = 80.0
+    c["dt"][1] = -30.0
+    c["dt_bias"].zero_()
+    check_scan(c, True)
+    d = c["dt"].clone().uniform_(-12, -4)  # softplus of these is near their exponential: relative accuracy counts
+    one = dict(c, dt=d, A=torch.zeros_like(c["A"]), B=torch.ones_like(c["B"]), C=torch.ones_like(c["C"]) / 4, D=None, x=torch.ones_like(c["x"]), state=None)
+    y = ops.selective_scan(one["x"], d, one["A"], one["B"], one["C"], softplus=True)
+    want = torch.nn.functional.softplus(d.double()).cumsum(1)
+    # each step: 8 + |v| <= 20 roundings of softplus, then 24 sums; all terms are positive
+    assert float(((y.double() - want) / want).abs().max()) < (20 + 24 + 8) * 2.0 ** -24
+
+
+def test_scan_grows_where_a_is_positive():
+    c = scan_case(10, 1, 40, 16, 4, 1, F32, DEV)
+    c["A"] = c["A"].abs() * 0.1
+    check_scan(c, True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("B,W,N,G", [(1, 1, 1, 1), (3, 64, 16, 1), (5, 37, 13, 1), (2, 30, 64, 3), (1024, 256, 16, 1), (7, 24, 8, 2), (4, 12, 3, 4)])
+def test_scan_step_continues_a_sequence(dtype, B, W, N, G):
+    c = scan_case(B + W, B, 4, W, N, G, dtype, DEV)
+    args = (c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], None)
+    r, m = ref.scan(*args), ref.scan(*args, magnitude=True)
+    k = ref.scan_bounds(r, c["x"], N, G)
+    s = c["state"].clone()
+    pad = torch.randn(B, 4, W + 5, device=DEV).to(dtype)
+    pad[..., 1:W + 1] = c["x"]
+    ys = [ops.selective_scan_step(pad[:, l, 1:W + 1], c["dt"][:, l], c["A"], c["B"][:, l], c["C"][:, l], s, c["D"], c["z"][:, l], c["dt_bias"], True) for l in range(4)]
+    assert ref.off(torch.stack(ys, 1), r["y"], m["y"], k["y"], dtype) <= 1
+    assert ref.off(s, r["last"], m["last"], k["last"], F32) <= 1
+
+
+# ---- how they are called ----
+
+def test_offsets_beyond_32_bits():
+    rows, W = 2, 16
+    far = (1 << 32) + 64  # elements between the rows
+    base = torch.zeros(far + 64 * 64, device=DEV, dtype=BF16)
+    c = scan_case(11, rows, 33, W, 8, 1, BF16, DEV)
+    for k in ("x", "dt", "z"):
+        view = base.as_strided((rows, 33, W), (far, 64, 1))
+        view.copy_(c[k])
+        want = ops.selective_scan(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True)
+        got = dict(c, **{k: view})
+        assert torch.equal(want, ops.selective_scan(got["x"], got["dt"], c["A"], c["B"], c["C"], c["D"], got["z"], c["dt_bias"], True)), k
+    view.copy_(c["x"])
+    w = torch.randn(W, 4, device=DEV)
+    assert torch.equal(ops.causal_conv(view, w), ops.causal_conv(c["x"], w))
+    steps = base.as_strided((2, 3, W), (64, far // 2, 1))  # and between the positions
+    steps.copy_(c["x"][:, :3])
+    assert torch.equal(ops.causal_conv(steps, w), ops.causal_conv(c["x"][:, :3], w))
+
+
+def test_same_results_every_time_and_on_another_stream():
+    c = scan_case(12, 3, 200, 80, 16, 1, BF16, DEV, [200, 150, 3])
+    v = conv_case(12, 3, 200, 80, 4, BF16, DEV, [200, 150, 3])
+    first, conv = check_scan(c, True), check_conv(v, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again, conv2 = check_scan(c, True), check_conv(v, True)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(first[k], again[k]) for k in first) and all(torch.equal(conv[k], conv2[k]) for k in conv)
+
+
+def block(x, p):
+    """the operators in a row, as a policy with memory runs them"""
+    u = ops.causal_conv(x, p["w"], p["b"], silu=True)
+    bc = u @ p["proj"]
+    N = p["A"].shape[1]
+    return ops.selective_scan(u, u @ p["to_dt"], p["A"], bc[..., :N], bc[..., N:], p["D"], x, p["dt_bias"], True)
+
+
+def block_params(W=48, N=16, dtype=F32):
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    p = dict(w=r(W, 4) * 0.5, b=r(W) * 0.1, proj=(r(W, 2 * N) / W ** 0.5).to(dtype), to_dt=(r(W, W) * 0.3 / W ** 0.5).to(dtype), A=-torch.rand(W, N, generator=g) * 4, D=r(W),
+             dt_bias=r(W) - 3)
+    return {k: v.to(DEV).requires_grad_() for k, v in p.items()}
+
+
+def test_a_block_of_them_against_the_plain_path():
+    p = block_params()
+    x = torch.randn(4, 37, 48, device=DEV)
+    y = block(x, p)
+    grads = torch.autograd.grad(y.square().sum(), list(p.values()))
+    norm = ops.clip_grad_norm(list(grads), 1.0)
+    host = {k: v.detach().cpu().requires_grad_() for k, v in p.items()}
+    y0 = block(x.cpu(), host)
+    g0 = list(torch.autograd.grad(y0.square().sum(), list(host.values())))
+    n0 = ops.clip_grad_norm(g0, 1.0)
+    # both sides run in 32 bits: 37 positions, sums over 48 and 148 values, products of two of them
+    assert torch.allclose(y.cpu(), y0, rtol=1e-4, atol=1e-4) and abs(float(norm) / float(n0) - 1) < 1e-4
+    assert all(float((a.cpu() - b).norm() / b.norm()) < 1e-4 for a, b in zip(grads, g0))
+
+
+def test_captured_forward_and_backward_replayed():
+    p, x = block_params(), torch.randn(2, 40, 48, device=DEV)
+    xs = [torch.randn(2, 40, 48, device=DEV) for _ in range(3)]
+
+    def step():
+        y = block(x, p)
+        grads = list(torch.autograd.grad(y, list(p.values()), torch.ones_like(y)))
+        return [y.detach(), ops.clip_grad_norm(grads, 0.5)] + grads
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    held = []
+    for graph in graphs:  # two graphs of the same work: neither uses the other's memory
+        with torch.cuda.graph(graph):
+            held.append(step())
+    for k in range(3):
+        x.copy_(xs[k])
+        want = [t.clone() for t in step()]
+        for graph, outs in zip(graphs, held):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs, want)), k
+        torch.randn(1 << 20, device=DEV).sum().item()
+    for graph in graphs:  # one after the other, nothing waits between
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held[0], held[1]))
+
+
+def test_captured_steps_advance_their_state():
+    W, N = 64, 16
+    c = scan_case(13, 8, 6, W, N, 1, F32, DEV)
+    x, dt, B, Cc, z = (c[k][:, 0].clone() for k in ("x", "dt", "B", "C", "z"))
+    s = c["state"].clone()
+    out = torch.empty(8, W, device=DEV)
+    go = lambda: out.copy_(ops.selective_scan_step(x, dt, c["A"], B, Cc, s, c["D"], z, c["dt_bias"], True))  # noqa: E731
+    go()
+    s.copy_(c["state"])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        go()
+    s.copy_(c["state"])
+    t = c["state"].clone()
+    for l in range(6):
+        for held, k in ((x, "x"), (dt, "dt"), (B, "B"), (Cc, "C"), (z, "z")):
+            held.copy_(c[k][:, l])
+        graph.replay()
+        want = ops.selective_scan_step(c["x"][:, l], c["dt"][:, l], c["A"], c["B"][:, l], c["C"][:, l], t, c["D"], c["z"][:, l], c["dt_bias"], True)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(s, t)
+
+
+def test_tensors_of_two_places_are_refused():
+    c = scan_case(1, 2, 5, 6, 4, 1, F32, DEV)
+    with pytest.raises(ValueError):
+        ops.selective_scan(c["x"], c["dt"].cpu(), c["A"], c["B"], c["C"])
+    with pytest.raises(ValueError):
+        ops.causal_conv(c["x"], torch.randn(6, 4))
+    with pytest.raises(ValueError):
+        ops.clip_grad_norm([c["x"], c["x"].cpu()], 1.0)
+
+
+def test_tensors_of_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    c = scan_case(1, 2, 20, 6, 4, 1, F32, "cuda:1")
+    check_scan(c, True)
+    assert torch.cuda.current_device() == 0
+
+
+# ---- norm and clipping ----
+
+def grads_of(sizes, dtypes, seed=0, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return [(torch.randn(s, generator=g) * scale).to(dtypes[i % len(dtypes)]).to(DEV) for i, s in enumerate(sizes)]
+
+
+@pytest.mark.parametrize("dtypes", [[F32], [BF16], [F16], [F32, BF16, F16]])
+@pytest.mark.parametrize("sizes", [[1], [0, 3], [5, 64, 1, 0, 257], [1000, 33333, 7], [70001], [3] * 250 + [100000], [300001, 2, 65536, 65537]])
+def test_clip(dtypes, sizes):
+    grads = grads_of(sizes, dtypes)
+    before = [g.clone() for g in grads]
+    want = torch.cat([g.double().cpu() for g in before]).norm()
+    tol = 2 * U24 * float(want)  # a double's rounding, then one to 32 bits (the bound of the rounding doubled)
+    norm = ops.grad_norm(grads)
+    assert norm.shape == () and norm.dtype == F32 and abs(float(norm) - float(want)) <= tol
+    for part in (0.3, 4.0):
+        limit = part * float(want)
+        for dest in (None, F32, BF16, F16):
+            mine = [b.clone() for b in before]
+            out = None if dest is None else [torch.full(b.shape, 7.0, dtype=dest, device=DEV) for b in before]
+            got = ops.clip_grad_norm(mine, limit, out=out)
+            assert abs(float(got) - float(want)) <= tol
+            scale = min(1.0, limit / (float(want) + 1e-6))
+            for b, m, o in zip(before, mine, out or mine):
+                assert out is None or torch.equal(m, b)
+                if part > 1 and o.dtype == b.dtype:
+                    assert torch.equal(o, b)
+                w = b.double() * scale  # the factor and the product round once each in 32 bits
+                err = (o.double() - w).abs() - (ref.half_step(o.dtype) * (1 + 4 * U24) + 4 * U24) * w.abs()
+                assert not err.numel() or float(err.max()) <= 2.0 ** -25
+
+
+U24 = 2.0 ** -24
+
+
+def test_clip_of_views_at_any_alignment():
+    flat = grads_of([100003], [BF16])[0]
+    cuts = [1, 2, 7, 8, 1000, 4097, 33000, 0, 61888]
+    assert sum(cuts) == 100003
+    views = list(flat.split(cuts))
+    want = float(flat.double().norm())
+    keep = flat.clone()
+    assert abs(float(ops.clip_grad_norm(views, want / 2)) - want) <= 2 * U24 * want
+    err = (flat.double() - keep.double() * 0.5).abs() - 2.0 ** -8 * (keep.double() * 0.5).abs() * 1.001
+    assert float(err.max()) <= 1e-12
+    g = torch.randn(40, 30, device=DEV).t()
+    h = g.clone()
+    ops.clip_grad_norm([h], 1.0)
+    assert torch.allclose(h, g / g.norm(), rtol=1e-6, atol=0) and h.stride() == g.stride()
+
+
+def test_clip_of_what_is_not_finite():
+    a, b = torch.tensor([1.0, float("inf")], device=DEV), torch.tensor([2.0], device=DEV)
+    assert float(ops.clip_grad_norm([a, b], 1.0)) == float("inf") and b.tolist() == [0.0] and a[0] == 0 and a[1].isnan()
+    a, b = torch.tensor([1.0, float("nan")], device=DEV), torch.tensor([2.0], device=DEV)
+    assert ops.clip_grad_norm([a, b], 1.0).isnan() and a.isnan().all() and b.isnan().all()
+    a = torch.full((1000,), 1e30, device=DEV)  # squares beyond 32 bits
+    assert abs(float(ops.clip_grad_norm([a], 1.0)) / (1e30 * 1000 ** 0.5) - 1) < 1e-6 and abs(float(a.double().norm()) - 1) < 1e-6
+    a = torch.full((1000,), 1e-30, device=DEV)
+    assert abs(float(ops.grad_norm([a])) / (1e-30 * 1000 ** 0.5) - 1) < 1e-6
+    a = torch.randn(100, device=DEV)
+    keep = a.clone()
+    ops.clip_grad_norm([a], float("inf"))
+    assert torch.equal(a, keep)
+    ops.clip_grad_norm([a], 0.0)
+    assert torch.equal(a, torch.zeros_like(a))
+
+
+def test_clip_refuses_tensors_that_overlap():
+    a = torch.ones(100, device=DEV)
+    for grads, out in (([a, a], None), ([a[:60], a[50:]], None), ([a[:50]], [a[25:75]])):
+        with pytest.raises(ops.OpsError, match="overlap"):
+            ops.clip_grad_norm(grads, 1.0, out=out)
+    assert torch.equal(a, torch.ones_like(a))
+    assert abs(float(ops.grad_norm([a, a])) - 200 ** 0.5) < 1e-5  # read only: the same tensor twice counts twice
+
+
+def test_clip_same_bits_every_time():
+    grads = grads_of([1 << 20, 12345, 7], [F32, BF16])
+    first = ops.grad_norm(grads)
+    assert all(torch.equal(ops.grad_norm(grads), first) for _ in range(5))

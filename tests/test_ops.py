@@ -1,0 +1,312 @@
+"""rlfluidcontrol_amd.ops on the CPU: the formulas against differences, the plain path against the formulas, refusals, and the
+C ABI's own checks (which refuse before any device is touched)."""
+import ctypes as C
+import os
+import re
+
+import pytest
+import torch
+
+from rlfluidcontrol_amd import build, ops
+from tests import ops_reference as ref
+from tests.conftest import ROOT
+
+
+def conv_case(seed, B, L, W, K, dtype=torch.float32, device="cpu", lengths=None, state=True, bias=True):
+    g = torch.Generator().manual_seed(seed)
+
+    def r(*s):
+        return torch.randn(*s, generator=g)
+
+    return dict(x=r(B, L, W).to(dtype).to(device), weight=(0.5 * r(W, K)).to(device), bias=(0.3 * r(W)).to(device) if bias else None,
+                state=r(B, K - 1, W).to(dtype).to(device) if state else None, dy=r(B, L, W).to(dtype).to(device), dlast=r(B, K - 1, W).to(dtype).to(device),
+                lengths=None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=device))
+
+
+def scan_case(seed, B, L, W, N, G=1, dtype=torch.float32, device="cpu", lengths=None, D=True, z=True, bias=True, state=True):
+    g = torch.Generator().manual_seed(seed)
+
+    def r(*s):
+        return torch.randn(*s, generator=g)
+
+    def to(t, on=True):
+        return t.to(dtype).to(device) if on else None
+
+    return dict(x=to(r(B, L, W)), dt=to(0.5 * r(B, L, W) - 2), A=(-torch.rand(W, N, generator=g) * 4 - 0.1).to(device), B=to(r(B, L, G, N)), C=to(r(B, L, G, N)),
+                D=(1 + 0.3 * r(W)).to(device) if D else None, z=to(r(B, L, W), z), dt_bias=(0.3 * r(W) - 1).to(device) if bias else None,
+                state=r(B, W, N).to(device) if state else None, dy=to(r(B, L, W)), dlast=r(B, W, N).to(device),
+                lengths=None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=device))
+
+
+def check_conv(c, silu, dy=True, dlast=True):
+    """forward and backward of ops.causal_conv against the reference"""
+    leaves = {k: c[k].detach().clone().requires_grad_() for k in ("x", "weight", "bias", "state") if c[k] is not None}
+    y, last = ops.causal_conv(leaves["x"], leaves["weight"], leaves.get("bias"), silu, leaves.get("state"), c["lengths"], return_final_state=True)
+    outs = [(y, c["dy"])] * dy + [(last, c["dlast"])] * dlast
+    got = torch.autograd.grad([o for o, _ in outs], list(leaves.values()), [g for _, g in outs], allow_unused=True)
+    args = (c["x"], c["weight"], c["bias"], silu, c["state"], c["lengths"], c["dy"] if dy else torch.zeros_like(c["dy"]), c["dlast"] if dlast else None)
+    r, m = ref.conv(*args), ref.conv(*args, magnitude=True)
+    k = ref.conv_bounds(m, c["x"].dtype, c["x"], c["weight"].shape[1], silu)
+    res = dict(y=y, last=last, **{"d" + n: t for n, t in zip(leaves, got)})
+    for name, t in res.items():
+        t = torch.zeros_like(leaves[name[1:]]) if t is None else t
+        assert ref.off(t, r[name], m[name], k[name], t.dtype) <= 1, name
+    return res
+
+
+def check_scan(c, softplus, dy=True, dlast=True):
+    names = [n for n in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "state") if c[n] is not None]
+    leaves = {n: c[n].detach().requires_grad_() for n in names}
+    y, last = ops.selective_scan(leaves["x"], leaves["dt"], leaves["A"], leaves["B"], leaves["C"], leaves.get("D"), leaves.get("z"), leaves.get("dt_bias"),
+                                 softplus, leaves.get("state"), c["lengths"], return_final_state=True)
+    outs = [(y, c["dy"])] * dy + [(last, c["dlast"])] * dlast
+    got = torch.autograd.grad([o for o, _ in outs], list(leaves.values()), [g for _, g in outs], allow_unused=True)
+    args = (c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], softplus, c["state"], c["lengths"],
+            c["dy"] if dy else torch.zeros_like(c["dy"]), c["dlast"] if dlast else None)
+    r, m = ref.scan(*args), ref.scan(*args, magnitude=True)
+    k = ref.scan_bounds(r, c["x"], c["A"].shape[1], c["B"].shape[2])
+    res = dict(y=y, last=last, **{"d" + ("bias" if n == "dt_bias" else "dt" if n == "dt" else n): t for n, t in zip(leaves, got)})
+    for name, t in res.items():
+        t = torch.zeros_like(leaves[name[1:]]) if t is None else t
+        assert ref.off(t, r[name], m[name], k[name], t.dtype) <= 1, name
+    # without gradients the same values come back (another kernel may have made them)
+    with torch.no_grad():
+        y2, last2 = ops.selective_scan(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], softplus, c["state"], c["lengths"],
+                                       return_final_state=True)
+    assert ref.off(y2, r["y"], m["y"], k["y"], y2.dtype) <= 1 and ref.off(last2, r["last"], m["last"], k["last"], last2.dtype) <= 1
+    return res
+
+
+# ---- the reference's gradients against differences ----
+
+def test_scan_gradients_against_differences():
+    c = scan_case(1, 2, 5, 4, 3, G=2, lengths=[5, 3])
+    c = {k: v.double() if v is not None and v.is_floating_point() else v for k, v in c.items()}
+
+    def loss(**kw):
+        a = dict(c, **kw)
+        r = ref.scan(a["x"], a["dt"], a["A"], a["B"], a["C"], a["D"], a["z"], a["dt_bias"], True, a["state"], a["lengths"])
+        return float((r["y"] * c["dy"]).sum() + (r["last"] * c["dlast"]).sum())
+
+    r = ref.scan(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], c["lengths"], c["dy"], c["dlast"])
+    g = torch.Generator().manual_seed(2)
+    for name, grad in (("x", "dx"), ("dt", "ddt"), ("A", "dA"), ("B", "dB"), ("C", "dC"), ("D", "dD"), ("z", "dz"), ("dt_bias", "dbias"), ("state", "dstate")):
+        way = torch.randn(c[name].shape, generator=g, dtype=torch.float64)
+        eps = 1e-5  # central differences: off by eps^2 f'''/6 (some 1e-9) and 2^-53 |loss| / eps (some 1e-10)
+        diff = (loss(**{name: c[name] + eps * way}) - loss(**{name: c[name] - eps * way})) / (2 * eps)
+        assert abs(diff - float((r[grad] * way).sum())) < 1e-6 * (1 + abs(diff)), name
+
+
+def test_conv_gradients_against_differences():
+    c = conv_case(1, 3, 5, 4, 3, lengths=[5, 0, 2])
+    c = {k: v.double() if v is not None and v.is_floating_point() else v for k, v in c.items()}
+
+    def loss(**kw):
+        a = dict(c, **kw)
+        r = ref.conv(a["x"], a["weight"], a["bias"], True, a["state"], a["lengths"])
+        return float((r["y"] * c["dy"]).sum() + (r["last"] * c["dlast"]).sum())
+
+    r = ref.conv(c["x"], c["weight"], c["bias"], True, c["state"], c["lengths"], c["dy"], c["dlast"])
+    g = torch.Generator().manual_seed(2)
+    for name in ("x", "weight", "bias", "state"):
+        way = torch.randn(c[name].shape, generator=g, dtype=torch.float64)
+        eps = 1e-5
+        diff = (loss(**{name: c[name] + eps * way}) - loss(**{name: c[name] - eps * way})) / (2 * eps)
+        assert abs(diff - float((r["d" + name] * way).sum())) < 1e-6 * (1 + abs(diff)), name
+
+
+# ---- the plain path ----
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [None, [7, 0, 3]])
+def test_plain_path_follows_the_formulas(dtype, lengths):
+    check_conv(conv_case(3, 3, 7, 6, 4, dtype=dtype, lengths=lengths), True)
+    check_scan(scan_case(4, 3, 7, 6, 5, G=2, dtype=dtype, lengths=lengths), True)
+
+
+def test_plain_steps_continue_a_sequence():
+    with torch.no_grad():
+        c = conv_case(5, 2, 6, 4, 4)
+        y, last = ops.causal_conv(c["x"], c["weight"], c["bias"], True, c["state"], return_final_state=True)
+        s = c["state"].clone()
+        steps = torch.stack([ops.causal_conv_step(c["x"][:, l], s, c["weight"], c["bias"], True) for l in range(6)], 1)
+        assert torch.equal(s, last) and torch.allclose(steps, y, atol=1e-6)
+        c = scan_case(6, 2, 6, 4, 5, G=2)
+        y, last = ops.selective_scan(c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], return_final_state=True)
+        s = c["state"].clone()
+        steps = torch.stack([ops.selective_scan_step(c["x"][:, l], c["dt"][:, l], c["A"], c["B"][:, l], c["C"][:, l], s, c["D"], c["z"][:, l], c["dt_bias"], True)
+                             for l in range(6)], 1)
+        assert torch.allclose(s, last, atol=1e-6) and torch.allclose(steps, y, atol=1e-6)
+
+
+def test_plain_clip():
+    grads = [torch.tensor([3.0, 0.0]), None, torch.tensor([[4.0]]).bfloat16()]
+    assert float(ops.grad_norm(grads)) == 5.0
+    assert float(ops.clip_grad_norm(grads, 10.0)) == 5.0 and grads[0].tolist() == [3.0, 0.0]
+    out = [torch.empty(2), None, torch.empty(1, 1)]
+    assert float(ops.clip_grad_norm(grads, 2.5, out=out)) == 5.0
+    assert torch.allclose(out[0], torch.tensor([1.5, 0.0]), atol=1e-6) and abs(float(out[2]) - 2.0) < 1e-6
+    assert float(ops.clip_grad_norm([], 1.0)) == 0.0
+
+
+# ---- refusals ----
+
+def refused(f, *a, error=ValueError, **kw):
+    with pytest.raises(error):
+        f(*a, **kw)
+
+
+def test_refusals_of_conv():
+    x, w = torch.randn(2, 5, 4), torch.randn(4, 3)
+    refused(ops.causal_conv, x[0], w)
+    refused(ops.causal_conv, x.double(), w)
+    refused(ops.causal_conv, x, torch.randn(4, 5))
+    refused(ops.causal_conv, x, torch.randn(4, 1))
+    refused(ops.causal_conv, x, torch.randn(5, 3))
+    refused(ops.causal_conv, x, w.bfloat16())
+    refused(ops.causal_conv, x, w, torch.randn(3))
+    refused(ops.causal_conv, x, w, initial_state=torch.randn(2, 3, 4))
+    refused(ops.causal_conv, x, w, lengths=torch.tensor([1, 2]))
+    refused(ops.causal_conv, x.transpose(1, 2).contiguous().transpose(1, 2), w)
+    refused(ops.causal_conv, x.tolist(), w, error=TypeError)
+    refused(ops.causal_conv, x, None, error=TypeError)
+    refused(ops.causal_conv_step, x[:, 0], torch.randn(2, 2, 4).transpose(0, 1).contiguous().transpose(0, 1), w)
+    refused(ops.causal_conv_step, x[:, 0], torch.randn(2, 3, 4), w)
+    refused(ops.causal_conv_step, x[:, 0], torch.randn(2, 2, 4), w.clone().requires_grad_())
+
+
+def test_refusals_of_scan():
+    c = scan_case(1, 2, 5, 6, 4, G=2)
+    ok = dict(x=c["x"], dt=c["dt"], A=c["A"], B=c["B"], C=c["C"])
+    ops.selective_scan(**ok)
+    for bad in (dict(x=c["x"][0]), dict(dt=c["dt"][:, :4]), dict(dt=c["dt"].bfloat16()), dict(A=c["A"].double()), dict(A=torch.randn(6, 65)), dict(A=torch.randn(6, 0)),
+                dict(B=torch.randn(2, 5, 4, 4), C=torch.randn(2, 5, 4, 4)), dict(C=c["C"][:, :, :1]), dict(B=torch.randn(2, 5)), dict(z=c["z"][:, :1]),
+                dict(D=torch.randn(5)), dict(dt_bias=torch.randn(6, 1)), dict(initial_state=torch.randn(2, 6, 5)), dict(initial_state=torch.randn(2, 6, 4).half()),
+                dict(lengths=torch.ones(3, dtype=torch.int32)), dict(lengths=torch.ones(2))):
+        refused(ops.selective_scan, **{**ok, **bad})
+    refused(ops.selective_scan, **{**ok, "A": 1.0}, error=TypeError)
+    step = dict(x=c["x"][:, 0], dt=c["dt"][:, 0], A=c["A"], B=c["B"][:, 0], C=c["C"][:, 0], state=c["state"])
+    ops.selective_scan_step(**step)
+    refused(ops.selective_scan_step, **{**step, "state": c["state"].transpose(1, 2).contiguous().transpose(1, 2)})
+    refused(ops.selective_scan_step, **{**step, "state": c["state"][:1]})
+    refused(ops.selective_scan_step, **{**step, "x": step["x"].clone().requires_grad_()})
+
+
+def test_refusals_of_clip():
+    g = torch.randn(4, 4)
+    refused(ops.clip_grad_norm, [g], -1.0)
+    refused(ops.clip_grad_norm, [g], float("nan"))
+    refused(ops.clip_grad_norm, g, 1.0, error=TypeError)
+    refused(ops.clip_grad_norm, [g.double()], 1.0)
+    refused(ops.clip_grad_norm, [g[:, ::2]], 1.0)
+    refused(ops.clip_grad_norm, [g[:1].expand(4, 4)], 1.0)
+    refused(ops.clip_grad_norm, [g], 1.0, out=[])
+    refused(ops.clip_grad_norm, [g], 1.0, out=[g.t().contiguous().t()])
+    refused(ops.clip_grad_norm, [g, None], 1.0, out=[None, g])
+    refused(ops.clip_grad_norm, [g, "x"], 1.0, error=TypeError)
+    refused(ops.clip_grad_norm, [g.clone().requires_grad_()], 1.0)
+    assert ops._without_gaps(g.t()) and ops._without_gaps(torch.randn(2, 3, 4, 5).permute(3, 0, 2, 1)) and not ops._without_gaps(g[:, :3])
+
+
+# ---- the C ABI ----
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build_ops()
+    return ops.load_library()
+
+
+def test_header_symbols_exported(lib):
+    txt = re.sub(r"/\*.*?\*/", "", open(os.path.join(ROOT, "include", "afc_ops.h")).read(), flags=re.S)
+    decl = sorted(set(re.findall(r"\b(afc_[a-z0-9_]+)\s*\(", txt)))
+    assert sorted(ops.ABI_SYMBOLS) == decl
+    for name in decl:
+        assert hasattr(lib, name), name
+
+
+def test_struct_layouts_follow_the_header(tmp_path):
+    import subprocess
+    src = tmp_path / "sizes.c"
+    fields = [("afc_seq", ops.Seq), ("afc_conv_args", ops.ConvArgs), ("afc_scan_args", ops.ScanArgs), ("afc_clip_args", ops.ClipArgs)]
+    lines = []
+    for name, t in fields:
+        lines.append('printf("%%zu\\n", sizeof(%s));' % name)
+        for f, _ in t._fields_:
+            lines.append('printf("%%zu\\n", offsetof(%s, %s));' % (name, "in" if f == "inp" else f))
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "afc_ops.h"\nint main(void) {%s return 0;}' % "\n".join(lines))
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(tmp_path / "sizes")])
+    got = [int(v) for v in subprocess.check_output([str(tmp_path / "sizes")], text=True).split()]
+    want = []
+    for _, t in fields:
+        want.append(C.sizeof(t))
+        want += [getattr(t, f).offset for f, _ in t._fields_]
+    assert got == want
+
+
+def fake_conv(**kw):
+    p = ops.ConvArgs()
+    p.taps, p.batch, p.length, p.width, p.weight = 3, 2, 5, 4, 4096
+    p.x = p.y = p.dy = p.dx = ops.Seq(4096, 20, 4, 0)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def fake_scan(**kw):
+    p = ops.ScanArgs()
+    p.state, p.batch, p.length, p.width, p.groups, p.a, p.checkpoints = 4, 2, 5, 4, 2, 4096, 4096
+    for k in ("x", "dt", "b", "c", "y", "dy", "dx", "ddt", "db", "dc"):
+        setattr(p, k, ops.Seq(4096, 20, 4, 4))
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def test_c_abi_refuses_bad_arguments(lib):
+    """pointers here are made up: every one of these calls is turned down on the host"""
+    def bad(f, p):
+        assert f(p if p is None else C.byref(p), None) == -1
+        assert lib.afc_ops_last_error()
+
+    big = 1 << 62
+    for f in (lib.afc_conv, lib.afc_conv_grad, lib.afc_conv_step, lib.afc_scan, lib.afc_scan_grad, lib.afc_scan_step, lib.afc_clip):
+        bad(f, None)
+    for kw in (dict(dtype=3), dict(dtype=-1), dict(taps=1), dict(taps=5), dict(batch=-1), dict(length=-1), dict(width=0), dict(weight=0), dict(length=1 << 31),
+               dict(x=ops.Seq(0, 20, 4, 0)), dict(x=ops.Seq(4096, -20, 4, 0)), dict(y=ops.Seq(4096, big, 4, 0)), dict(y=ops.Seq(0, 20, 4, 0))):
+        bad(lib.afc_conv, fake_conv(**kw))
+    for kw in (dict(dx=ops.Seq()), dict(dy=ops.Seq())):
+        bad(lib.afc_conv_grad, fake_conv(**kw))
+    for kw in (dict(length=2), dict(length=1), dict(length=1, initial_state=4096, final_state=8192), dict(length=1, initial_state=4096, final_state=4096, lengths=4096)):
+        bad(lib.afc_conv_step, fake_conv(**kw))
+    for kw in (dict(dtype=3), dict(state=0), dict(state=65), dict(groups=0), dict(groups=3), dict(width=0), dict(a=0), dict(batch=-1), dict(length=-1),
+               dict(x=ops.Seq()), dict(dt=ops.Seq()), dict(b=ops.Seq()), dict(c=ops.Seq(4096, 1, 1, big)), dict(z=ops.Seq(4096, 1, -1, 0)), dict(y=ops.Seq())):
+        bad(lib.afc_scan, fake_scan(**kw))
+    for kw in (dict(dx=ops.Seq()), dict(ddt=ops.Seq()), dict(db=ops.Seq()), dict(dc=ops.Seq()), dict(checkpoints=0), dict()):  # the last: no workspace
+        bad(lib.afc_scan_grad, fake_scan(**kw))
+    bad(lib.afc_scan_step, fake_scan(length=1))
+
+    def clip(ins, numel, outs=None, in_dtype=None, out_dtype=None, max_norm=1.0, norm=4096, ws=1 << 30, size=1 << 30, count=None):
+        n = len(ins)
+        keep = [(C.c_void_p * n)(*ins), (C.c_int64 * n)(*numel), (C.c_int32 * n)(*(in_dtype or [0] * n)), (C.c_void_p * n)(*(outs or [0] * n)),
+                (C.c_int32 * n)(*(out_dtype or [0] * n))]
+        p = ops.ClipArgs()
+        p.count, p.norm, p.workspace, p.workspace_bytes, p.max_norm = n if count is None else count, norm, ws, size, max_norm
+        p.inp, p.numel, p.in_dtype, p.out_dtype = (C.addressof(keep[k]) for k in (0, 1, 2, 4))
+        p.out = C.addressof(keep[3]) if outs else None
+        p.keep = keep
+        return p
+
+    a, b = 1 << 20, 1 << 21
+    for p in (clip([a], [4], norm=0), clip([a], [4], count=-1), clip([a], [-1]), clip([0], [4]), clip([a], [4], in_dtype=[3]), clip([a], [4], ws=0),
+              clip([a], [4], size=8), clip([a], [4], ws=(1 << 30) + 8), clip([a], [4], outs=[0]), clip([a], [4], outs=[b], out_dtype=[7]),
+              clip([a], [4], outs=[a], max_norm=-1.0), clip([a], [4], outs=[a], max_norm=float("nan")), clip([a], [4], outs=[a], out_dtype=[1]),
+              clip([a, a], [4, 4], outs=[a, a]), clip([a, a + 8], [4, 4], outs=[a, a + 8]), clip([a], [4], outs=[a + 4]), clip([a, b], [4, 4], outs=[b, a]),
+              clip([a, b], [4, 4], outs=[b + 64, b + 68])):
+        bad(lib.afc_clip, p)
+
+
+def test_no_cpu_fallback_of_the_library(lib):
+    if torch.cuda.is_available():
+        pytest.skip("GPU present")
+    assert lib.afc_conv(C.byref(fake_conv()), None) == -2 and b"no HIP device" in lib.afc_ops_last_error()
+    assert lib.afc_scan(C.byref(fake_scan()), None) == -2
