@@ -247,7 +247,7 @@ void check(const afc_conv_args *p, bool grad, bool step) {
   want(p->dtype >= AFC_F32 && p->dtype <= AFC_F16, "dtype must be AFC_F32, AFC_BF16 or AFC_F16");
   want(p->taps >= 2 && p->taps <= 4, "taps must be 2, 3 or 4");
   want(p->batch >= 0 && p->length >= 0 && p->width >= 1, "batch, length or width");
-  want(p->length < (int64_t)1 << 31 && p->width < (int64_t)1 << 31 && p->batch < (int64_t)1 << 31, "an axis of 2^31 or more");
+  want(p->length < kMostAxis && p->width < kMostAxis && p->batch < kMostAxis, "an axis of 2^30 or more");
   want(p->weight != nullptr, "weight is missing");
   if (step) want(p->length == 1 && !p->lengths && p->final_state && p->final_state == p->initial_state, "a step takes length 1, no lengths, and its state as initial_state and final_state");
   if (p->batch == 0 || p->length == 0) return;

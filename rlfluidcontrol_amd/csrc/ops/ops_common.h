@@ -65,6 +65,8 @@ int entry(const char *name, F &&f) {
   }
 }
 
+constexpr int64_t kMostAxis = (int64_t)1 << 30;  // indices along an axis, rounded up to a tile, fit 32 bits
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint64_t up256(uint64_t n) { return (n + 255) & ~(uint64_t)255; }
 
