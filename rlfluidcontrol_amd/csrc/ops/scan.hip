@@ -50,14 +50,29 @@ __device__ inline float swap_add32(float a, float b) {
   return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
 }
 
-// the sum over a channel's NL lanes, in all of them
+// The sums of four positions' values over a channel's NL lanes: a lane gets the one of position four_at<NL>(nl).  Where the
+// lanes are 16 and 32 apart a step halves the values (a lane keeps two of four, one of two), inside 16 lanes the rotations
+// leave the sum in all of them: 11 instructions for four sums whatever NL is.
 template <int NL>
-__device__ inline float sum_states(float v) {
+__device__ inline int four_at(int nl) {
+  return NL == 4 ? nl : NL == 8 ? (nl >> 2) * 2 + (nl & 1) : nl >> 2;
+}
+__device__ inline float sum_four_lanes(float v) {
   v += dpp<kRor8>(v);
-  v += dpp<kRor4>(v);
-  if (NL > 4) v = swap_add16(v, v);
-  if (NL > 8) v = swap_add32(v, v);
-  return v;
+  return v + dpp<kRor4>(v);
+}
+template <int NL>
+__device__ inline float sum_four(float v0, float v1, float v2, float v3, int nl) {
+  if (NL == 4) {
+    v0 = sum_four_lanes(v0), v1 = sum_four_lanes(v1), v2 = sum_four_lanes(v2), v3 = sum_four_lanes(v3);
+    const float lo = nl & 1 ? v1 : v0, hi = nl & 1 ? v3 : v2;
+    return nl & 2 ? hi : lo;
+  }
+  if (NL == 8) {
+    v0 = sum_four_lanes(swap_add16(v0, v2)), v1 = sum_four_lanes(swap_add16(v1, v3));
+    return nl & 1 ? v1 : v0;
+  }
+  return sum_four_lanes(swap_add16(swap_add32(v0, v2), swap_add32(v1, v3)));
 }
 
 // v[i], i < CPW: the lane of channel c gets the sum of v[c] over the wave's channels.  Each step halves the values: a lane keeps
@@ -141,6 +156,16 @@ __device__ inline void store_states(float *p, const float *h) {
   *reinterpret_cast<typename States<S>::V *>(p) = v;
 }
 
+// a thread's own place in a tensor, moved from chunk to chunk (64-bit products of strides cost more than the loads they serve)
+template <int DT>
+struct Stream {
+  Elem<DT> *p;
+  int64_t step;
+  __device__ Stream(const afc_seq &s, int64_t b, int64_t l, int64_t w) : p((Elem<DT> *)s.data + b * s.stride_batch + l * s.stride_length + w), step(K * s.stride_length) {}
+  __device__ void next() { p += step; }
+  __device__ void back() { p -= step; }
+};
+
 // where a thread is
 template <int S, int NL>
 struct Place {
@@ -174,14 +199,27 @@ struct Place {
 template <int DT, int S, int NL>
 struct Rows {
   typedef Shape<S, NL> H;
-  Elem<DT> v[H::NB];
-  __device__ inline void load(const afc_seq &s, const Place<S, NL> &at, int l0, int N) {
+  static constexpr int R = 256 / H::NP;  // positions between a thread's values
+  const Elem<DT> *p;
+  int64_t stride, step;
+  int k, n;
+  Elem<DT> v[H::NB], ahead[H::NB];
+  __device__ Rows(const afc_seq &s, const Place<S, NL> &at, int64_t l0)
+      : stride(s.stride_length * R), step(K * s.stride_length), k(threadIdx.x / H::NP), n(threadIdx.x % H::NP) {
+    p = (const Elem<DT> *)s.data + at.b * s.stride_batch + (l0 + k) * s.stride_length + at.g * s.stride_group + n;
+  }
+  __device__ void next() { p += step; }
+  __device__ void back() { p -= step; }
+  __device__ inline void load(int left, int N) {  // left: positions of the chunk within the row
 #pragma unroll
     for (int i = 0; i < H::NB; ++i) {
-      const int k = (threadIdx.x + 256 * i) / H::NP, n = (threadIdx.x + 256 * i) % H::NP, l = l0 + k;
-      v[i] = (Elem<DT>)0.f;
-      if (k < K && n < N && l < at.len) v[i] = ((const Elem<DT> *)s.data)[at.b * s.stride_batch + l * s.stride_length + at.g * s.stride_group + n];
+      ahead[i] = (Elem<DT>)0.f;
+      if (k + i * R < (left < K ? left : K) && n < N) ahead[i] = p[i * stride];
     }
+  }
+  __device__ inline void take() {
+#pragma unroll
+    for (int i = 0; i < H::NB; ++i) v[i] = ahead[i];
   }
   __device__ inline void put(float *to) const {
 #pragma unroll
@@ -190,11 +228,17 @@ struct Rows {
   }
 };
 
-template <int DT, int E, bool VEC>
-__device__ inline Piece<DT, E, VEC> piece(const afc_seq &s, int64_t b, int64_t l, int64_t w, int n) {
-  Piece<DT, E, VEC> p;
-  p.load((const Elem<DT> *)s.data + b * s.stride_batch + l * s.stride_length + w, n);
-  return p;
+// (all E of them side by side: a chain of transcendentals leaves room for three others)
+template <int E, class P>
+__device__ inline void step_sizes(float *step, const P &dt, const float *bias, bool soft, int n) {
+#pragma unroll
+  for (int i = 0; i < E; ++i) step[i] = dt[i] + bias[i];
+  if (soft) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) step[i] = softplus(step[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) step[i] = i < n ? step[i] : 0.f;
 }
 
 // decays are computed as 2^(delta A log2 e)
@@ -230,15 +274,56 @@ struct Carry {
   float *state, *steps;
 };
 
+// The S states' operands of four positions, loaded one group of positions ahead of their use
+template <int S, int NL, bool WITH_B, bool WITH_C>
+struct Operands {
+  float2 d[4];
+  float B[WITH_B ? 4 : 1][S], C[WITH_C ? 4 : 1][S];
+  __device__ inline void load(const float2 (*steps)[Shape<S, NL>::CB], const float *bs, const float *cs, int k4, const Place<S, NL> &at) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      d[k] = steps[k4 + k][at.cb];
+      if (WITH_B) load_states<S>(B[k], bs + (k4 + k) * S * NL + at.nl * S);
+      if (WITH_C) load_states<S>(C[k], cs + (k4 + k) * S * NL + at.nl * S);
+    }
+  }
+};
+
+// What reaches a part from those on its far side: h starts as what the row begins with, `from` is the part at that end.  (The
+// loads of eight parts are in flight together.)
+template <int S, int NL>
+__device__ inline void take_carries(float *h, const float *a2, const Carry &carry, int from, int parts, int way, const afc_scan_args &P, const Plan &T, const Place<S, NL> &at) {
+  if (at.cb >= at.nw) return;
+  for (int j0 = 0; j0 < parts; j0 += 8) {
+    float e[8][S], d[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t row = ((int64_t)at.b * T.segs + from + way * min(j0 + j, parts - 1)) * P.width + at.w0 + at.cb;
+      load_states<S>(e[j], carry.state + row * S * NL + at.nl * S);
+      d[j] = carry.steps[row];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const float next = __builtin_fmaf(__builtin_amdgcn_exp2f(d[j] * a2[s]), h[s], e[j][s]);
+        h[s] = j0 + j < parts ? next : h[s];
+      }
+  }
+}
+
 // ---- forwards ----
+// One barrier a chunk.  While the recurrence runs over chunk i, whose step sizes and rows lie in LDS, the same threads work out
+// the step sizes of chunk i + 1 (into the other half of LDS), finish the outputs of chunk i - 1 and have the loads of chunk
+// i + 2 in flight: the chains of the recurrence leave issue slots that the rest fills, also with a single wave on each SIMD.
 // CARRY: only the carries are computed (of all parts but the last)
 template <int DT, int S, int NL, bool VEC, bool CARRY>
 __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry carry) {
   typedef Shape<S, NL> H;
   constexpr int E = H::E;
-  __shared__ float2 steps[K][H::CB];  // delta, delta x
-  __shared__ __align__(16) float bs[K * H::NP], cs[CARRY ? 4 : K * H::NP];
-  __shared__ float ys[CARRY ? 1 : K][H::CB];
+  __shared__ float2 steps[2][K][H::CB];  // delta, delta x
+  __shared__ __align__(16) float bs[2][K * H::NP], cs[2][CARRY ? 4 : K * H::NP];
+  __shared__ float ys[2][CARRY ? 1 : K][H::CB];
   const Place<S, NL> at(P, T);
   if (CARRY && at.seg == T.segs - 1) return;
   float a2[S], h[S], total = 0.f;
@@ -248,13 +333,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
     for (int s = 0; s < S; ++s) h[s] = 0.f;
   } else {
     state_or_zero<S, NL>(h, P.initial_state, P, at);
-    if (at.cb < at.nw)
-      for (int j = 0; j < at.seg; ++j) {
-        float e[S];
-        load_states<S>(e, carry.state + (((int64_t)at.b * T.segs + j) * P.width + w) * H::NP + at.nl * S);
-        const float d = carry.steps[((int64_t)at.b * T.segs + j) * P.width + w];
-        for (int s = 0; s < S; ++s) h[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a2[s]), h[s], e[s]);
-      }
+    take_carries<S, NL>(h, a2, carry, 0, at.seg, 1, P, T, at);
   }
   float bias[E], D[E];
 #pragma unroll
@@ -263,67 +342,99 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
     D[i] = P.d && i < at.n ? P.d[at.w0 + at.q + i] : 0.f;
   }
   const int first = at.first_chunk(T), live = at.live_end(T), end = at.end_chunk(T);
-  Piece<DT, E, VEC> x{}, dt{}, z{};
-  Rows<DT, S, NL> rb, rc;
+  Piece<DT, E, VEC> x{}, dt{}, z{}, xa{}, dta{}, za{};  // of the chunk whose step sizes come next, and of the one after it
+  const int64_t l0 = (int64_t)first * K;
+  Rows<DT, S, NL> rb(P.b, at, l0), rc(P.c, at, l0);
+  Stream<DT> xs(P.x, at.b, l0 + at.r, at.w0 + at.q), dts(P.dt, at.b, l0 + at.r, at.w0 + at.q), zs(P.z, at.b, l0 + at.r, at.w0 + at.q),
+      out(P.y, at.b, l0 + at.r, at.w0 + at.q);
+  const bool gate = !CARRY && P.z.data, soft = P.softplus;
   auto fetch = [&](int ch) {
-    const int l = ch * K + at.r, n = l < at.len ? at.n : 0;
-    x = piece<DT, E, VEC>(P.x, at.b, l, at.w0 + at.q, n);
-    dt = piece<DT, E, VEC>(P.dt, at.b, l, at.w0 + at.q, n);
-    if (!CARRY && P.z.data) z = piece<DT, E, VEC>(P.z, at.b, l, at.w0 + at.q, n);
-    rb.load(P.b, at, ch * K, P.state);
-    if (!CARRY) rc.load(P.c, at, ch * K, P.state);
+    const int n = ch < live && ch * K + at.r < at.len ? at.n : 0, rows = ch < live ? at.len - ch * K : 0;
+    xa.load(xs.p, n);
+    dta.load(dts.p, n);
+    if (!CARRY) za.load(zs.p, gate ? n : 0);
+    rb.load(rows, P.state);
+    if (!CARRY) rc.load(rows, P.state);
+    xs.next(), dts.next(), zs.next(), rb.next(), rc.next();
   };
-  if (first < live) fetch(first);
-  for (int ch = first; ch < live; ++ch) {
-    const int l = ch * K + at.r;
+  auto take = [&] {
+    x = xa, dt = dta, z = za;
+    rb.take(), rc.take();
+  };
+  auto step_of = [&](int i, int ch) {
+    const float v = dt[i] + bias[i], soft_v = softplus(v);
+    return ch * K + at.r < at.len && i < at.n ? (soft ? soft_v : v) : 0.f;
+  };
+  float step[E];
+  auto put = [&](int half) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const float v = dt[i] + bias[i], step = l < at.len && i < at.n ? (P.softplus ? softplus(v) : v) : 0.f;
-      steps[at.r][at.q + i] = make_float2(step, step * x[i]);
-    }
-    rb.put(bs);
-    if (!CARRY) rc.put(cs);
-    const Piece<DT, E, VEC> x0 = x, z0 = z;
+    for (int i = 0; i < E; ++i) steps[half][at.r][at.q + i] = make_float2(step[i], step[i] * x[i]);
+    rb.put(bs[half]);
+    if (!CARRY) rc.put(cs[half]);
+  };
+  Piece<DT, E, VEC> x1{}, z1{}, x2{}, z2{};  // of the chunk in the recurrence, and of the one before it
+  float y[E];
+  auto finish = [&](int i) {
+    const float v = __builtin_fmaf(D[i], x2[i], y[i]), gated = v * silu(z2[i]);
+    y[i] = gate ? gated : v;
+  };
+  auto put_y = [&](int ch) {
+    const int l = ch * K + at.r;
+    if (l >= P.length) return;
+#pragma unroll
+    for (int i = 0; i < E; ++i) y[i] = l < at.len ? y[i] : 0.f;
+    store<DT, E, VEC>(out.p, y, at.n);
+    out.next();
+  };
+  if (first < live) {
+    fetch(first);
+    take();
+    fetch(first + 1);
+#pragma unroll
+    for (int i = 0; i < E; ++i) step[i] = step_of(i, first);
+    put(0);
+    x1 = x, z1 = z;
+    take();
     __syncthreads();
-    if (ch + 1 < live) fetch(ch + 1);
+  }
+  for (int ch = first; ch < live; ++ch) {
+    const int half = (ch - first) & 1;
+    fetch(ch + 2);
     if (!CARRY && P.checkpoints && at.cb < at.nw) store_states<S>(P.checkpoints + (((int64_t)at.b * T.chunks + ch) * P.width + w) * H::NP + at.nl * S, h);
+    if (!CARRY) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) y[i] = ys[half ^ 1][at.r][at.q + i];
+    }
+    Operands<S, NL, true, !CARRY> now, ahead;
+    ahead.load(steps[half], bs[half], cs[half], 0, at);
 #pragma unroll
     for (int k4 = 0; k4 < K; k4 += 4) {
-      float y[4];
+      now = ahead;
+      if (k4 + 4 < K) ahead.load(steps[half], bs[half], cs[half], k4 + 4, at);
+      float yk[4];
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const int k = k4 + kk;
-        const float2 d = steps[k][at.cb];
-        float B[S], C[S];
-        load_states<S>(B, bs + k * H::NP + at.nl * S);
-        if (!CARRY) load_states<S>(C, cs + k * H::NP + at.nl * S);
-        y[kk] = 0.f;
+      for (int k = 0; k < 4; ++k) {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          h[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(d.x * a2[s]), h[s], d.y * B[s]);
-          if (!CARRY) y[kk] = s ? __builtin_fmaf(C[s], h[s], y[kk]) : C[s] * h[s];
+          h[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(now.d[k].x * a2[s]), h[s], now.d[k].y * now.B[k][s]);
+          if (!CARRY) yk[k] = s ? __builtin_fmaf(now.C[k][s], h[s], yk[k]) : now.C[k][s] * h[s];
         }
-        if (CARRY)
-          total += d.x;
-        else
-          y[kk] = sum_states<NL>(y[kk]);
+        if (CARRY) total += now.d[k].x;
       }
       if (!CARRY) {
-        const float lo = at.nl & 1 ? y[1] : y[0], hi = at.nl & 1 ? y[3] : y[2];
-        if (at.nl < 4) ys[k4 + at.nl][at.cb] = at.nl & 2 ? hi : lo;
+        ys[half][k4 + four_at<NL>(at.nl)][at.cb] = sum_four<NL>(yk[0], yk[1], yk[2], yk[3], at.nl);
       }
-    }
-    __syncthreads();
-    if (!CARRY && l < P.length) {
-      float y[E];
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        y[i] = __builtin_fmaf(D[i], x0[i], ys[at.r][at.q + i]);
-        if (P.z.data) y[i] *= silu(z0[i]);
-        y[i] = l < at.len ? y[i] : 0.f;
+      for (int i = k4 / 4 * E / 4; i < (k4 / 4 + 1) * E / 4; ++i) {
+        step[i] = step_of(i, ch + 1);
+        if (!CARRY) finish(i);
       }
-      store<DT, E, VEC>((Elem<DT> *)P.y.data + at.b * P.y.stride_batch + l * P.y.stride_length + at.w0 + at.q, y, at.n);
     }
+    put(half ^ 1);
+    if (!CARRY && ch > first) put_y(ch - 1);
+    x2 = x1, z2 = z1, x1 = x, z1 = z;
+    take();
+    __syncthreads();
   }
   if (CARRY) {
     if (at.cb < at.nw) {
@@ -332,49 +443,126 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
     }
     return;
   }
-  for (int ch = live; ch < end; ++ch) {
-    const int l = ch * K + at.r;
+  if (first < live) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      y[i] = ys[(live - 1 - first) & 1][at.r][at.q + i];
+      finish(i);
+    }
+    put_y(live - 1);
+  }
+  for (int ch = live; ch < end; ++ch, out.next()) {
     const float zero[E] = {};
-    if (l < P.length) store<DT, E, VEC>((Elem<DT> *)P.y.data + at.b * P.y.stride_batch + l * P.y.stride_length + at.w0 + at.q, zero, at.n);
+    if (ch * K + at.r < P.length) store<DT, E, VEC>(out.p, zero, at.n);
   }
   if (at.seg == T.segs - 1) put_state<S, NL>(P.final_state, h, P, at);
 }
 
 // ---- backwards ----
-// sums that are finished by k_scan_finish: bc [batch, groups, tiles, length, 2, NP], a [batch, segs, width, NP], d and bias
-// [batch, segs, width]
+// sums that are finished by k_scan_bc and k_scan_params: bc [batch, groups, tiles, length, 2, NP], a [batch, segs, width, NP], d
+// and bias [batch, segs, width]
 struct Sums {
   float *bc, *a, *d, *bias;
 };
 
-// A chunk is run forwards again from its checkpoint with the states and decays of its K positions in registers, then
-// backwards.
-template <int DT, int S, int NL, bool VEC, bool CARRY>
-__global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carry carry, Sums sums) {
+// What a part hands on to the one before it, from a zero adjoint behind it (of all parts but the first)
+template <int DT, int S, int NL, bool VEC>
+__global__ __launch_bounds__(256) void k_scan_grad_carry(afc_scan_args P, Plan T, Carry carry) {
   typedef Shape<S, NL> H;
-  constexpr int E = H::E, V = 2 * S;
-  __shared__ float2 steps[K][H::CB];
-  __shared__ float dys[K][H::CB];
-  __shared__ __align__(16) float bs[CARRY ? 4 : K * H::NP], cs[K * H::NP];
-  __shared__ float ys[CARRY ? 1 : K][H::CB], dus[CARRY ? 1 : K][H::CB], tas[CARRY ? 1 : K][H::CB];
-  __shared__ float part[CARRY ? 1 : 4][CARRY ? 1 : K * 2 * H::NP];
+  constexpr int E = H::E;
+  __shared__ float2 steps[2][K][H::CB];  // delta, dy
+  __shared__ __align__(16) float cs[2][K * H::NP];
   const Place<S, NL> at(P, T);
-  if (CARRY && at.seg == 0) return;
-  float a2[S], g[S], total = 0.f;
+  if (at.seg == 0) return;
+  float a2[S], g[S] = {}, total = 0.f;
   decay_rates<S, NL>(a2, P, at);
   const int64_t w = at.w0 + at.cb;
-  if (CARRY) {
-    for (int s = 0; s < S; ++s) g[s] = 0.f;
-  } else {
-    state_or_zero<S, NL>(g, P.dfinal_state, P, at);
-    if (at.cb < at.nw)
-      for (int j = T.segs - 1; j > at.seg; --j) {
-        float e[S];
-        load_states<S>(e, carry.state + (((int64_t)at.b * T.segs + j) * P.width + w) * H::NP + at.nl * S);
-        const float d = carry.steps[((int64_t)at.b * T.segs + j) * P.width + w];
-        for (int s = 0; s < S; ++s) g[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(d * a2[s]), g[s], e[s]);
-      }
+  float bias[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) bias[i] = P.dt_bias && i < at.n ? P.dt_bias[at.w0 + at.q + i] : 0.f;
+  const int first = at.first_chunk(T), live = at.live_end(T);
+  Piece<DT, E, VEC> dt{}, z{}, dout{}, dta{}, za{}, douta{};
+  const int64_t l0 = (int64_t)(live - 1) * K;
+  Rows<DT, S, NL> rc(P.c, at, l0);
+  Stream<DT> dts(P.dt, at.b, l0 + at.r, at.w0 + at.q), zs(P.z, at.b, l0 + at.r, at.w0 + at.q), douts(P.dy, at.b, l0 + at.r, at.w0 + at.q);
+  const bool gate = P.z.data, soft = P.softplus;
+  auto fetch = [&](int ch) {
+    const int n = ch >= first && ch * K + at.r < at.len ? at.n : 0;
+    dta.load(dts.p, n);
+    za.load(zs.p, gate ? n : 0);
+    douta.load(douts.p, n);
+    rc.load(ch >= first ? at.len - ch * K : 0, P.state);
+    dts.back(), zs.back(), douts.back(), rc.back();
+  };
+  auto take = [&] {
+    dt = dta, z = za, dout = douta;
+    rc.take();
+  };
+  float step[E], dy[E];
+  auto prepare = [&](int i, int ch) {
+    const float v = dt[i] + bias[i], soft_v = softplus(v), d = dout[i], gated = d * silu(z[i]);
+    step[i] = ch * K + at.r < at.len && i < at.n ? (soft ? soft_v : v) : 0.f;
+    dy[i] = gate ? gated : d;
+  };
+  auto put = [&](int half) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) steps[half][at.r][at.q + i] = make_float2(step[i], dy[i]);
+    rc.put(cs[half]);
+  };
+  if (first < live) {
+    fetch(live - 1);
+    take();
+    fetch(live - 2);
+#pragma unroll
+    for (int i = 0; i < E; ++i) prepare(i, live - 1);
+    put(0);
+    take();
+    __syncthreads();
   }
+  for (int ch = live - 1; ch >= first; --ch) {
+    const int half = (live - 1 - ch) & 1;
+    fetch(ch - 2);
+    Operands<S, NL, false, true> now, ahead;
+    ahead.load(steps[half], nullptr, cs[half], K - 4, at);
+#pragma unroll
+    for (int k4 = K - 4; k4 >= 0; k4 -= 4) {
+      now = ahead;
+      if (k4) ahead.load(steps[half], nullptr, cs[half], k4 - 4, at);
+#pragma unroll
+      for (int k = 3; k >= 0; --k) {
+        total += now.d[k].x;
+#pragma unroll
+        for (int s = 0; s < S; ++s) g[s] = __builtin_amdgcn_exp2f(now.d[k].x * a2[s]) * __builtin_fmaf(now.d[k].y, now.C[k][s], g[s]);
+      }
+#pragma unroll
+      for (int i = k4 / 4 * E / 4; i < (k4 / 4 + 1) * E / 4; ++i) prepare(i, ch - 1);
+    }
+    put(half ^ 1);
+    take();
+    __syncthreads();
+  }
+  if (at.cb < at.nw) {
+    store_states<S>(carry.state + (((int64_t)at.b * T.segs + at.seg) * P.width + w) * H::NP + at.nl * S, g);
+    if (at.nl == 0) carry.steps[((int64_t)at.b * T.segs + at.seg) * P.width + w] = total;
+  }
+}
+
+// A chunk is run forwards again from its checkpoint with the states and decays of its K positions in registers (beside it, the
+// outputs of the chunk behind it are finished), then backwards (beside it, the chunk in front of it is prepared).
+template <int DT, int S, int NL, bool VEC>
+__global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carry carry, Sums sums) {
+  typedef Shape<S, NL> H;
+  constexpr int E = H::E, V = 2 * S, SET = H::CPW > V ? H::CPW : V, NO = (K * 2 * H::NP + 255) / 256;
+  __shared__ float2 steps[2][K][H::CB];  // delta, delta x
+  __shared__ float dys[2][K][H::CB], ys[2][K][H::CB], dus[K][H::CB], tas[K][H::CB];
+  __shared__ __align__(16) float bs[2][K * H::NP], cs[2][K * H::NP];
+  __shared__ float part[4][K * 2 * H::NP];
+  const Place<S, NL> at(P, T);
+  float a2[S], g[S];
+  decay_rates<S, NL>(a2, P, at);
+  const int64_t w = at.w0 + at.cb;
+  state_or_zero<S, NL>(g, P.dfinal_state, P, at);
+  take_carries<S, NL>(g, a2, carry, T.segs - 1, T.segs - 1 - at.seg, -1, P, T, at);
   float bias[E], D[E], sum_d[E], sum_b[E], sum_a[S];
 #pragma unroll
   for (int i = 0; i < E; ++i) {
@@ -385,165 +573,203 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
 #pragma unroll
   for (int s = 0; s < S; ++s) sum_a[s] = 0.f;
   const int first = at.first_chunk(T), live = at.live_end(T), end = at.end_chunk(T);
-  Piece<DT, E, VEC> x{}, dt{}, z{}, dout{};
-  Rows<DT, S, NL> rb, rc;
-  float h0[S];
+  const bool gate = P.z.data, soft = P.softplus;
+  Piece<DT, E, VEC> x{}, dt{}, z{}, dout{}, xa{}, dta{}, za{}, douta{};  // of the chunk that is prepared next, and of the one in front of it
+  const int64_t l0 = (int64_t)(live - 1) * K, lr = l0 + at.r, wq = at.w0 + at.q;
+  Rows<DT, S, NL> rb(P.b, at, l0), rc(P.c, at, l0);
+  Stream<DT> xs(P.x, at.b, lr, wq), dts(P.dt, at.b, lr, wq), zs(P.z, at.b, lr, wq), douts(P.dy, at.b, lr, wq), dxs(P.dx, at.b, lr, wq), ddts(P.ddt, at.b, lr, wq),
+      dzs(P.dz, at.b, lr, wq);
   auto fetch = [&](int ch) {
-    const int l = ch * K + at.r, n = l < at.len ? at.n : 0;
-    if (!CARRY) x = piece<DT, E, VEC>(P.x, at.b, l, at.w0 + at.q, n);
-    dt = piece<DT, E, VEC>(P.dt, at.b, l, at.w0 + at.q, n);
-    if (P.z.data) z = piece<DT, E, VEC>(P.z, at.b, l, at.w0 + at.q, n);
-    dout = piece<DT, E, VEC>(P.dy, at.b, l, at.w0 + at.q, n);
-    if (!CARRY) rb.load(P.b, at, ch * K, P.state);
-    rc.load(P.c, at, ch * K, P.state);
-    if (!CARRY) {
-      for (int s = 0; s < S; ++s) h0[s] = 0.f;
-      if (at.cb < at.nw) load_states<S>(h0, P.checkpoints + (((int64_t)at.b * T.chunks + ch) * P.width + w) * H::NP + at.nl * S);
-    }
+    const int n = ch >= first && ch * K + at.r < at.len ? at.n : 0, rows = ch >= first ? at.len - ch * K : 0;
+    xa.load(xs.p, n);
+    dta.load(dts.p, n);
+    za.load(zs.p, gate ? n : 0);
+    douta.load(douts.p, n);
+    rb.load(rows, P.state);
+    rc.load(rows, P.state);
+    xs.back(), dts.back(), zs.back(), douts.back(), rb.back(), rc.back();
   };
-  if (!CARRY) {  // behind the row's end
-    const float zero[E] = {};
-    for (int ch = live; ch < end; ++ch) {
-      const int l = ch * K + at.r;
-      if (l < P.length) {
-        store<DT, E, VEC>((Elem<DT> *)P.dx.data + at.b * P.dx.stride_batch + l * P.dx.stride_length + at.w0 + at.q, zero, at.n);
-        store<DT, E, VEC>((Elem<DT> *)P.ddt.data + at.b * P.ddt.stride_batch + l * P.ddt.stride_length + at.w0 + at.q, zero, at.n);
-        if (P.dz.data) store<DT, E, VEC>((Elem<DT> *)P.dz.data + at.b * P.dz.stride_batch + l * P.dz.stride_length + at.w0 + at.q, zero, at.n);
-      }
-      for (int i = threadIdx.x; i < K * 2 * H::NP; i += 256)
-        if (ch * K + i / (2 * H::NP) < P.length)
-          sums.bc[((((int64_t)at.b * P.groups + at.g) * T.tiles + at.tile) * P.length + ch * K) * 2 * H::NP + i] = 0.f;
-    }
-  }
-  if (first < live) fetch(live - 1);
-  for (int ch = live - 1; ch >= first; --ch) {
-    const int l = ch * K + at.r;
-    float delta[E], dy[E];
+  auto take = [&] {
+    x = xa, dt = dta, z = za, dout = douta;
+    rb.take(), rc.take();
+  };
+  float h[S], h0[S];
+  auto fetch_state = [&](int ch) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) h0[s] = 0.f;
+    if (ch >= first && at.cb < at.nw) load_states<S>(h0, P.checkpoints + (((int64_t)at.b * T.chunks + ch) * P.width + w) * H::NP + at.nl * S);
+  };
+  float step[E], dy[E];
+  auto prepare = [&](int i, int ch) {
+    const float v = dt[i] + bias[i], soft_v = softplus(v), d = dout[i], gated = d * silu(z[i]);
+    step[i] = ch * K + at.r < at.len && i < at.n ? (soft ? soft_v : v) : 0.f;
+    dy[i] = gate ? gated : d;
+  };
+  auto put = [&](int half) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const float v = dt[i] + bias[i];
-      delta[i] = l < at.len && i < at.n ? (P.softplus ? softplus(v) : v) : 0.f;
-      dy[i] = dout[i];
-      if (P.z.data) dy[i] *= silu(z[i]);
-      steps[at.r][at.q + i] = make_float2(delta[i], CARRY ? 0.f : delta[i] * x[i]);
-      dys[at.r][at.q + i] = dy[i];
+      steps[half][at.r][at.q + i] = make_float2(step[i], step[i] * x[i]);
+      dys[half][at.r][at.q + i] = dy[i];
     }
-    if (!CARRY) rb.put(bs);
-    rc.put(cs);
-    const Piece<DT, E, VEC> x0 = x, dt0 = dt, z0 = z, dout0 = dout;
-    float h[S];
-    if (!CARRY)
-      for (int s = 0; s < S; ++s) h[s] = h0[s];
-    __syncthreads();
-    if (ch > first) fetch(ch - 1);
-    if (CARRY) {
+    rb.put(bs[half]);
+    rc.put(cs[half]);
+  };
+  // the chunk in the recurrence, and the one behind it
+  struct Kept {
+    Piece<DT, E, VEC> x, dt, z, dout;
+    float step[E], dy[E];
+  } k1{}, k2{};
+  auto keep = [&] {
+    k2 = k1;
+    k1.x = x, k1.dt = dt, k1.z = z, k1.dout = dout;
 #pragma unroll
-      for (int k = K - 1; k >= 0; --k) {
-        const float d = steps[k][at.cb].x, dyk = dys[k][at.cb];
-        float C[S];
-        load_states<S>(C, cs + k * H::NP + at.nl * S);
-        total += d;
+    for (int i = 0; i < E; ++i) k1.step[i] = step[i], k1.dy[i] = dy[i];
+  };
+  float dx[E], ddt[E], dz[E], bc[NO];
+  auto finish = [&](int i, int half) {
+    const float du = dus[at.r][at.q + i], ta = tas[at.r][at.q + i], y = ys[half][at.r][at.q + i], xi = k2.x[i], zi = k2.z[i];
+    const float slope = sigmoid(k2.dt[i] + bias[i]), d = __builtin_fmaf(du, xi, ta * 0.693147180559945309f);
+    dx[i] = __builtin_fmaf(du, k2.step[i], D[i] * k2.dy[i]);
+    ddt[i] = soft ? slope * d : d;
+    dz[i] = k2.dout[i] * __builtin_fmaf(D[i], xi, y) * silu_slope(zi, sigmoid(zi));
+  };
+  auto finish_bc = [&] {
 #pragma unroll
-        for (int s = 0; s < S; ++s) g[s] = __builtin_amdgcn_exp2f(d * a2[s]) * __builtin_fmaf(dyk, C[s], g[s]);
+    for (int j = 0; j < NO; ++j) {
+      const int i = threadIdx.x + 256 * j;
+      bc[j] = K * 2 * H::NP >= 256 * (j + 1) || i < K * 2 * H::NP ? (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]) : 0.f;
+    }
+  };
+  const int64_t bc_tile = (((int64_t)at.b * P.groups + at.g) * T.tiles + at.tile) * P.length;
+  auto put_grads = [&](int ch) {
+    const int l = ch * K + at.r;
+#pragma unroll
+    for (int j = 0; j < NO; ++j) {
+      const int i = threadIdx.x + 256 * j;
+      if (i < K * 2 * H::NP && ch * K + i / (2 * H::NP) < P.length) sums.bc[(bc_tile + ch * K) * 2 * H::NP + i] = bc[j];
+    }
+    if (l < P.length) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const bool on = l < at.len;
+        dx[i] = on ? dx[i] : 0.f;
+        ddt[i] = on ? ddt[i] : 0.f;
+        dz[i] = on ? dz[i] : 0.f;
+        sum_d[i] = __builtin_fmaf(k2.dy[i], k2.x[i], sum_d[i]);
+        sum_b[i] += ddt[i];
       }
-      __syncthreads();
-      continue;
+      store<DT, E, VEC>(dxs.p, dx, at.n);
+      store<DT, E, VEC>(ddts.p, ddt, at.n);
+      if (P.dz.data) store<DT, E, VEC>(dzs.p, dz, at.n);
     }
+    dxs.back(), ddts.back(), dzs.back();
+  };
+  {  // behind the row's end
+    const float zero[E] = {};
+    for (int ch = live; ch < end; ++ch) {
+      dxs.next(), ddts.next(), dzs.next();
+      if (ch * K + at.r < P.length) {
+        store<DT, E, VEC>(dxs.p, zero, at.n);
+        store<DT, E, VEC>(ddts.p, zero, at.n);
+        if (P.dz.data) store<DT, E, VEC>(dzs.p, zero, at.n);
+      }
+      for (int i = threadIdx.x; i < K * 2 * H::NP; i += 256)
+        if (ch * K + i / (2 * H::NP) < P.length) sums.bc[(bc_tile + ch * K) * 2 * H::NP + i] = 0.f;
+    }
+    for (int ch = live; ch < end; ++ch) dxs.back(), ddts.back(), dzs.back();
+  }
+  if (first < live) {
+    fetch(live - 1);
+    fetch_state(live - 1);
+    take();
+    fetch(live - 2);
+#pragma unroll
+    for (int i = 0; i < E; ++i) prepare(i, live - 1);
+    put(0);
+    keep();
+    take();
+    __syncthreads();
+  }
+  for (int ch = live - 1; ch >= first; --ch) {
+    const int half = (live - 1 - ch) & 1;
+#pragma unroll
+    for (int s = 0; s < S; ++s) h[s] = h0[s];
+    fetch_state(ch - 1);
+    fetch(ch - 2);
     float before[K][S], a[K][S];
+    Operands<S, NL, true, true> now, ahead;
+    ahead.load(steps[half], bs[half], cs[half], 0, at);
+    finish_bc();
 #pragma unroll
     for (int k4 = 0; k4 < K; k4 += 4) {
+      now = ahead;
+      if (k4 + 4 < K) ahead.load(steps[half], bs[half], cs[half], k4 + 4, at);
       float y[4];
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
         const int k = k4 + kk;
-        const float2 d = steps[k][at.cb];
-        float B[S], C[S];
-        load_states<S>(B, bs + k * H::NP + at.nl * S);
-        load_states<S>(C, cs + k * H::NP + at.nl * S);
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           before[k][s] = h[s];
-          a[k][s] = __builtin_amdgcn_exp2f(d.x * a2[s]);
-          h[s] = __builtin_fmaf(a[k][s], h[s], d.y * B[s]);
-          y[kk] = s ? __builtin_fmaf(C[s], h[s], y[kk]) : C[s] * h[s];
+          a[k][s] = __builtin_amdgcn_exp2f(now.d[kk].x * a2[s]);
+          h[s] = __builtin_fmaf(a[k][s], h[s], now.d[kk].y * now.B[kk][s]);
+          y[kk] = s ? __builtin_fmaf(now.C[kk][s], h[s], y[kk]) : now.C[kk][s] * h[s];
         }
-        y[kk] = sum_states<NL>(y[kk]);
       }
-      const float lo = at.nl & 1 ? y[1] : y[0], hi = at.nl & 1 ? y[3] : y[2];
-      if (at.nl < 4) ys[k4 + at.nl][at.cb] = at.nl & 2 ? hi : lo;
+      ys[half][k4 + four_at<NL>(at.nl)][at.cb] = sum_four<NL>(y[0], y[1], y[2], y[3], at.nl);
+#pragma unroll
+      for (int i = k4 / 4 * E / 4; i < (k4 / 4 + 1) * E / 4; ++i) finish(i, half ^ 1);
     }
-    float v[H::CPW > V ? H::CPW : V];
+    if (ch < live - 1) put_grads(ch + 1);
+    __syncthreads();
+    float v[SET];
+    ahead.load(steps[half], bs[half], cs[half], K - 4, at);
 #pragma unroll
     for (int k4 = K - 4; k4 >= 0; k4 -= 4) {
+      now = ahead;
+      if (k4) ahead.load(steps[half], bs[half], cs[half], k4 - 4, at);
       float du[4], ta[4];
 #pragma unroll
       for (int kk = 3; kk >= 0; --kk) {
         const int k = k4 + kk;
-        const float2 d = steps[k][at.cb];
-        const float dyk = dys[k][at.cb];
-        float B[S], C[S];
-        load_states<S>(B, bs + k * H::NP + at.nl * S);
-        load_states<S>(C, cs + k * H::NP + at.nl * S);
-        const int o = (K - 1 - k) * V % (H::CPW > V ? H::CPW : V);
+        const float dyk = dys[half][k][at.cb];
+        const int o = (K - 1 - k) * V % SET;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          g[s] = __builtin_fmaf(dyk, C[s], g[s]);
-          v[o + s] = g[s] * d.y;
+          g[s] = __builtin_fmaf(dyk, now.C[kk][s], g[s]);
+          v[o + s] = g[s] * now.d[kk].y;
           v[o + S + s] = dyk * (k == K - 1 ? h[s] : before[k < K - 1 ? k + 1 : k][s]);
-          du[kk] = s ? __builtin_fmaf(g[s], B[s], du[kk]) : g[s] * B[s];
+          du[kk] = s ? __builtin_fmaf(g[s], now.B[kk][s], du[kk]) : g[s] * now.B[kk][s];
           g[s] *= a[k][s];
           const float t = g[s] * before[k][s];
-          sum_a[s] = __builtin_fmaf(t, d.x, sum_a[s]);
+          sum_a[s] = __builtin_fmaf(t, now.d[kk].x, sum_a[s]);
           ta[kk] = s ? __builtin_fmaf(t, a2[s], ta[kk]) : t * a2[s];
         }
-        du[kk] = sum_states<NL>(du[kk]);
-        ta[kk] = sum_states<NL>(ta[kk]);
         // the set of CPW values that is complete: value i belongs to position K - 1 - i / V of the chunk
         if (o + V >= H::CPW) {
 #pragma unroll
-          for (int m = 0; m < (H::CPW > V ? H::CPW : V); m += H::CPW) {
-            const int i = (K - 1 - k) * V + V - (H::CPW > V ? H::CPW : V) + m + at.c;
+          for (int m = 0; m < SET; m += H::CPW) {
+            const int i = (K - 1 - k) * V + V - SET + m + at.c;
             const float sum = sum_channels<NL>(v + m, at.lane);
             part[at.wave][(K - 1 - i / V) * 2 * H::NP + (i % V / S) * H::NP + at.nl * S + i % S] = sum;
           }
         }
       }
-      if (at.nl < 4) {
-        dus[k4 + at.nl][at.cb] = at.nl & 2 ? (at.nl & 1 ? du[3] : du[2]) : (at.nl & 1 ? du[1] : du[0]);
-        tas[k4 + at.nl][at.cb] = at.nl & 2 ? (at.nl & 1 ? ta[3] : ta[2]) : (at.nl & 1 ? ta[1] : ta[0]);
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < K * 2 * H::NP; i += 256)
-      if (ch * K + i / (2 * H::NP) < P.length)
-        sums.bc[((((int64_t)at.b * P.groups + at.g) * T.tiles + at.tile) * P.length + ch * K) * 2 * H::NP + i] =
-            (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]);
-    if (l < P.length) {
-      const bool on = l < at.len;
-      float dx[E], ddt[E], dz[E];
+      dus[k4 + four_at<NL>(at.nl)][at.cb] = sum_four<NL>(du[0], du[1], du[2], du[3], at.nl);
+      tas[k4 + four_at<NL>(at.nl)][at.cb] = sum_four<NL>(ta[0], ta[1], ta[2], ta[3], at.nl);
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const float du = dus[at.r][at.q + i], xi = x0[i];
-        dx[i] = on ? __builtin_fmaf(du, delta[i], D[i] * dy[i]) : 0.f;
-        ddt[i] = __builtin_fmaf(du, xi, tas[at.r][at.q + i] * 0.693147180559945309f);
-        if (P.softplus) ddt[i] *= sigmoid(dt0[i] + bias[i]);
-        ddt[i] = on ? ddt[i] : 0.f;
-        sum_d[i] = __builtin_fmaf(dy[i], xi, sum_d[i]);
-        sum_b[i] += ddt[i];
-        const float zi = z0[i];
-        dz[i] = on ? dout0[i] * __builtin_fmaf(D[i], xi, ys[at.r][at.q + i]) * silu_slope(zi, sigmoid(zi)) : 0.f;
-      }
-      store<DT, E, VEC>((Elem<DT> *)P.dx.data + at.b * P.dx.stride_batch + l * P.dx.stride_length + at.w0 + at.q, dx, at.n);
-      store<DT, E, VEC>((Elem<DT> *)P.ddt.data + at.b * P.ddt.stride_batch + l * P.ddt.stride_length + at.w0 + at.q, ddt, at.n);
-      if (P.dz.data) store<DT, E, VEC>((Elem<DT> *)P.dz.data + at.b * P.dz.stride_batch + l * P.dz.stride_length + at.w0 + at.q, dz, at.n);
+      for (int i = k4 / 4 * E / 4; i < (k4 / 4 + 1) * E / 4; ++i) prepare(i, ch - 1);
     }
+    put(half ^ 1);
+    keep();
+    take();
+    __syncthreads();
   }
-  if (CARRY) {
-    if (at.cb < at.nw) {
-      store_states<S>(carry.state + (((int64_t)at.b * T.segs + at.seg) * P.width + w) * H::NP + at.nl * S, g);
-      if (at.nl == 0) carry.steps[((int64_t)at.b * T.segs + at.seg) * P.width + w] = total;
-    }
-    return;
+  if (first < live) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) finish(i, (live - 1 - first) & 1);
+    finish_bc();
+    put_grads(first);
   }
   const int64_t row = (int64_t)at.b * T.segs + at.seg;
   if (at.cb < at.nw) store_states<S>(sums.a + (row * P.width + w) * H::NP + at.nl * S, sum_a);
@@ -673,13 +899,15 @@ void check(const afc_scan_args *p, bool grad, bool step) {
   }
 }
 
-// states of a lane and lanes of a channel: as few lanes as hold the state, four at least
+// States of a lane and lanes of a channel.  Few states a lane leave registers for two and more waves on a SIMD and make more of
+// them: a state of 16 in 8 lanes of 2, 4 of 4 and 16 of 1 takes 813, 836 and 1010 us at 8 x 2048 x 2048 bf16 forwards and
+// backwards (VALU 75 % busy at 2 waves a SIMD, 67 % at 1), and 33 us, 44 us and 30 us at 8 x 64 x 256 f32.
 struct Split {
   int s, nl;
 };
 Split split(const afc_scan_args *p) {
   const int n = p->state;
-  return n <= 4 ? Split{1, 4} : n <= 8 ? Split{2, 4} : n <= 16 ? Split{4, 4} : n <= 32 ? Split{4, 8} : Split{4, 16};
+  return n <= 4 ? Split{1, 4} : n <= 8 ? Split{1, 8} : n <= 16 ? Split{2, 8} : n <= 32 ? Split{2, 16} : Split{4, 16};
 }
 int padded(const afc_scan_args *p) { return split(p).s * split(p).nl; }
 
@@ -689,8 +917,12 @@ Plan plan(const afc_scan_args *p) {
   t.tiles = (int)ceil_div(p->width / p->groups, cb);
   t.chunks = (int)ceil_div(p->length, K);
   const int64_t blocks = p->batch * p->groups * t.tiles;
+  // Parts cost a pass of their own for the carries (two thirds of the forward pass), so they are made where rows and channels
+  // give less than two blocks for each of 256 CUs, up to four, and no shorter than 256 positions.  1 x 8191 x 2048 (64 blocks):
+  // 256 us in 4 parts, 179 in 8, 163 in 16; 8 x 2048 x 2048 (512 blocks) forwards and backwards: 813 us whole, 987 in 2 parts.
   int64_t segs = 1;
-  while (blocks * segs < 512 && t.chunks / (segs * 2) >= 8 && segs < 64) segs *= 2;
+  if (blocks < 512)
+    while (blocks * segs < 1024 && t.chunks / (segs * 2) >= 16) segs *= 2;
   t.seg_chunks = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, segs);
   t.segs = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, t.seg_chunks);
   want(blocks * t.segs < (int64_t)1 << 31, "too many blocks");
@@ -706,13 +938,13 @@ bool vectors(const afc_scan_args *p, std::initializer_list<const afc_seq *> seqs
   return true;
 }
 
-#define SCAN_SHAPE(DT, VEC, C)                       \
-  switch (p->state <= 16 ? split(p).s : split(p).nl) { \
-    case 1: SCAN_GO(DT, 1, 4, VEC, C); break;        \
-    case 2: SCAN_GO(DT, 2, 4, VEC, C); break;        \
-    case 4: SCAN_GO(DT, 4, 4, VEC, C); break;        \
-    case 8: SCAN_GO(DT, 4, 8, VEC, C); break;        \
-    default: SCAN_GO(DT, 4, 16, VEC, C); break;      \
+#define SCAN_SHAPE(DT, VEC, C)                \
+  switch (split(p).s * 100 + split(p).nl) {   \
+    case 104: SCAN_GO(DT, 1, 4, VEC, C); break;  \
+    case 108: SCAN_GO(DT, 1, 8, VEC, C); break;  \
+    case 208: SCAN_GO(DT, 2, 8, VEC, C); break;  \
+    case 216: SCAN_GO(DT, 2, 16, VEC, C); break; \
+    default: SCAN_GO(DT, 4, 16, VEC, C); break;  \
   }
 #define SCAN_VEC(DT, C)          \
   if (wide) {                    \
@@ -792,12 +1024,14 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   if (p->batch > 0) {
     const bool wide = vectors(p, {&p->x, &p->dt, &p->z, &p->dy, &p->dx, &p->ddt, &p->dz});
     const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
-#define SCAN_GO(DT, S, NL, VEC, C) k_scan_grad<DT, S, NL, VEC, C><<<grid, 256, 0, st>>>(*p, t, carry, sums)
     if (t.segs > 1) {
-      SCAN_ALL(true)
-      launched("k_scan_grad (carry)");
+#define SCAN_GO(DT, S, NL, VEC, C) k_scan_grad_carry<DT, S, NL, VEC><<<grid, 256, 0, st>>>(*p, t, carry)
+      SCAN_ALL(0)
+#undef SCAN_GO
+      launched("k_scan_grad_carry");
     }
-    SCAN_ALL(false)
+#define SCAN_GO(DT, S, NL, VEC, C) k_scan_grad<DT, S, NL, VEC><<<grid, 256, 0, st>>>(*p, t, carry, sums)
+    SCAN_ALL(0)
 #undef SCAN_GO
     launched("k_scan_grad");
     const int64_t n = ceil_div(p->batch * p->length * p->groups * 2 * padded(p), 256);
