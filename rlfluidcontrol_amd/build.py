@@ -1,7 +1,7 @@
 """Builds libafc_env.so (the environment: HIP kernels + C ABI) and libafc_ops.so (the learner's sequence and gradient
-operators) in-tree for gfx950.
+operators) with its torch binding _ops_torch.so in-tree for gfx950.
 
-    python -m rlfluidcontrol_amd.build [--force] [--ops]     (--ops: only libafc_ops.so)
+    python -m rlfluidcontrol_amd.build [--force] [--ops]     (--ops: only libafc_ops.so and its binding)
 
 hipcc cross-compiles without a GPU.  -ffp-contract=off: the reference (Java) never fuses
 multiply-add, and parity with the oracle is checked at the bit level wherever the
@@ -39,6 +39,8 @@ OPS_CSRC = os.path.join(CSRC, "ops")
 OPS_SOURCES = ["conv.hip", "scan.hip", "clip.hip"]
 OPS_STAMP = os.path.join(HERE, "build", "ops_flags.stamp")
 OPS_FLAGS = FLAGS + ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+BINDING = os.path.join(HERE, "_ops_torch.so")
+BINDING_STAMP = os.path.join(HERE, "build", "binding_flags.stamp")
 
 
 def _ops_deps():
@@ -46,13 +48,25 @@ def _ops_deps():
     return d + [os.path.join(HERE, "..", "include", f) for f in ("afc_ops.h", "afc_env.h")]
 
 
+def _binding_flags():
+    """(compile, link) flags of _ops_torch.so: host code only, against the torch that imports it"""
+    import sysconfig
+    import torch
+    inc, lib = os.path.join(os.path.dirname(torch.__file__), "include"), os.path.join(os.path.dirname(torch.__file__), "lib")
+    compile_ = ["-O2", "-std=c++17", "-fPIC", "-x", "c++", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_ops_torch",
+                "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+    for d in (inc, os.path.join(inc, "torch", "csrc", "api", "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]):
+        compile_ += ["-isystem", d]
+    return compile_, ["-L" + HERE, "-lafc_ops", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lc10", "-lc10_hip"]
+
+
 class _Library:
-    def __init__(self, path, csrc, sources, deps, flags, stamp):
-        self.path, self.csrc, self.sources, self.deps, self.flags, self.stamp = path, csrc, sources, deps, flags, stamp
+    def __init__(self, path, csrc, sources, deps, flags, stamp, link=()):
+        self.path, self.csrc, self.sources, self.deps, self.flags, self.stamp, self.link = path, csrc, sources, deps, flags, stamp, list(link)
 
     def flag_string(self):
         """the effective compile + link flags: a library built with other flags (AFC_EXTRA_FLAGS) is not reused silently"""
-        return " ".join(self.flags) + " | HIPCC=" + os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+        return " ".join(self.flags + self.link) + " | HIPCC=" + os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
     def needs_build(self):
         if not os.path.exists(self.path):
@@ -70,7 +84,7 @@ class _Library:
 
 
 ENV = _Library(LIB, CSRC, SOURCES, _deps, FLAGS, STAMP)
-OPS = _Library(OPS_LIB, OPS_CSRC, OPS_SOURCES, _ops_deps, OPS_FLAGS, OPS_STAMP)
+OPS = _Library(OPS_LIB, OPS_CSRC, OPS_SOURCES, _ops_deps, OPS_FLAGS, OPS_STAMP, ["-Wl,-soname,libafc_ops.so"])
 
 
 def needs_build():
@@ -78,13 +92,20 @@ def needs_build():
 
 
 def build(force=False, verbose=False):
-    """Both libraries; returns the environment's."""
+    """Everything; returns the environment's library."""
     build_ops(force, verbose)
     return _build(ENV, force, verbose)
 
 
 def build_ops(force=False, verbose=False):
-    return _build(OPS, force, verbose)
+    """libafc_ops.so (returned) and, where torch is, its binding"""
+    path = _build(OPS, force, verbose)
+    try:
+        flags, link = _binding_flags()
+    except ImportError:
+        return path
+    _build(_Library(BINDING, OPS_CSRC, ["binding.cpp"], _ops_deps, flags, BINDING_STAMP, link), force, verbose)
+    return path
 
 
 def _build(lib, force, verbose):
@@ -123,7 +144,7 @@ def _build(lib, force, verbose):
                     # the extra flags reach the link step too (a CPU-side -fsanitize needs its runtime there)
                     extra = os.environ.get("AFC_EXTRA_FLAGS", "").split()
                     subprocess.check_call([hipcc] + extra + ["-shared", "-fPIC", "--offload-arch=gfx950", "-o", tmp] +
-                                          [j[0] for j in jobs])
+                                          [j[0] for j in jobs] + lib.link)
                     os.replace(tmp, lib.path)
                     with open(lib.stamp, "w") as f:
                         f.write(lib.flag_string())

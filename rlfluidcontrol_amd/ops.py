@@ -15,7 +15,6 @@ Sums, states and activations are computed in float32 and rounded once at the end
 device) gives the rows' own lengths in a padded batch, clamped to 0..length: behind them nothing is read, outputs and
 gradients are zero, and the final state is the one at the row's own end.
 """
-import ctypes as C
 import os
 
 import torch
@@ -23,11 +22,7 @@ import torch
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libafc_ops.so")
 
-# every symbol include/afc_ops.h declares (tests check the library exports all of them)
-ABI_SYMBOLS = ["afc_ops_last_error", "afc_conv", "afc_conv_grad", "afc_conv_workspace", "afc_conv_step", "afc_scan", "afc_scan_grad",
-               "afc_scan_workspace", "afc_scan_step", "afc_clip", "afc_clip_workspace"]
-
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_STATE = 64
 
 
@@ -35,87 +30,26 @@ class OpsError(RuntimeError):
     pass
 
 
-class Seq(C.Structure):
-    """struct afc_seq"""
-    _fields_ = [("data", C.c_void_p), ("stride_batch", C.c_int64), ("stride_length", C.c_int64), ("stride_group", C.c_int64)]
+_gpu_module = None
 
 
-class ConvArgs(C.Structure):
-    """struct afc_conv_args"""
-    _fields_ = [("device", C.c_int32), ("dtype", C.c_int32), ("taps", C.c_int32), ("silu", C.c_int32),
-                ("batch", C.c_int64), ("length", C.c_int64), ("width", C.c_int64), ("x", Seq), ("y", Seq),
-                ("weight", C.c_void_p), ("bias", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p),
-                ("lengths", C.c_void_p), ("dy", Seq), ("dfinal_state", C.c_void_p), ("dx", Seq), ("dweight", C.c_void_p),
-                ("dbias", C.c_void_p), ("dinitial_state", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
-
-
-class ScanArgs(C.Structure):
-    """struct afc_scan_args"""
-    _fields_ = [("device", C.c_int32), ("dtype", C.c_int32), ("softplus", C.c_int32), ("state", C.c_int32),
-                ("batch", C.c_int64), ("length", C.c_int64), ("width", C.c_int64), ("groups", C.c_int64),
-                ("x", Seq), ("dt", Seq), ("b", Seq), ("c", Seq), ("z", Seq), ("y", Seq), ("a", C.c_void_p), ("d", C.c_void_p),
-                ("dt_bias", C.c_void_p), ("initial_state", C.c_void_p), ("final_state", C.c_void_p), ("lengths", C.c_void_p),
-                ("checkpoints", C.c_void_p), ("dy", Seq), ("dfinal_state", C.c_void_p), ("dx", Seq), ("ddt", Seq), ("db", Seq),
-                ("dc", Seq), ("dz", Seq), ("da", C.c_void_p), ("dd", C.c_void_p), ("ddt_bias", C.c_void_p),
-                ("dinitial_state", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
-
-
-class ClipArgs(C.Structure):
-    """struct afc_clip_args"""
-    _fields_ = [("device", C.c_int32), ("count", C.c_int32), ("inp", C.c_void_p), ("out", C.c_void_p), ("numel", C.c_void_p),
-                ("in_dtype", C.c_void_p), ("out_dtype", C.c_void_p), ("max_norm", C.c_float), ("norm", C.c_void_p),
-                ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
-
-
-_lib = None
-
-
-def load_library():
-    """Loads libafc_ops.so; raises if it has not been built."""
-    global _lib
-    if _lib is None:
+def _gpu():
+    """The torch binding of libafc_ops.so; raises if it has not been built."""
+    global _gpu_module
+    if _gpu_module is None:
         if not os.path.exists(LIB_PATH):
             raise OpsError("libafc_ops.so is missing: build it with `python -m rlfluidcontrol_amd.build`")
-        L = C.CDLL(LIB_PATH)
-        L.afc_ops_last_error.restype = C.c_char_p
-        u64 = C.POINTER(C.c_uint64)
-        for f in ("afc_conv", "afc_conv_grad", "afc_conv_step"):
-            getattr(L, f).argtypes = [C.POINTER(ConvArgs), C.c_void_p]
-        for f in ("afc_scan", "afc_scan_grad", "afc_scan_step"):
-            getattr(L, f).argtypes = [C.POINTER(ScanArgs), C.c_void_p]
-        L.afc_clip.argtypes = [C.POINTER(ClipArgs), C.c_void_p]
-        L.afc_conv_workspace.argtypes = [C.POINTER(ConvArgs), u64]
-        L.afc_scan_workspace.argtypes = [C.POINTER(ScanArgs), u64, u64, u64]
-        L.afc_clip_workspace.argtypes = [C.POINTER(ClipArgs), u64]
-        _lib = L
-    return _lib
+        from . import _ops_torch
+        _ops_torch.set_error_class(OpsError)
+        _gpu_module = _ops_torch
+    return _gpu_module
 
 
-def _ok(rc):
-    if rc != 0:
-        raise OpsError("%s (%d)" % (_lib.afc_ops_last_error().decode(), rc))
+def _on_gpu(t):
+    return isinstance(t, torch.Tensor) and t.is_cuda
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _ptr(t):
-    return t.data_ptr() if t is not None else None
-
-
-def _seq(t):
-    if t is None:
-        return Seq()
-    s = t.stride()
-    return Seq(t.data_ptr(), s[0], s[1] if len(s) > 2 else 0, s[2] if len(s) > 3 else 0)
-
-
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-
-# ---- checks of arguments ----
+# ---- checks of arguments (tensors on the CPU; csrc/ops/binding.cpp has the same for those on a GPU) ----
 
 def _refuse(ok, text, *values):
     if not ok:
@@ -146,25 +80,13 @@ def _input(x, dims):
         raise TypeError("x must be a tensor, not %s" % type(x).__name__)
     _refuse(x.dim() == dims, "x must have %d axes, it has %d", dims, x.dim())
     _refuse(x.dtype in _DTYPES, "x is %s: float32, bfloat16 or float16 is expected", x.dtype)
-    _refuse(x.device.type in ("cuda", "cpu"), "x is on %s: a GPU or the CPU is expected", x.device)
+    _refuse(x.device.type == "cpu", "x is on %s: a GPU or the CPU is expected", x.device)
     _refuse(x.shape[-1] >= 1, "x has no channels")
 
 
 def _no_grad(*tensors):
     _refuse(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
             "a step has no gradient: call it under torch.no_grad(), or the whole-sequence form")
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _last_contiguous(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
-
-
-def _dense(t):
-    return t.contiguous() if t is not None else None
 
 
 # ---- short causal convolution ----
@@ -176,18 +98,16 @@ def causal_conv(x, weight, bias=None, silu=False, initial_state=None, lengths=No
     [batch, taps-1, width] of x's type, the inputs in front of the row, oldest first (default: zeros); lengths: see the module.
     Returns y, or (y, final_state) with the last taps-1 inputs of every row.  Differentiable in x, weight, bias and
     initial_state, through y and final_state."""
+    if _on_gpu(x):
+        out = _gpu().causal_conv(x, weight, bias, silu, initial_state, lengths, return_final_state)
+        return tuple(out) if return_final_state else out[0]
     _input(x, 3)
     B, L, W = x.shape
     _sequence("x", x, x.shape, x.dtype, x.device)
     _filter(weight, bias, W, x.device)
     _optional("initial_state", initial_state, (B, weight.shape[1] - 1, W), x.dtype, x.device)
     _optional("lengths", lengths, (B,), torch.int32, x.device)
-    if x.device.type == "cpu":
-        y, last = _plain_conv(x, weight, bias, silu, initial_state, lengths)
-    elif _wants_grad(x, weight, bias, initial_state):
-        y, last = _Conv.apply(x, weight, bias, initial_state, lengths, bool(silu), bool(return_final_state))
-    else:
-        y, last = _conv(x, weight, bias, initial_state, lengths, silu, return_final_state)
+    y, last = _plain_conv(x, weight, bias, silu, initial_state, lengths)
     return (y, last) if return_final_state else y
 
 
@@ -199,82 +119,20 @@ def _filter(weight, bias, W, device):
     _optional("bias", bias, (W,), torch.float32, device)
 
 
-def _conv_args(x, weight, bias, state, lengths, silu):
-    p = ConvArgs()
-    p.device, p.dtype, p.taps, p.silu = x.device.index, _DTYPES[x.dtype], weight.shape[1], int(silu)
-    p.batch, p.length, p.width = x.shape
-    p.x, p.weight, p.bias, p.initial_state, p.lengths = _seq(x), _ptr(weight), _ptr(bias), _ptr(state), _ptr(lengths)
-    return p
-
-
-def _conv(x, weight, bias, state, lengths, silu, want_last):
-    weight, bias, state, lengths = _dense(weight), _dense(bias), _dense(state), _dense(lengths)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    last = torch.empty(x.shape[0], weight.shape[1] - 1, x.shape[2], dtype=x.dtype, device=x.device) if want_last else None
-    p = _conv_args(x, weight, bias, state, lengths, silu)
-    p.y, p.final_state = _seq(y), _ptr(last)
-    _ok(load_library().afc_conv(C.byref(p), _stream(x.device)))
-    return y, last
-
-
-class _Conv(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, state, lengths, silu, want_last):
-        y, last = _conv(x, weight, bias, state, lengths, silu, want_last)
-        ctx.save_for_backward(x, weight, bias, state, lengths)
-        ctx.silu = silu
-        ctx.set_materialize_grads(False)
-        return y, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dlast):
-        if dy is None and dlast is None:
-            return (None,) * 7
-        x, weight, bias, state, lengths = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        weight, bias, state, lengths = _dense(weight), _dense(bias), _dense(state), _dense(lengths)
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _last_contiguous(dy)
-        dlast = _dense(dlast)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dw = torch.empty_like(weight) if need[1] else None
-        db = torch.empty_like(bias) if bias is not None and need[2] else None
-        ds = torch.empty_like(state) if state is not None and need[3] else None
-        p = _conv_args(x, weight, bias, state, lengths, ctx.silu)
-        p.dy, p.dfinal_state, p.dx, p.dweight, p.dbias, p.dinitial_state = _seq(dy), _ptr(dlast), _seq(dx), _ptr(dw), _ptr(db), _ptr(ds)
-        L = load_library()
-        if need[1] or need[2]:
-            n = C.c_uint64()
-            p.y = _seq(dx)  # (sizes only)
-            _ok(L.afc_conv_workspace(C.byref(p), C.byref(n)))
-            ws = _workspace(n.value, x.device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
-        _ok(L.afc_conv_grad(C.byref(p), _stream(x.device)))
-        return dx, dw, db, ds, None, None, None
-
-
 def causal_conv_step(x, state, weight, bias=None, silu=False):
     """One position of causal_conv for every row: x [batch, width] -> y [batch, width]; state [batch, taps-1, width]
     (contiguous, x's type) moves on by x in place.  No gradient."""
+    if _on_gpu(x):
+        return _gpu().causal_conv_step(x, state, weight, bias, silu)
     _input(x, 2)
     _sequence("x", x, x.shape, x.dtype, x.device)
     _filter(weight, bias, x.shape[1], x.device)
     _tensor("state", state, (x.shape[0], weight.shape[1] - 1, x.shape[1]), x.dtype, x.device)
     _refuse(state.is_contiguous(), "state must be contiguous")
     _no_grad(x, state, weight, bias)
-    if x.device.type == "cpu":
-        y, last = _plain_conv(x[:, None], weight, bias, silu, state, None)
-        state.copy_(last)
-        return y[:, 0]
-    weight, bias = _dense(weight), _dense(bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    p = ConvArgs()
-    p.device, p.dtype, p.taps, p.silu = x.device.index, _DTYPES[x.dtype], weight.shape[1], int(silu)
-    p.batch, p.length, p.width = x.shape[0], 1, x.shape[1]
-    p.x, p.y, p.weight, p.bias = Seq(x.data_ptr(), x.stride(0), 0, 0), Seq(y.data_ptr(), y.stride(0), 0, 0), _ptr(weight), _ptr(bias)
-    p.initial_state = p.final_state = state.data_ptr()
-    _ok(load_library().afc_conv_step(C.byref(p), _stream(x.device)))
-    return y
+    y, last = _plain_conv(x[:, None], weight, bias, silu, state, None)
+    state.copy_(last)
+    return y[:, 0]
 
 
 # ---- selective scan ----
@@ -289,17 +147,15 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False,
     D, dt_bias [width] float32; initial_state [batch, width, state] float32 (default: zeros); lengths: see the module.
     Returns y, or (y, final_state).  Differentiable in everything but lengths, through y and final_state; a forward pass that
     will be differentiated also keeps states for the backward pass."""
+    if _on_gpu(x):
+        out = _gpu().selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus, initial_state, lengths, return_final_state)
+        return tuple(out) if return_final_state else out[0]
     _input(x, 3)
     Bn, L, W = x.shape
-    B4, C4, N = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
+    B, C, N = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
     _optional("initial_state", initial_state, (Bn, W, N), torch.float32, x.device)
     _optional("lengths", lengths, (Bn,), torch.int32, x.device)
-    if x.device.type == "cpu":
-        y, last = _plain_scan(x, dt, A, B4, C4, D, z, dt_bias, softplus, initial_state, lengths)
-    elif _wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
-        y, last = _Scan.apply(x, dt, A, B4, C4, D, z, dt_bias, initial_state, lengths, bool(softplus), bool(return_final_state))
-    else:
-        y, last, _ = _scan(x, dt, A, B4, C4, D, z, dt_bias, initial_state, lengths, softplus, return_final_state, False)
+    y, last = _plain_scan(x, dt, A, B, C, D, z, dt_bias, softplus, initial_state, lengths)
     return (y, last) if return_final_state else y
 
 
@@ -329,100 +185,19 @@ def _scan_inputs(x, dt, A, B, C, D, z, dt_bias):
     return B, C, N
 
 
-def _scan_args(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus):
-    p = ScanArgs()
-    p.device, p.dtype, p.softplus, p.state = x.device.index, _DTYPES[x.dtype], int(softplus), A.shape[1]
-    p.batch, p.length, p.width, p.groups = x.shape[0], x.shape[1], x.shape[2], B.shape[2]
-    p.x, p.dt, p.b, p.c, p.z = _seq(x), _seq(dt), _seq(B), _seq(C), _seq(z)
-    p.a, p.d, p.dt_bias, p.initial_state, p.lengths = _ptr(A), _ptr(D), _ptr(dt_bias), _ptr(state), _ptr(lengths)
-    return p
-
-
-def _scan_sizes(p):
-    n = (C.c_uint64 * 3)()
-    at = [C.cast(C.byref(n, 8 * k), C.POINTER(C.c_uint64)) for k in range(3)]
-    _ok(load_library().afc_scan_workspace(C.byref(p), *at))
-    return n[0], n[1], n[2]
-
-
-def _scan(x, dt, A, B, C_, D, z, dt_bias, state, lengths, softplus, want_last, keep):
-    A, D, dt_bias, state, lengths = _dense(A), _dense(D), _dense(dt_bias), _dense(state), _dense(lengths)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    last = torch.empty(x.shape[0], x.shape[2], A.shape[1], dtype=torch.float32, device=x.device) if want_last else None
-    p = _scan_args(x, dt, A, B, C_, D, z, dt_bias, state, lengths, softplus)
-    p.y, p.final_state = _seq(y), _ptr(last)
-    kept, space, _ = _scan_sizes(p)
-    points = _workspace(kept, x.device) if keep else None
-    ws = _workspace(space, x.device) if space else None
-    p.checkpoints, p.workspace, p.workspace_bytes = _ptr(points), _ptr(ws), space
-    _ok(load_library().afc_scan(C.byref(p), _stream(x.device)))
-    return y, last, points
-
-
-class _Scan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, dt, A, B, C_, D, z, dt_bias, state, lengths, softplus, want_last):
-        y, last, points = _scan(x, dt, A, B, C_, D, z, dt_bias, state, lengths, softplus, want_last, True)
-        ctx.save_for_backward(x, dt, A, B, C_, D, z, dt_bias, state, lengths)
-        ctx.points, ctx.softplus = points, softplus
-        ctx.set_materialize_grads(False)
-        return y, last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dlast):
-        if dy is None and dlast is None:
-            return (None,) * 12
-        x, dt, A, B, C_, D, z, dt_bias, state, lengths = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        A, D, dt_bias, state, lengths = _dense(A), _dense(D), _dense(dt_bias), _dense(state), _dense(lengths)
-
-        def like(t, wanted=True):
-            return torch.empty(t.shape, dtype=t.dtype, device=t.device) if t is not None and wanted else None
-
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else _last_contiguous(dy)
-        dlast = _dense(dlast)
-        dx, ddt, dB, dC, dz = like(x), like(dt), like(B), like(C_), like(z, need[6])
-        dA, dD, dbias, dstate = like(A, need[2]), like(D, need[5]), like(dt_bias, need[7]), like(state, need[8])
-        p = _scan_args(x, dt, A, B, C_, D, z, dt_bias, state, lengths, ctx.softplus)
-        p.checkpoints, p.dy, p.dfinal_state = _ptr(ctx.points), _seq(dy), _ptr(dlast)
-        p.dx, p.ddt, p.db, p.dc, p.dz = _seq(dx), _seq(ddt), _seq(dB), _seq(dC), _seq(dz)
-        p.da, p.dd, p.ddt_bias, p.dinitial_state = _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dstate)
-        space = _scan_sizes(p)[2]
-        ws = _workspace(space, x.device)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), space
-        _ok(load_library().afc_scan_grad(C.byref(p), _stream(x.device)))
-        return dx, ddt, dA, dB, dC, dD, dz, dbias, dstate, None, None, None
-
-
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, softplus=False):
     """One position of selective_scan for every row: x, dt, z [batch, width], B, C [batch, state] or [batch, groups, state]
     -> y [batch, width]; state [batch, width, state] (contiguous, float32) moves on in place.  No gradient."""
+    if _on_gpu(x):
+        return _gpu().selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, softplus)
     _input(x, 2)
     B, C, N = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
     _tensor("state", state, (x.shape[0], x.shape[1], N), torch.float32, x.device)
     _refuse(state.is_contiguous(), "state must be contiguous")
     _no_grad(x, dt, A, B, C, state, D, z, dt_bias)
-    if x.device.type == "cpu":
-        y, last = _plain_scan(x[:, None], dt[:, None], A, B[:, None], C[:, None], D, z[:, None] if z is not None else None, dt_bias,
-                              softplus, state, None)
-        state.copy_(last)
-        return y[:, 0]
-    return _scan_step(x, dt, _dense(A), B, C, state, _dense(D), z, _dense(dt_bias), softplus)
-
-
-def _scan_step(x, dt, A, B, C_, state, D, z, dt_bias, softplus):
-    def one(t):
-        return Seq(t.data_ptr(), t.stride(0), 0, t.stride(1) if t.dim() > 2 else 0) if t is not None else Seq()
-
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    p = ScanArgs()
-    p.device, p.dtype, p.softplus, p.state = x.device.index, _DTYPES[x.dtype], int(softplus), A.shape[1]
-    p.batch, p.length, p.width, p.groups = x.shape[0], 1, x.shape[1], B.shape[1]
-    p.x, p.dt, p.b, p.c, p.z, p.y = one(x), one(dt), one(B), one(C_), one(z), one(y)
-    p.a, p.d, p.dt_bias, p.initial_state, p.final_state = _ptr(A), _ptr(D), _ptr(dt_bias), state.data_ptr(), state.data_ptr()
-    _ok(load_library().afc_scan_step(C.byref(p), _stream(x.device)))
-    return y
+    y, last = _plain_scan(x[:, None], dt[:, None], A, B[:, None], C[:, None], D, z[:, None] if z is not None else None, dt_bias, softplus, state, None)
+    state.copy_(last)
+    return y[:, 0]
 
 
 # ---- global gradient norm ----
@@ -469,36 +244,19 @@ def _clip(grads, max_norm, out):
     grads = [g for g in grads if g is not None]
     if not grads:
         return torch.zeros(())
-    dev = grads[0].device
+    if _on_gpu(grads[0]):
+        return _gpu().clip(grads, -1.0 if max_norm is None else max_norm, out)
     for g in grads + (out or []):
         if not isinstance(g, torch.Tensor):
             raise TypeError("gradients must be tensors, not %s" % type(g).__name__)
         _refuse(g.dtype in _DTYPES, "a gradient is %s: float32, bfloat16 or float16 is expected", g.dtype)
-        _refuse(g.device == dev, "gradients on %s and on %s", dev, g.device)
+        _refuse(g.device.type == "cpu" and g.device == grads[0].device, "gradients on %s and on %s", grads[0].device, g.device)
         _refuse(g.layout == torch.strided and _without_gaps(g), "a gradient has gaps or repeated elements in memory")
         _refuse(not (torch.is_grad_enabled() and g.requires_grad and max_norm is not None), "a gradient to be scaled requires a gradient itself")
     for g, o in zip(grads, out or ()):
         _refuse(g.shape == o.shape and g.stride() == o.stride(), "an output has shape %s and strides %s, its gradient %s and %s",
                 tuple(o.shape), o.stride(), tuple(g.shape), g.stride())
-    _refuse(dev.type in ("cuda", "cpu"), "gradients are on %s: a GPU or the CPU is expected", dev)
-    if dev.type == "cpu":
-        return _plain_clip(grads, max_norm, out)
-    n = len(grads)
-    codes = (C.c_int32 * n)(*[_DTYPES[g.dtype] for g in grads])
-    ins, numel = (C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads])
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    p = ClipArgs()
-    p.device, p.count, p.norm = dev.index, n, norm.data_ptr()
-    p.inp, p.numel, p.in_dtype = C.addressof(ins), C.addressof(numel), C.addressof(codes)
-    if max_norm is not None:
-        outs, out_codes = (ins, codes) if out is None else ((C.c_void_p * n)(*[o.data_ptr() for o in out]), (C.c_int32 * n)(*[_DTYPES[o.dtype] for o in out]))
-        p.out, p.out_dtype, p.max_norm = C.addressof(outs), C.addressof(out_codes), max_norm
-    L, size = load_library(), C.c_uint64()
-    _ok(L.afc_clip_workspace(C.byref(p), C.byref(size)))
-    ws = _workspace(size.value, dev)
-    p.workspace, p.workspace_bytes = ws.data_ptr(), size.value
-    _ok(L.afc_clip(C.byref(p), _stream(dev)))
-    return norm
+    return _plain_clip(grads, max_norm, out)
 
 
 # ---- the same formulas in plain torch, for tensors on the CPU ----

@@ -4,15 +4,29 @@ import torch
 
 from rlfluidcontrol_amd import ops
 from tests import ops_reference as ref
-from tests.test_ops import check_conv, check_scan, conv_case, scan_case
+from tests.test_ops import check_conv, check_scan, conv_case, refusals_of_clip, refusals_of_conv, refusals_of_scan, scan_case
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
-def on_gpu(c, **kw):
-    return {k: v.to(DEV) if isinstance(v, torch.Tensor) else v for k, v in c.items()}
+# ---- refusals ----
+
+@pytest.mark.parametrize("which", [refusals_of_conv, refusals_of_scan, refusals_of_clip])
+def test_refusals(which):
+    which(DEV)
+
+
+def test_no_gradient_of_a_gradient():
+    c = conv_case(1, 1, 4, 8, 2, F32, DEV)
+    x = c["x"].requires_grad_()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(ops.causal_conv(x, c["weight"]).sum(), [x], create_graph=True)
+    y = ops.causal_conv(x, c["weight"]).sum()
+    y.backward()
+    with pytest.raises(RuntimeError):  # what the first pass has used is gone
+        y.backward()
 
 
 # ---- convolution ----
@@ -352,6 +366,8 @@ def test_tensors_of_another_device_than_the_current_one():
         pytest.skip("one GPU")
     c = scan_case(1, 2, 20, 6, 4, 1, F32, "cuda:1")
     check_scan(c, True)
+    check_conv(conv_case(1, 2, 20, 8, 4, F32, "cuda:1"), True)
+    ops.clip_grad_norm([c["x"]], 1.0)
     assert torch.cuda.current_device() == 0
 
 
