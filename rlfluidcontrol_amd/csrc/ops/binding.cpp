@@ -98,7 +98,6 @@ Tensor fresh(const Tensor &like) { return at::empty(like.sizes(), like.options()
 Tensor fresh_if(const Tensor &like, bool wanted) { return like.defined() && wanted ? fresh(like) : Tensor(); }
 Tensor space(const Tensor &x, uint64_t bytes) { return at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)); }
 Tensor value(const Maybe &t) { return t ? *t : Tensor(); }
-Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
 
 void first_order_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "the gradients of these operators have no gradient of their own (create_graph=True)");

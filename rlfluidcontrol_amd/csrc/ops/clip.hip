@@ -19,7 +19,6 @@ int fail(int code, const std::string &msg) {
 // The tables of pointers travel in the kernel arguments (at most 4 KB): no copy that would have to outlive the call, and a
 // captured launch carries its own.
 constexpr int kTensors = 110;
-constexpr int64_t kChunk = 32768;  // elements of a block
 
 struct Batch {
   const void *in[kTensors];
@@ -28,21 +27,9 @@ struct Batch {
   int32_t first[kTensors + 1];  // the batch's first block of each tensor
   uint8_t in_dtype[kTensors], out_dtype[kTensors];
   int32_t count;
+  int64_t chunk;  // elements of a block
 };
 
-__device__ inline float load(const void *p, int dtype, int64_t i) {
-  if (dtype == AFC_F32) return ((const float *)p)[i];
-  if (dtype == AFC_BF16) return (float)((const __bf16 *)p)[i];
-  return (float)((const _Float16 *)p)[i];
-}
-__device__ inline void store(void *p, int dtype, int64_t i, float v) {
-  if (dtype == AFC_F32)
-    ((float *)p)[i] = v;
-  else if (dtype == AFC_BF16)
-    ((__bf16 *)p)[i] = (__bf16)v;
-  else
-    ((_Float16 *)p)[i] = (_Float16)v;
-}
 __device__ inline int tensor_of(const Batch &T, int block) {
   int lo = 0, hi = T.count;
   while (hi - lo > 1) {
@@ -52,45 +39,130 @@ __device__ inline int tensor_of(const Batch &T, int block) {
   return lo;
 }
 
+// V elements at once (16 bytes of the wider type) from any place: the memory pipeline takes accesses that start inside 16 bytes (a
+// tensor may be a slice of a flat buffer), and the compiler is told no more than the element's own alignment.
+template <int DT, int V>
+struct VecT {
+  typedef Elem<DT> type __attribute__((ext_vector_type(V), aligned(sizeof(Elem<DT>))));
+};
+template <int DT, int V>
+using Vec = typename VecT<DT, V>::type;
+
 __device__ inline double block_sum(double a, double *red) {
   for (int m = 32; m; m >>= 1) a += __shfl_xor(a, m);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  a = 0;
+  for (unsigned i = 0; i < blockDim.x / 64; ++i) a += red[i];
+  return a;
 }
 
+template <int DT>
+__device__ double squares(const Elem<DT> *p, int64_t n) {
+  constexpr int V = 16 / sizeof(Elem<DT>);
+  double a[4] = {};
+  const int64_t body = n / V;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < body; i += 256) {
+    const Vec<DT, V> v = *reinterpret_cast<const Vec<DT, V> *>(p + i * V);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const double d = (double)(float)v[k];
+      a[k & 3] = __builtin_fma(d, d, a[k & 3]);
+    }
+  }
+  for (int64_t i = body * V + threadIdx.x; i < n; i += 256) {
+    const double d = (double)(float)p[i];
+    a[0] = __builtin_fma(d, d, a[0]);
+  }
+  return (a[0] + a[1]) + (a[2] + a[3]);
+}
+
+// One partial sum for each block.  Double costs nothing beside the loads (a conversion and a multiply-add for each element).
 __global__ __launch_bounds__(256) void k_squares(Batch T, double *part) {
   __shared__ double red[4];
-  const int t = tensor_of(T, blockIdx.x);
-  const int64_t from = (int64_t)(blockIdx.x - T.first[t]) * kChunk, to = min(from + kChunk, T.numel[t]);
-  double a = 0;
-  for (int64_t i = from + threadIdx.x; i < to; i += 256) {
-    const double v = load(T.in[t], T.in_dtype[t], i);
-    a = __builtin_fma(v, v, a);
-  }
+  const int t = tensor_of(T, blockIdx.x), dt = T.in_dtype[t];
+  const int64_t from = (int64_t)(blockIdx.x - T.first[t]) * T.chunk, n = min(T.chunk, T.numel[t] - from);
+  double a;
+  if (dt == AFC_F32)
+    a = squares<AFC_F32>((const float *)T.in[t] + from, n);
+  else if (dt == AFC_BF16)
+    a = squares<AFC_BF16>((const __bf16 *)T.in[t] + from, n);
+  else
+    a = squares<AFC_F16>((const _Float16 *)T.in[t] + from, n);
   a = block_sum(a, red);
   if (threadIdx.x == 0) part[blockIdx.x] = a;
 }
 
-// coef[0] = what the gradients are multiplied with
-__global__ __launch_bounds__(256) void k_norm(const double *part, int64_t n, float max_norm, float *norm, float *coef) {
-  __shared__ double red[4];
+// the norm from the partial sums, in their order, and what the gradients are multiplied with
+__device__ inline double norm_of(const double *part, int64_t n, double *red) {
   double a = 0;
-  for (int64_t i = threadIdx.x; i < n; i += 256) a += part[i];
-  a = sqrt(block_sum(a, red));
-  if (threadIdx.x) return;
-  *norm = (float)a;
-  const float c = (float)((double)max_norm / (a + 1e-6));
-  *coef = c > 1.f ? 1.f : c;  // (a NaN stays one)
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) a += part[i];
+  return sqrt(block_sum(a, red));
+}
+__device__ inline float factor(double norm, float max_norm) {
+  const float c = (float)((double)max_norm / (norm + 1e-6));
+  return c > 1.f ? 1.f : c;  // (a NaN stays one)
 }
 
-__global__ __launch_bounds__(256) void k_scale(Batch T, const float *coef) {
-  const int t = tensor_of(T, blockIdx.x);
-  const int64_t from = (int64_t)(blockIdx.x - T.first[t]) * kChunk, to = min(from + kChunk, T.numel[t]);
-  const float c = *coef;
+__global__ __launch_bounds__(1024) void k_norm(const double *part, int64_t n, float max_norm, float *norm, float *coef) {
+  __shared__ double red[16];
+  const double a = norm_of(part, n, red);
+  if (threadIdx.x) return;
+  *norm = (float)a;
+  *coef = factor(a, max_norm);
+}
+
+template <int DI, int DO>
+__device__ void scale(const Elem<DI> *p, Elem<DO> *o, int64_t n, float c) {
+  constexpr int V = DI == AFC_F32 || DO == AFC_F32 ? 4 : 8;
+  const int64_t body = n / V;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < body; i += 256) {
+    const Vec<DI, V> v = *reinterpret_cast<const Vec<DI, V> *>(p + i * V);
+    Vec<DO, V> r;
+#pragma unroll
+    for (int k = 0; k < V; ++k) r[k] = (Elem<DO>)(c * (float)v[k]);
+    *reinterpret_cast<Vec<DO, V> *>(o + i * V) = r;
+  }
+  for (int64_t i = body * V + threadIdx.x; i < n; i += 256) o[i] = (Elem<DO>)(c * (float)p[i]);
+}
+template <int DI>
+__device__ void scale_to(const void *in, void *out, int dt, int64_t from, int64_t n, float c) {
+  const Elem<DI> *p = (const Elem<DI> *)in + from;
+  if (dt == AFC_F32)
+    scale<DI, AFC_F32>(p, (float *)out + from, n, c);
+  else if (dt == AFC_BF16)
+    scale<DI, AFC_BF16>(p, (__bf16 *)out + from, n, c);
+  else
+    scale<DI, AFC_F16>(p, (_Float16 *)out + from, n, c);
+}
+
+// Blocks go backwards over the tensors: what k_squares has read last is still in the last-level cache.  FEW: the partial sums are
+// few enough for every block to add them up by itself, which saves k_norm's launch.
+template <bool FEW>
+__global__ __launch_bounds__(256) void k_scale(Batch T, const float *coef, const double *part, int64_t n_part, float max_norm, float *norm) {
+  __shared__ double red[4];
+    const int block = gridDim.x - 1 - blockIdx.x;
+  float c;
+  if (FEW) {
+    const double a = norm_of(part, n_part, red);
+    c = factor(a, max_norm);
+    if (norm && block == 0 && threadIdx.x == 0) *norm = (float)a;
+  } else {
+    c = *coef;
+  }
+  const int t = tensor_of(T, block), di = T.in_dtype[t], dt = T.out_dtype[t];
   if (c == 1.f && T.in[t] == T.out[t]) return;
-  for (int64_t i = from + threadIdx.x; i < to; i += 256) store(T.out[t], T.out_dtype[t], i, c * load(T.in[t], T.in_dtype[t], i));
+  const int64_t from = (int64_t)(block - T.first[t]) * T.chunk, n = min(T.chunk, T.numel[t] - from);
+  if (di == AFC_F32)
+    scale_to<AFC_F32>(T.in[t], T.out[t], dt, from, n, c);
+  else if (di == AFC_BF16)
+    scale_to<AFC_BF16>(T.in[t], T.out[t], dt, from, n, c);
+  else
+    scale_to<AFC_F16>(T.in[t], T.out[t], dt, from, n, c);
 }
 
 namespace {
@@ -136,35 +208,44 @@ void check_outputs(const afc_clip_args *p) {
   }
 }
 
-uint64_t workspace(const afc_clip_args *p) {
-  uint64_t n = 0;
-  for (int i = 0; i < p->count; ++i) n += (uint64_t)ceil_div(p->numel[i], kChunk);
-  return 256 + up256(8 * n);
+// Elements of a block: some 4096 blocks for all tensors together, so that the partial sums stay few, and 4096 elements at least
+int64_t chunk_of(const afc_clip_args *p) {
+  int64_t all = 0;
+  for (int i = 0; i < p->count; ++i) all += p->numel[i];
+  return std::max<int64_t>(4096, ceil_div(ceil_div(all, 4096), 2048) * 2048);
 }
+int64_t partials(const afc_clip_args *p) {
+  const int64_t chunk = chunk_of(p);
+  int64_t n = 0;
+  for (int i = 0; i < p->count; ++i) n += ceil_div(p->numel[i], chunk);
+  return n;
+}
+uint64_t workspace(const afc_clip_args *p) { return 256 + up256(8 * (uint64_t)partials(p)); }
 
-template <class F>
-void batches(const afc_clip_args *p, F &&go) {
-  int i = 0;
-  while (i < p->count) {
-    Batch t;
-    t.count = 0;
-    int64_t blocks = 0;
-    for (; i < p->count && t.count < kTensors; ++i) {
-      const int64_t n = ceil_div(p->numel[i], kChunk);
-      if (n == 0) continue;
-      want(n < (int64_t)1 << 30, "numel");
-      if (blocks + n >= (int64_t)1 << 31) break;
-      const int k = t.count++;
-      t.in[k] = p->in[i];
-      t.out[k] = p->out ? p->out[i] : nullptr;
-      t.numel[k] = p->numel[i];
-      t.in_dtype[k] = (uint8_t)p->in_dtype[i];
-      t.out_dtype[k] = p->out ? (uint8_t)p->out_dtype[i] : 0;
-      t.first[k] = (int32_t)blocks;
-      blocks += n;
+std::vector<Batch> batches(const afc_clip_args *p) {
+  std::vector<Batch> all;
+  const int64_t chunk = chunk_of(p);
+  int64_t blocks = 0;
+  for (int i = 0; i < p->count; ++i) {
+    if (p->numel[i] == 0) continue;
+    if (all.empty() || all.back().count == kTensors) {
+      all.emplace_back();
+      all.back().count = 0;
+      all.back().chunk = chunk;
+      blocks = 0;
     }
-    if (blocks) go(t, blocks);
+    Batch &t = all.back();
+    const int k = t.count++;
+    t.in[k] = p->in[i];
+    t.out[k] = p->out ? p->out[i] : nullptr;
+    t.numel[k] = p->numel[i];
+    t.in_dtype[k] = (uint8_t)p->in_dtype[i];
+    t.out_dtype[k] = p->out ? (uint8_t)p->out_dtype[i] : 0;
+    t.first[k] = (int32_t)blocks;
+    blocks += ceil_div(p->numel[i], chunk);
+    t.first[k + 1] = (int32_t)blocks;  // (a tensor has at most 4096 blocks, a batch 110 tensors)
   }
+  return all;
 }
 
 void clip(const afc_clip_args *p, hipStream_t st) {
@@ -179,19 +260,28 @@ void clip(const afc_clip_args *p, hipStream_t st) {
   OnDevice on(p->device);
   float *coef = (float *)p->workspace;
   double *part = (double *)((char *)p->workspace + 256);
+  const std::vector<Batch> all = batches(p);
   int64_t n = 0;
-  batches(p, [&](const Batch &t, int64_t blocks) {
-    k_squares<<<dim3((unsigned)blocks), 256, 0, st>>>(t, part + n);
+  for (const Batch &t : all) {
+    k_squares<<<dim3((unsigned)t.first[t.count]), 256, 0, st>>>(t, part + n);
     launched("k_squares");
-    n += blocks;
-  });
-  k_norm<<<1, 256, 0, st>>>(part, n, p->out ? p->max_norm : 0.f, p->norm, coef);
-  launched("k_norm");
+    n += t.first[t.count];
+  }
+  // Adding up 1024 partial sums in every block costs about what the launch of k_norm does
+  const bool few = p->out && n && n <= 1024;
+  if (!few) {
+    k_norm<<<1, 1024, 0, st>>>(part, n, p->out ? p->max_norm : 0.f, p->norm, coef);
+    launched("k_norm");
+  }
   if (!p->out) return;
-  batches(p, [&](const Batch &t, int64_t blocks) {
-    k_scale<<<dim3((unsigned)blocks), 256, 0, st>>>(t, coef);
+  for (size_t i = all.size(); i-- > 0;) {
+    const dim3 grid((unsigned)all[i].first[all[i].count]);
+    if (few)
+      k_scale<true><<<grid, 256, 0, st>>>(all[i], coef, part, n, p->max_norm, i ? nullptr : p->norm);
+    else
+      k_scale<false><<<grid, 256, 0, st>>>(all[i], coef, part, n, p->max_norm, nullptr);
     launched("k_scale");
-  });
+  }
 }
 
 }  // namespace

@@ -28,17 +28,30 @@ __device__ inline void store(Elem<DT> *p, const float (&f)[V]) {
   }
 }
 
+// V neighbouring elements as they were loaded (converted where they are used, so that loads stay in flight)
+template <int DT, int V>
+struct Raw {
+  Vec<DT, V> v;
+  __device__ inline void load(const Elem<DT> *p, bool on) {
+    v = (Vec<DT, V>)(Elem<DT>)0.f;
+    if (on) v = *reinterpret_cast<const Vec<DT, V> *>(p);
+  }
+  __device__ inline float operator[](int i) const { return (float)v[i]; }
+};
+
 struct Tiling {
   int log_cx;          // lanes side by side along the channels (the others: positions)
   int run;             // positions of a thread
   int64_t tiles_c, tiles_l;
 };
 
-constexpr int kRun = 8;  // positions of a forward thread
-
+// A thread takes T.run positions of V channels (16 bytes of a row): the filter and the last K - 1 inputs stay in registers, and
+// the next U positions are in flight while U are computed.  It reads and writes each element once (and K - 1 in front of each
+// run, mostly from cache): memory bounds it.
 template <int DT, int V, int K, bool SILU>
 __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
   typedef Elem<DT> E;
+  constexpr int U = 4;
   int64_t blk = blockIdx.x;
   const int64_t ct = blk % T.tiles_c;
   blk /= T.tiles_c;
@@ -46,7 +59,7 @@ __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
   const int cx = 1 << T.log_cx;
   const int64_t c = (ct * cx + (threadIdx.x & (cx - 1))) * V;
   if (c >= P.width) return;
-  const int64_t l0 = (lt * (256 >> T.log_cx) + (threadIdx.x >> T.log_cx)) * kRun;
+  const int64_t l0 = (lt * (256 >> T.log_cx) + (threadIdx.x >> T.log_cx)) * T.run;
   const int len = row_length(P.lengths, b, P.length);
   const E *x = (const E *)P.x.data + b * P.x.stride_batch + c;
   const E *s0 = P.initial_state ? (const E *)P.initial_state + b * (K - 1) * P.width + c : nullptr;
@@ -62,13 +75,14 @@ __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
     }
   }
   if (l0 >= P.length) return;
-  float w[K][V], bias[V] = {}, win[K - 1 + kRun][V];
+  const int64_t end = min(l0 + T.run, P.length);
+  float w[K][V], bias[V] = {}, win[K - 1 + U][V];
   for (int i = 0; i < V; ++i) {
     for (int k = 0; k < K; ++k) w[k][i] = P.weight[(c + i) * K + k];
     if (P.bias) bias[i] = P.bias[c + i];
   }
 #pragma unroll
-  for (int j = 0; j < K - 1 + kRun; ++j) {
+  for (int j = 0; j < K - 1; ++j) {
     const int64_t p = l0 + j - (K - 1);
     for (int i = 0; i < V; ++i) win[j][i] = 0.f;
     if (p < 0) {
@@ -77,18 +91,34 @@ __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
       load<DT, V>(win[j], x + p * P.x.stride_length);
     }
   }
-  E *y = (E *)P.y.data + b * P.y.stride_batch + c;
+  E *y = (E *)P.y.data + b * P.y.stride_batch + l0 * P.y.stride_length + c;
+  x += l0 * P.x.stride_length;
+  Raw<DT, V> ahead[U];
 #pragma unroll
-  for (int j = 0; j < kRun; ++j) {
-    const int64_t l = l0 + j;
-    if (l >= P.length) break;
-    float v[V];
-    for (int i = 0; i < V; ++i) {
-      float a = bias[i];
-      for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], win[j + k][i], a);
-      v[i] = l < len ? (SILU ? silu(a) : a) : 0.f;
+  for (int j = 0; j < U; ++j) ahead[j].load(x + j * P.x.stride_length, l0 + j < len && l0 + j < end);
+  for (int64_t l = l0; l < end; l += U) {
+    x += U * P.x.stride_length;
+    Raw<DT, V> now[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) now[j] = ahead[j];
+#pragma unroll
+    for (int j = 0; j < U; ++j) ahead[j].load(x + j * P.x.stride_length, l + U + j < len && l + U + j < end);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        win[K - 1 + j][i] = now[j][i];
+        float a = bias[i];
+        for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], win[j + k][i], a);
+        v[i] = l + j < len ? (SILU ? silu(a) : a) : 0.f;
+      }
+      if (l + j < end) store<DT, V>(y, v);
+      y += P.y.stride_length;
     }
-    store<DT, V>(y + l * P.y.stride_length, v);
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j)
+      for (int i = 0; i < V; ++i) win[j][i] = win[j + U][i];
   }
 }
 
@@ -156,48 +186,59 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
         load<DT, V>(xw[j], x + p * P.x.stride_length);
       }
     }
-    for (int64_t q = s; q < e + K - 1; ++q) {
-      float xn[V] = {}, dn[V] = {};
-      const bool live = q < len;
-      if (live) {
-        load<DT, V>(xn, x + q * P.x.stride_length);
-        load<DT, V>(dn, dy + q * P.dy.stride_length);
-      }
-      for (int i = 0; i < V; ++i) {
+    constexpr int U = 2;
+    const int64_t last = e + K - 1;
+    const E *xq = x + s * P.x.stride_length, *dq = dy + s * P.dy.stride_length;
+    Raw<DT, V> xa[U], da[U];
 #pragma unroll
-        for (int k = 0; k + 1 < K; ++k) {
-          xw[k][i] = xw[k + 1][i];
-          dp[k][i] = dp[k + 1][i];
-        }
-        xw[K - 1][i] = xn[i];
-        float d = dn[i];
-        if (SILU) {
-          float a = bias[i];
-          for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], xw[k][i], a);
-          d *= silu_slope(a, sigmoid(a));
-        }
-        d = live ? d : 0.f;
-        dp[K - 1][i] = d;
-        if (q < e) {
-          for (int k = 0; k < K; ++k) dw[k][i] = __builtin_fmaf(d, xw[k][i], dw[k][i]);
-          dw[K][i] += d;
-        }
+    for (int j = 0; j < U; ++j) {
+      xa[j].load(xq + j * P.x.stride_length, s + j < len && s + j < last);
+      da[j].load(dq + j * P.dy.stride_length, s + j < len && s + j < last);
+    }
+    for (int64_t q0 = s; q0 < last; q0 += U) {
+      xq += U * P.x.stride_length, dq += U * P.dy.stride_length;
+      Raw<DT, V> xn[U], dn[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) xn[j] = xa[j], dn[j] = da[j];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        xa[j].load(xq + j * P.x.stride_length, q0 + U + j < len && q0 + U + j < last);
+        da[j].load(dq + j * P.dy.stride_length, q0 + U + j < len && q0 + U + j < last);
       }
-      const int64_t l = q - (K - 1);
-      if (l < s && (l >= 0 || s > 0)) continue;
-      float v[V];
-      const int64_t jf = l - len + K - 1;
-      float add[V] = {};
-      if (df && jf >= 0 && jf < K - 1) load<DT, V>(add, df + jf * P.width);
-      for (int i = 0; i < V; ++i) {
-        float a = add[i];
-        for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], dp[K - 1 - k][i], a);
-        v[i] = l < len ? a : 0.f;
-      }
-      if (l < 0) {
-        if (ds) store<DT, V>(ds + (l + K - 1) * P.width, v);
-      } else {
-        store<DT, V>(dx + l * P.dx.stride_length, v);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int64_t q = q0 + j, l = q - (K - 1), jf = l - len + K - 1;
+        const bool live = q < len;
+        float v[V] = {};
+        if (df && jf >= 0 && jf < K - 1 && q < last) load<DT, V>(v, df + jf * P.width);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+#pragma unroll
+          for (int k = 0; k + 1 < K; ++k) {
+            xw[k][i] = xw[k + 1][i];
+            dp[k][i] = dp[k + 1][i];
+          }
+          xw[K - 1][i] = xn[j][i];
+          float d = dn[j][i];
+          if (SILU) {
+            float a = bias[i];
+            for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], xw[k][i], a);
+            d *= silu_slope(a, sigmoid(a));
+          }
+          d = live ? d : 0.f;
+          dp[K - 1][i] = d;
+          const float own = q < e ? d : 0.f;
+          for (int k = 0; k < K; ++k) dw[k][i] = __builtin_fmaf(own, xw[k][i], dw[k][i]);
+          dw[K][i] += own;
+          for (int k = 0; k < K; ++k) v[i] = __builtin_fmaf(w[k][i], dp[K - 1 - k][i], v[i]);
+          v[i] = l < len ? v[i] : 0.f;
+        }
+        if (q >= last || (l < s && (l >= 0 || s > 0))) continue;
+        if (l < 0) {
+          if (ds) store<DT, V>(ds + (l + K - 1) * P.width, v);
+        } else {
+          store<DT, V>(dx + l * P.dx.stride_length, v);
+        }
       }
     }
   }
@@ -285,17 +326,21 @@ int64_t blocks(const afc_conv_args *p, const Tiling &t) {
   want(n < (int64_t)1 << 31, "too many blocks");
   return n;
 }
-// positions of a gradient thread: long runs save partial rows and the K - 1 positions that neighbours both compute, short
-// ones give the chip enough threads
-Tiling grad_tiling(const afc_conv_args *p, int v) {
-  int run = 64;
+// Positions of a thread: long runs read the filter and the K - 1 positions that neighbours share less often (and leave fewer
+// partial rows of the filter's gradient), short ones give the chip enough threads.
+Tiling run_tiling(const afc_conv_args *p, int v, int run) {
   Tiling t = tiling(p, v, run);
   while (run > 8 && p->batch * t.tiles_l * t.tiles_c < 1024) t = tiling(p, v, run /= 2);
   return t;
 }
+// Channels of a gradient thread where rows are aligned.  Eight 16-bit ones would make 16 bytes a load, but with the windows of
+// inputs and of dp, the filter and its gradient they need 288 registers: 275 us against 250 for 3 x 8191 x 4096 forwards and
+// backwards.
+constexpr int kGradVector = 4;
+Tiling grad_tiling(const afc_conv_args *p, int v) { return run_tiling(p, v, 64); }
 uint64_t grad_bytes(const afc_conv_args *p) {
   uint64_t most = 0;
-  for (int v : {1, 16 / elem_bytes(p->dtype)}) {
+  for (int v : {1, kGradVector}) {
     const Tiling t = grad_tiling(p, v);
     const uint64_t n = up256((uint64_t)p->batch * t.tiles_l * (p->taps + 1) * p->width * 4);
     most = n > most ? n : most;
@@ -306,10 +351,10 @@ uint64_t grad_bytes(const afc_conv_args *p) {
 #define CONV_SILU(DT, V, K, ...) (p->silu ? CONV_GO(DT, V, K, true, __VA_ARGS__) : CONV_GO(DT, V, K, false, __VA_ARGS__))
 #define CONV_TAPS(DT, V, ...) \
   (p->taps == 2 ? CONV_SILU(DT, V, 2, __VA_ARGS__) : p->taps == 3 ? CONV_SILU(DT, V, 3, __VA_ARGS__) : CONV_SILU(DT, V, 4, __VA_ARGS__))
-#define CONV_TYPES(wide, ...)                                                                              \
-  (p->dtype == AFC_F32 ? (wide ? CONV_TAPS(AFC_F32, 4, __VA_ARGS__) : CONV_TAPS(AFC_F32, 1, __VA_ARGS__))  \
-   : p->dtype == AFC_BF16 ? (wide ? CONV_TAPS(AFC_BF16, 8, __VA_ARGS__) : CONV_TAPS(AFC_BF16, 1, __VA_ARGS__)) \
-                          : (wide ? CONV_TAPS(AFC_F16, 8, __VA_ARGS__) : CONV_TAPS(AFC_F16, 1, __VA_ARGS__)))
+#define CONV_TYPES(wide, VF, VH)                                                                   \
+  (p->dtype == AFC_F32 ? (wide ? CONV_TAPS(AFC_F32, VF, 0) : CONV_TAPS(AFC_F32, 1, 0))             \
+   : p->dtype == AFC_BF16 ? (wide ? CONV_TAPS(AFC_BF16, VH, 0) : CONV_TAPS(AFC_BF16, 1, 0))        \
+                          : (wide ? CONV_TAPS(AFC_F16, VH, 0) : CONV_TAPS(AFC_F16, 1, 0)))
 
 }  // namespace
 
@@ -318,10 +363,10 @@ static void conv(const afc_conv_args *p, hipStream_t st) {
   OnDevice on(p->device);
   if (p->batch == 0 || (p->length == 0 && !p->final_state)) return;
   const bool wide = vectors(p, {&p->x, &p->y}, {p->initial_state, p->final_state});
-  const Tiling t = tiling(p, wide ? 16 / elem_bytes(p->dtype) : 1, kRun);
+  const Tiling t = run_tiling(p, wide ? 16 / elem_bytes(p->dtype) : 1, 32);
   const dim3 grid((unsigned)blocks(p, t));
 #define CONV_GO(DT, V, K, S, ...) (k_conv<DT, V, K, S><<<grid, 256, 0, st>>>(*p, t), 0)
-  (void)CONV_TYPES(wide, 0);
+  (void)CONV_TYPES(wide, 4, 8);
 #undef CONV_GO
   launched("k_conv");
 }
@@ -335,7 +380,7 @@ static void conv_step(const afc_conv_args *p, hipStream_t st) {
   want(n < (int64_t)1 << 31, "too many blocks");
   const dim3 grid((unsigned)n);
 #define CONV_GO(DT, V, K, S, ...) (k_conv_step<DT, V, K, S><<<grid, 256, 0, st>>>(*p), 0)
-  (void)CONV_TYPES(wide, 0);
+  (void)CONV_TYPES(wide, 4, 8);
 #undef CONV_GO
   launched("k_conv_step");
 }
@@ -345,7 +390,7 @@ static void conv_grad(const afc_conv_args *p, hipStream_t st) {
   OnDevice on(p->device);
   const bool params = p->dweight || p->dbias;
   const bool wide = vectors(p, {&p->x, &p->dy, &p->dx}, {p->initial_state, p->dfinal_state, p->dinitial_state});
-  const Tiling t = grad_tiling(p, wide ? 16 / elem_bytes(p->dtype) : 1);
+  const Tiling t = grad_tiling(p, wide ? kGradVector : 1);
   float *part = params ? (float *)p->workspace : nullptr;
   const int64_t rows = p->batch * t.tiles_l;
   if (params)
@@ -353,7 +398,7 @@ static void conv_grad(const afc_conv_args *p, hipStream_t st) {
   if (p->batch > 0) {
     const dim3 grid((unsigned)blocks(p, t));
 #define CONV_GO(DT, V, K, S, ...) (k_conv_grad<DT, V, K, S><<<grid, 256, 0, st>>>(*p, t, part), 0)
-    (void)CONV_TYPES(wide, 0);
+    (void)CONV_TYPES(wide, 4, 4);
 #undef CONV_GO
     launched("k_conv_grad");
   }

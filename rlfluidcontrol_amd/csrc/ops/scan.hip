@@ -833,7 +833,67 @@ __global__ __launch_bounds__(256) void k_scan_params(afc_scan_args P, Sums sums,
 }
 
 // ---- single tokens ----
-// A channel's states lie side by side in NP lanes (a power of two, lanes behind `state` hold zeros), 64 / NP channels in a wave.
+// Reading and writing the state is what bounds them.  Where `state` is a multiple of four a lane has four states (16 bytes) of a
+// channel, NL lanes a channel, side by side as in memory, and R rows of the batch, whose loads are all in flight before the
+// first is used; the channel's parameters are read once for them.
+template <int NL>
+__device__ inline float sum_side(float v) {
+  if (NL > 1) v += dpp<kXor1>(v);
+  if (NL > 2) v += dpp<kXor2>(v);
+  if (NL > 4) v += dpp<0x141>(v);  // mirrored halves of eight: all four lanes of the other half hold its sum
+  if (NL > 8) v += dpp<0x140>(v);  // mirrored sixteen
+  return v;
+}
+
+template <int DT, int NL, int R>
+__global__ __launch_bounds__(256) void k_scan_step4(afc_scan_args P, int tiles) {
+  typedef Elem<DT> E;
+  typedef float F4 __attribute__((ext_vector_type(4)));
+  const int tile = blockIdx.x % tiles;
+  const int64_t b0 = (int64_t)(blockIdx.x / tiles) * R, w = (int64_t)tile * (256 / NL) + threadIdx.x / NL;
+  const int n = threadIdx.x % NL * 4, rows = (int)min((int64_t)R, P.batch - b0);
+  if (w >= P.width) return;
+  const bool on = n < P.state;  // (a lane without states holds zeros: it takes part in the sums)
+  const int64_t g = (unsigned)w / (unsigned)(P.width / P.groups), st = (b0 * P.width + w) * P.state + n, row = P.width * P.state;
+  F4 h[R];
+  E x[R], dt[R], z[R], B[R][4], C[R][4];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r >= rows) continue;
+    const int64_t b = b0 + r;
+    h[r] = (F4)0.f;
+    if (on) h[r] = *reinterpret_cast<const F4 *>(P.final_state + st + r * row);
+    x[r] = ((const E *)P.x.data)[b * P.x.stride_batch + w];
+    dt[r] = ((const E *)P.dt.data)[b * P.dt.stride_batch + w];
+    if (P.z.data) z[r] = ((const E *)P.z.data)[b * P.z.stride_batch + w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      B[r][i] = on ? ((const E *)P.b.data)[b * P.b.stride_batch + g * P.b.stride_group + n + i] : (E)0.f;
+      C[r][i] = on ? ((const E *)P.c.data)[b * P.c.stride_batch + g * P.c.stride_group + n + i] : (E)0.f;
+    }
+  }
+  F4 a2 = (F4)0.f;
+  if (on) a2 = *reinterpret_cast<const F4 *>(P.a + w * P.state + n);
+  a2 *= 1.44269504088896341f;
+  const float bias = P.dt_bias ? P.dt_bias[w] : 0.f, D = P.d ? P.d[w] : 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    if (r >= rows) continue;
+    const float v = (float)dt[r] + bias, xr = (float)x[r], delta = P.softplus ? softplus(v) : v, u = delta * xr;
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[r][i] = __builtin_fmaf(__builtin_amdgcn_exp2f(delta * a2[i]), h[r][i], u * (float)B[r][i]);
+      y = __builtin_fmaf((float)C[r][i], h[r][i], y);
+    }
+    if (on) *reinterpret_cast<F4 *>(P.final_state + st + r * row) = h[r];
+    y = __builtin_fmaf(D, xr, sum_side<NL>(y));
+    if (P.z.data) y *= silu((float)z[r]);
+    if (n == 0) ((E *)P.y.data)[(b0 + r) * P.y.stride_batch + w] = (E)y;
+  }
+}
+
+// Any other state: one lane for each, in NP lanes (a power of two, lanes behind `state` hold zeros), 64 / NP channels in a wave.
 template <int NP>
 __device__ inline float sum_lanes(float v) {
   for (int m = 1; m < NP; m <<= 1) v += __shfl_xor(v, m);
@@ -1067,10 +1127,34 @@ int lanes(const afc_scan_args *p) {
     default: STEP_GO(DT, 64); break;       \
   }
 
+template <int DT, int NL>
+void go_step4(const afc_scan_args *p, hipStream_t st) {
+  const int64_t tiles = ceil_div(p->width, 256 / NL);
+  // four rows a thread where that leaves four blocks for every CU
+  const int rows = tiles * p->batch >= 4 * 1024 ? 4 : 1;
+  const int64_t n = tiles * ceil_div(p->batch, rows);
+  want(n < (int64_t)1 << 31, "too many blocks");
+  const dim3 grid((unsigned)n);
+  if (rows == 4)
+    k_scan_step4<DT, NL, 4><<<grid, 256, 0, st>>>(*p, (int)tiles);
+  else
+    k_scan_step4<DT, NL, 1><<<grid, 256, 0, st>>>(*p, (int)tiles);
+}
+void step4(const afc_scan_args *p, hipStream_t st) {
+#define STEP4(DT)                                                          \
+  p->state <= 4 ? go_step4<DT, 1>(p, st) : p->state <= 8 ? go_step4<DT, 2>(p, st) : p->state <= 16 ? go_step4<DT, 4>(p, st) : \
+  p->state <= 32 ? go_step4<DT, 8>(p, st) : go_step4<DT, 16>(p, st)
+  if (p->dtype == AFC_F32) STEP4(AFC_F32);
+  if (p->dtype == AFC_BF16) STEP4(AFC_BF16);
+  if (p->dtype == AFC_F16) STEP4(AFC_F16);
+  launched("k_scan_step4");
+}
+
 void scan_step(const afc_scan_args *p, hipStream_t st) {
   check(p, false, true);
   OnDevice on(p->device);
   if (p->batch == 0) return;
+  if (p->state % 4 == 0 && (uintptr_t)p->final_state % 16 == 0 && (uintptr_t)p->a % 16 == 0) return step4(p, st);
   const int64_t n = p->batch * ceil_div(p->width, 64 / lanes(p));
   want(n < (int64_t)1 << 31, "too many blocks");
   const dim3 grid((unsigned)n);

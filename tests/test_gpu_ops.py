@@ -217,7 +217,7 @@ def test_scan_grows_where_a_is_positive():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("B,W,N,G", [(1, 1, 1, 1), (3, 64, 16, 1), (5, 37, 13, 1), (2, 30, 64, 3), (1024, 256, 16, 1), (7, 24, 8, 2), (4, 12, 3, 4)])
+@pytest.mark.parametrize("B,W,N,G", [(1, 1, 1, 1), (3, 64, 16, 1), (5, 37, 13, 1), (2, 30, 64, 3), (1024, 256, 16, 1), (7, 24, 8, 2), (4, 12, 3, 4), (70, 1100, 16, 2), (9, 70, 12, 1), (3, 40, 48, 2), (5, 33, 4, 1), (6, 50, 32, 5)])
 def test_scan_step_continues_a_sequence(dtype, B, W, N, G):
     c = scan_case(B + W, B, 4, W, N, G, dtype, DEV)
     args = (c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], None)
