@@ -10,11 +10,18 @@ Reference constants (agent_TD3.py:12-27): lr 1e-4 (Adam, TF defaults), gamma 0.9
 batch 512, buffer 1e6, policy delay 2, exploration sigma 0.1, target smoothing sigma 0.2 clipped to
 0.5, actor 2->256->256->2 (ReLU, ReLU, tanh), twin critics (2+2)->256->256->1, Glorot-uniform
 kernels and zero biases (tf.layers.dense defaults).
+
+Beside the reference's actor there is one with memory (`actor="memory"`): the agent sees two force coefficients of a wake, and
+what it saw before tells more about the flow.  It reads the episode through a short causal convolution and a selective state
+space scan (rlfluidcontrol_amd.ops) and is trained on windows of the replay; `max_grad_norm` clips either kind's gradients by
+their global norm.
 """
 import math
 
 import torch
 import torch.nn as nn
+
+from . import ops
 
 REWARD_ACTION_COST = math.pi * (1 / 8) * 0.0097 * (3.66 ** 3)  # server.py:64 (= 0.186756...)
 
@@ -108,7 +115,8 @@ class ReplayBuffer:
         self.ptr, self.size, self.max_size = 0, 0, size
         self.device = device
 
-    def store(self, obs, act, rew, next_obs, done):
+    def store(self, obs, act, rew, next_obs, done, pos=0):
+        """`pos`: the transitions' place in their episode (WindowReplayBuffer keeps it)"""
         obs = torch.as_tensor(obs, dtype=torch.float32, device=self.device).reshape(-1, self.obs1_buf.shape[1])
         B = obs.shape[0]
         act = torch.as_tensor(act, dtype=torch.float32, device=self.device).reshape(B, -1)
@@ -167,6 +175,52 @@ class ReplayBuffer:
         self.ptr = int(sd["ptr"]) % self.max_size if same else n % self.max_size
 
 
+class WindowReplayBuffer(ReplayBuffer):
+    """A replay ring for an actor with memory: every store holds one transition of each of `rows` envs, so that an env's next
+    transition lies `rows` places on, and windows of consecutive transitions of one env and episode can be drawn."""
+
+    def __init__(self, obs_dim, act_dim, size, rows, device="cpu"):
+        super().__init__(obs_dim, act_dim, max(size // rows, 1) * rows, device=device)
+        self.rows = rows
+        self.pos_buf = torch.zeros(self.max_size, dtype=torch.int64, device=device)
+
+    def store(self, obs, act, rew, next_obs, done, pos=0):
+        at = self.ptr
+        obs = torch.as_tensor(obs, dtype=torch.float32, device=self.device).reshape(-1, self.obs1_buf.shape[1])
+        if obs.shape[0] != self.rows:
+            raise ValueError("a store holds one transition of each of %d envs, not %d" % (self.rows, obs.shape[0]))
+        super().store(obs, act, rew, next_obs, done)
+        self.pos_buf[at:at + self.rows] = pos
+
+    def sample_windows(self, batch_size, length, generator=None):
+        """`batch_size` windows [batch, length, ...] that start at any stored transition and end with the episode, the newest
+        transition or after `length`; `lengths` (int32) says where"""
+        start = torch.randint(0, self.size, (batch_size,), device=self.device, generator=generator)
+        newest = self.ptr - 1 - start
+        newest = newest % self.max_size if self.size == self.max_size else newest
+        k = torch.arange(length, device=self.device)
+        at = (start[:, None] + k * self.rows) % self.max_size
+        inside = (k <= torch.div(newest, self.rows, rounding_mode="floor")[:, None]) & (self.pos_buf[at] == self.pos_buf[start][:, None] + k)
+        lengths = inside.long().cumprod(1).sum(1).to(torch.int32)
+        return dict(obs1=self.obs1_buf[at], obs2=self.obs2_buf[at], acts=self.acts_buf[at], rews=self.rews_buf[at], done=self.done_buf[at], lengths=lengths)
+
+    def state_dict(self):
+        return dict(super().state_dict(), pos=self.pos_buf[:self.size].cpu(), rows=self.rows)
+
+    def check_state_dict(self, sd):
+        super().check_state_dict(sd)
+        if int(sd.get("rows", 0)) != self.rows or tuple(sd["pos"].shape) != (int(sd["size"]),):
+            raise ValueError("replay buffer checkpoint: transitions of %s envs side by side, expected %d" % (sd.get("rows"), self.rows))
+
+    def load_state_dict(self, sd):
+        super().load_state_dict(sd)
+        n, old_max = self.size, int(sd["max_size"])
+        order = torch.arange(n)
+        if old_max != self.max_size and n == old_max:  # unrolled as the transitions are
+            order = (order + int(sd["ptr"])) % max(n, 1)
+        self.pos_buf[:n] = sd["pos"][order].to(self.device)
+
+
 def _mlp(sizes, last):
     layers = []
     for i in range(len(sizes) - 1):
@@ -181,6 +235,57 @@ def _mlp(sizes, last):
     return nn.Sequential(*layers)
 
 
+class MemoryActor(nn.Module):
+    """States of an episode -> actions, each from all states up to its own:
+
+        (u, z) = W_in s     u = silu(causal convolution of u)     (d, B, C) = W_x u     y = scan(u, W_dt d, B, C) silu(z)
+        a = tanh(MLP(y))
+
+    `forward` takes whole windows [batch, length, state_dim] (with `lengths` of its own for each row), `step` one state of every
+    env and the memory it advances, which is of a fixed size whatever has been read."""
+
+    def __init__(self, state_dim, action_dim, width=256, state=16, taps=4):
+        super().__init__()
+        self.width, self.state, self.taps, self.rank = width, state, taps, max(1, width // 16)
+        self.proj_in = nn.Linear(state_dim, 2 * width)
+        self.conv_weight = nn.Parameter((2 * torch.rand(width, taps) - 1) / math.sqrt(taps))
+        self.conv_bias = nn.Parameter(torch.zeros(width))
+        self.proj_x = nn.Linear(width, self.rank + 2 * state, bias=False)
+        self.proj_dt = nn.Linear(self.rank, width, bias=False)
+        # decay rates 1 .. state for every channel; step sizes from 0.001 to 0.1 (dt_bias: the inverse of softplus at them)
+        self.log_rate = nn.Parameter(torch.log(torch.arange(1, state + 1, dtype=torch.float32)).repeat(width, 1))
+        dt = torch.exp(torch.rand(width) * (math.log(0.1) - math.log(0.001)) + math.log(0.001))
+        self.dt_bias = nn.Parameter(dt + torch.log(-torch.expm1(-dt)))
+        self.skip = nn.Parameter(torch.ones(width))
+        self.head = _mlp([width, 256, action_dim], nn.Tanh())
+        for lin in (self.proj_in, self.proj_x, self.proj_dt):
+            nn.init.xavier_uniform_(lin.weight)
+        nn.init.zeros_(self.proj_in.bias)
+
+    def _split(self, u):
+        d, B, C = self.proj_x(u).split([self.rank, self.state, self.state], -1)
+        return self.proj_dt(d), B, C
+
+    def forward(self, states, lengths=None):
+        u, z = self.proj_in(states).chunk(2, -1)
+        u = ops.causal_conv(u, self.conv_weight, self.conv_bias, silu=True, lengths=lengths)
+        dt, B, C = self._split(u)
+        y = ops.selective_scan(u, dt, -self.log_rate.exp(), B, C, D=self.skip, z=z, dt_bias=self.dt_bias, softplus=True, lengths=lengths)
+        return self.head(y)
+
+    def new_memory(self, rows):
+        dev = self.skip.device
+        return (torch.zeros(rows, self.taps - 1, self.width, device=dev), torch.zeros(rows, self.width, self.state, device=dev))
+
+    @torch.no_grad()
+    def step(self, states, memory):
+        u, z = self.proj_in(states).chunk(2, -1)
+        u = ops.causal_conv_step(u, memory[0], self.conv_weight, self.conv_bias, silu=True)
+        dt, B, C = self._split(u)
+        y = ops.selective_scan_step(u, dt, -self.log_rate.exp(), B, C, memory[1], D=self.skip, z=z, dt_bias=self.dt_bias, softplus=True)
+        return self.head(y)
+
+
 class Agent:
     """agent_TD3.py:10-184.  `get_action`, `train_iter`, `record`, `reset_agent`, `reset_episode`
     keep the reference's names and meaning; states/actions may carry any batch size."""
@@ -192,7 +297,18 @@ class Agent:
     STEPS_PER_EPISODE = 410
 
     def __init__(self, state_dim, action_dim, explore_noise="Gaussian", device="cpu", seed=None, num_envs=1, world=1,
-                 replay_capacity=None, replay_episodes=3, steps_per_episode=None):
+                 replay_capacity=None, replay_episodes=3, steps_per_episode=None, actor="mlp", window=64, max_grad_norm=None):
+        """actor: "mlp" (the reference's) or "memory" (MemoryActor: it acts on all states since reset_episode, one call of
+        get_action after the other, and learns from windows of `window` transitions, as many as make up the batch size; a
+        window starts with an empty memory).  max_grad_norm: the gradients of each update are clipped to this global norm."""
+        if actor not in ("mlp", "memory"):
+            raise ValueError("actor must be 'mlp' or 'memory', it is %r" % (actor,))
+        if window < 1:
+            raise ValueError("window must be 1 or more, it is %r" % (window,))
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError("max_grad_norm must be 0 or more, it is %r" % (max_grad_norm,))
+        self.actor, self.window, self.max_grad_norm = actor, int(window), max_grad_norm
+        self._memory = None
         self.world = world  # > 1: sharded learner (gradients averaged over the ranks, see _sync_grads)
         self.num_envs = num_envs
         self.n_grad_allreduce = 0
@@ -225,8 +341,14 @@ class Agent:
         self.steps_per_episode = int(steps_per_episode) if steps_per_episode else self.STEPS_PER_EPISODE
         self.replay_capacity = int(replay_capacity) if replay_capacity else max(
             self.bfs, int(replay_episodes) * local_envs * self.steps_per_episode)
-        self.replay_buffer = ReplayBuffer(state_dim, action_dim, self.replay_capacity, device=self.device)
+        self._rows = local_envs
+        self.replay_buffer = self._new_buffer()
         self.step_count = self.total_step_count = self.episode_count = self.train_count = 0
+
+    def _new_buffer(self):
+        if self.actor == "memory":
+            return WindowReplayBuffer(self.state_dim, self.action_dim, self.replay_capacity, self._rows, device=self.device)
+        return ReplayBuffer(self.state_dim, self.action_dim, self.replay_capacity, device=self.device)
 
     def _nets(self):
         return (self.main_actor, self.target_actor, self.main_critic_1, self.main_critic_2, self.target_critic_1,
@@ -251,8 +373,10 @@ class Agent:
 
     def _build(self):
         s, a, dev = self.state_dim, self.action_dim, self.device
-        self.main_actor = _mlp([s, 256, 256, a], nn.Tanh()).to(dev)
-        self.target_actor = _mlp([s, 256, 256, a], nn.Tanh()).to(dev)
+        self._memory = None
+        new_actor = (lambda: MemoryActor(s, a)) if self.actor == "memory" else (lambda: _mlp([s, 256, 256, a], nn.Tanh()))
+        self.main_actor = new_actor().to(dev)
+        self.target_actor = new_actor().to(dev)
         self.main_critic_1 = _mlp([s + a, 256, 256, 1], None).to(dev)
         self.main_critic_2 = _mlp([s + a, 256, 256, 1], None).to(dev)
         self.target_critic_1 = _mlp([s + a, 256, 256, 1], None).to(dev)
@@ -272,7 +396,12 @@ class Agent:
     @torch.no_grad()
     def get_action(self, state_data, stochastic=True):
         state = torch.as_tensor(state_data, dtype=torch.float32, device=self.device).reshape(-1, self.state_dim)
-        action = self.main_actor(state)
+        if self.actor == "memory":
+            if self._memory is None or self._memory[0].shape[0] != state.shape[0]:
+                self._memory = self.main_actor.new_memory(state.shape[0])
+            action = self.main_actor.step(state, self._memory)
+        else:
+            action = self.main_actor(state)
         if stochastic:
             if self.explore_noise == "Gaussian":
                 noise = self.explore_noise_size * torch.randn(action.shape, device=self.device, generator=self.gen)
@@ -301,6 +430,33 @@ class Agent:
         q_loss = ((self.main_critic_1(sa1) - y) ** 2).mean() + ((self.main_critic_2(sa1) - y) ** 2).mean()
         return q_loss, y
 
+    def window_losses(self, batch):
+        """losses() over windows [batch, length, ...]: the target actor reads each window's next states from its start, and the
+        mean runs over what lies within the windows"""
+        lengths = batch["lengths"]
+        keep = (torch.arange(batch["obs1"].shape[1], device=self.device) < lengths[:, None])[..., None]
+        with torch.no_grad():
+            nxt = self.target_actor(batch["obs2"], lengths)
+            noise = torch.clamp(self.criticreg_noise_size * torch.randn(nxt.shape, device=self.device, generator=self.gen),
+                                -self.criticreg_noise_clip, self.criticreg_noise_clip)
+            sa2 = torch.cat([batch["obs2"], torch.clamp(nxt + noise, -1, 1)], -1)
+            q_min = torch.minimum(self.target_critic_1(sa2), self.target_critic_2(sa2))
+            y = batch["rews"] + self.gamma * (1 - batch["done"]) * q_min
+        sa1 = torch.cat([batch["obs1"], batch["acts"]], -1)
+        off = (self.main_critic_1(sa1) - y) ** 2 + (self.main_critic_2(sa1) - y) ** 2
+        return torch.where(keep, off, 0.0).sum() / keep.sum(), y
+
+    def window_policy_loss(self, batch):
+        lengths = batch["lengths"]
+        keep = (torch.arange(batch["obs1"].shape[1], device=self.device) < lengths[:, None])[..., None]
+        q = self.main_critic_1(torch.cat([batch["obs1"], self.main_actor(batch["obs1"], lengths)], -1))
+        return -torch.where(keep, q, 0.0).sum() / keep.sum()
+
+    def _clip_grads(self, params):
+        """after _sync_grads: every rank clips the same averaged gradients by the same norm"""
+        if self.max_grad_norm is not None:
+            ops.clip_grad_norm([p.grad for p in params], self.max_grad_norm)
+
     def _sync_grads(self, params):
         """sharded learner: every rank holds the transitions of its own envs and a 1/world share of the batch; the
         gradients are averaged over the ranks (one all-reduce of the flattened gradients), so every rank applies the
@@ -323,17 +479,26 @@ class Agent:
         bs = self.bs // max(self.world, 1)  # this rank's share of the batch (bs is a multiple of world: __init__)
         if bs > self.replay_buffer.size:
             return
-        batch = self.replay_buffer.sample_batch(bs, generator=self.gen)
-        q_loss, _ = self.losses(batch)
+        if self.actor == "memory":
+            batch = self.replay_buffer.sample_windows(max(1, bs // self.window), self.window, generator=self.gen)
+            q_loss, _ = self.window_losses(batch)
+        else:
+            batch = self.replay_buffer.sample_batch(bs, generator=self.gen)
+            q_loss, _ = self.losses(batch)
         self.Q_opt.zero_grad(set_to_none=True)
         q_loss.backward()
         self._sync_grads(self._critic_params)
+        self._clip_grads(self._critic_params)
         self.Q_opt.step()
         if self.total_step_count % self.d == 0:
-            p_loss = -self.main_critic_1(torch.cat([batch["obs1"], self.main_actor(batch["obs1"])], 1)).mean()
+            if self.actor == "memory":
+                p_loss = self.window_policy_loss(batch)
+            else:
+                p_loss = -self.main_critic_1(torch.cat([batch["obs1"], self.main_actor(batch["obs1"])], 1)).mean()
             self.P_opt.zero_grad(set_to_none=True)
             p_loss.backward()
             self._sync_grads(list(self.main_actor.parameters()))
+            self._clip_grads(list(self.main_actor.parameters()))
             self.P_opt.step()
             with torch.no_grad():  # T_op
                 for t, m in self._pairs:
@@ -343,17 +508,18 @@ class Agent:
         self.total_step_count += 1
 
     def record(self, this_state, this_action, this_reward, this_done, next_state):
-        self.replay_buffer.store(obs=this_state, act=this_action, rew=this_reward, next_obs=next_state, done=this_done)
+        self.replay_buffer.store(obs=this_state, act=this_action, rew=this_reward, next_obs=next_state, done=this_done, pos=self.step_count)
         self.step_count += 1
 
     def reset_agent(self):
-        self.replay_buffer = ReplayBuffer(self.state_dim, self.action_dim, self.replay_capacity, device=self.device)
+        self.replay_buffer = self._new_buffer()
         self.step_count = self.total_step_count = self.train_count = self.episode_count = 0
         self._build()
         if self.world > 1:
             self._sync_from_rank0(0)  # a fresh model on every rank: rank 0's where a process group is up
 
     def reset_episode(self):
+        self._memory = None
         self.step_count = 0
         self.train_count = 0
         self.episode_count += 1
@@ -364,13 +530,16 @@ class Agent:
                                                            "target_critic_1", "target_critic_2")}
         return dict(nets=nets, Q_opt=self.Q_opt.state_dict(), P_opt=self.P_opt.state_dict(),
                     replay=self.replay_buffer.state_dict(), episode_count=self.episode_count,
-                    total_step_count=self.total_step_count)
+                    total_step_count=self.total_step_count, actor=self.actor)
 
     def load_state_dict(self, sd):
-        self.replay_buffer.check_state_dict(sd["replay"])  # validate everything before the first mutation
+        if sd.get("actor", "mlp") != self.actor:  # validate everything before the first mutation
+            raise ValueError("checkpoint of a %r actor, this agent has a %r one" % (sd.get("actor", "mlp"), self.actor))
+        self.replay_buffer.check_state_dict(sd["replay"])
         for n in sd["nets"]:
             if not hasattr(self, n):
                 raise ValueError("checkpoint has an unknown network %r" % n)
+        self._memory = None
         for n, s in sd["nets"].items():
             getattr(self, n).load_state_dict(s)
         self.Q_opt.load_state_dict(sd["Q_opt"])
@@ -399,16 +568,17 @@ class BatchedLearner:
     and at the end of the episode turn them into transitions and run `train_steps` TD3 iterations."""
 
     def __init__(self, num_envs, device="cpu", filter="None", explore_noise="Gaussian", one_action=False, seed=None,
-                 shard=None, steps_per_episode=None):
+                 shard=None, steps_per_episode=None, actor="mlp", window=64, max_grad_norm=None):
         """num_envs = ALL envs this learner acts for (every rank evaluates the same actor on the gathered obs).
         shard = (rank, world): the learner is sharded -- this rank stores the transitions of ITS envs only (the block
-        [rank*E, (rank+1)*E) of the env axis) and trains on a 1/world share of every batch with averaged gradients."""
+        [rank*E, (rank+1)*E) of the env axis) and trains on a 1/world share of every batch with averaged gradients.
+        actor, window, max_grad_norm: see Agent."""
         self.E = num_envs
         self.rank, self.world = shard if shard is not None else (0, 1)
         self.one_action = one_action
         self.action_dim = 1 if one_action else 2
         self.agent = Agent(2, self.action_dim, explore_noise=explore_noise, device=device, seed=seed, num_envs=num_envs,
-                           world=self.world, steps_per_episode=steps_per_episode)
+                           world=self.world, steps_per_episode=steps_per_episode, actor=actor, window=window, max_grad_norm=max_grad_norm)
         self.filter = KalmanFilter() if filter == "Kalman" else NoneFilter()
         self.state_record, self.action_record = [], []
 
@@ -437,6 +607,6 @@ class BatchedLearner:
                 s1, act, r, s2, done = s1[:, sl], act[:, sl], r[:, sl], s2[:, sl], done[:, sl]
             # time-major records -> one store per agent step keeps the reference's FIFO order per env
             for t in range(s1.shape[0]):
-                self.agent.replay_buffer.store(s1[t], act[t], r[t], s2[t], done[t])
+                self.agent.replay_buffer.store(s1[t], act[t], r[t], s2[t], done[t], pos=t)
         for _ in range(steps):
             self.agent.train_iter()

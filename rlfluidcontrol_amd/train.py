@@ -116,7 +116,7 @@ def run_episode(vec, learner, max_requests=None, stochastic=True, plan=None):
 
 def train(num_envs=1024, resolution=16, reynolds=100, episodes=1, train_steps=1000, device="cuda:0", seed=0,
           filter="None", explore_noise="Gaussian", init=None, max_requests=None, env_kwargs=None, batch_size=None,
-          log=print):
+          log=print, actor="mlp", window=64, max_grad_norm=None):
     from . import build, env as envmod
     build.build()
     dev = torch.device(device)
@@ -139,7 +139,8 @@ def train(num_envs=1024, resolution=16, reynolds=100, episodes=1, train_steps=10
     plan = None if c.carry_quirk else full_plan
     # (the replay ring holds whole episodes of this env configuration: its requests per episode, not the reference case's)
     learner = td3.BatchedLearner(vec.world * num_envs, device=dev, filter=filter, explore_noise=explore_noise, seed=seed,
-                                 shard=(vec.rank, vec.world), steps_per_episode=full_plan[1] + 2)
+                                 shard=(vec.rank, vec.world), steps_per_episode=full_plan[1] + 2, actor=actor, window=window,
+                                 max_grad_norm=max_grad_norm)
     if batch_size:
         learner.agent.bs = batch_size
     history = []
@@ -175,6 +176,9 @@ def main(argv=None):
     ap.add_argument("--max-requests", type=int, default=None)
     ap.add_argument("--filter", choices=["None", "Kalman"], default="None")
     ap.add_argument("--explore-noise", choices=["Gaussian", "Process"], default="Gaussian")
+    ap.add_argument("--actor", choices=["mlp", "memory"], default="mlp", help="mlp: the reference's; memory: acts on the whole episode so far")
+    ap.add_argument("--window", type=int, default=64, help="transitions of a training window (--actor memory)")
+    ap.add_argument("--max-grad-norm", type=float, default=None, help="clip each update's gradients to this global norm (default: no clipping)")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--gpus", type=int, default=1, help="ranks to spawn (one per GPU) when not started by a launcher")
     ap.add_argument("--init", default=None, help=".npz with u, v, p: the reset state (default: free stream)")
@@ -204,7 +208,7 @@ def main(argv=None):
     try:
         train(num_envs=a.envs, resolution=a.res, reynolds=a.reynolds, episodes=a.episodes, train_steps=a.train_steps,
               max_requests=a.max_requests, filter=a.filter, explore_noise=a.explore_noise, seed=a.seed, device=dev,
-              init=init)
+              init=init, actor=a.actor, window=a.window, max_grad_norm=a.max_grad_norm)
     finally:
         if world > 1:
             dist.destroy_process_group()
