@@ -161,7 +161,6 @@ struct Conv : torch::autograd::Function<Conv> {
     p.dweight = ptr<float>(dw), p.dbias = ptr<float>(db), p.dinitial_state = ptr(ds);
     Tensor ws;
     if (dw.defined() || db.defined()) {
-      p.y = p.dx;  // (sizes only)
       ok(afc_conv_workspace(&p, &p.workspace_bytes));
       ws = space(x, p.workspace_bytes);
       p.workspace = ptr(ws);

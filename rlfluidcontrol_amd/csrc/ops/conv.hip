@@ -283,12 +283,16 @@ namespace {
 
 int elem_bytes(int dtype) { return dtype == AFC_F32 ? 4 : 2; }
 
-void check(const afc_conv_args *p, bool grad, bool step) {
+void check_sizes(const afc_conv_args *p) {
   want(p != nullptr, "null arguments");
   want(p->dtype >= AFC_F32 && p->dtype <= AFC_F16, "dtype must be AFC_F32, AFC_BF16 or AFC_F16");
   want(p->taps >= 2 && p->taps <= 4, "taps must be 2, 3 or 4");
   want(p->batch >= 0 && p->length >= 0 && p->width >= 1, "batch, length or width");
   want(p->length < kMostAxis && p->width < kMostAxis && p->batch < kMostAxis, "an axis of 2^30 or more");
+}
+
+void check(const afc_conv_args *p, bool grad, bool step) {
+  check_sizes(p);
   want(p->weight != nullptr, "weight is missing");
   if (step) want(p->length == 1 && !p->lengths && p->final_state && p->final_state == p->initial_state, "a step takes length 1, no lengths, and its state as initial_state and final_state");
   if (p->batch == 0 || p->length == 0) return;
@@ -423,7 +427,7 @@ int afc_conv_grad(const afc_conv_args *args, void *hip_stream) {
 }
 int afc_conv_workspace(const afc_conv_args *args, uint64_t *bytes) {
   return afc_ops::entry("afc_conv_workspace", [&] {
-    afc_ops::check(args, false, false);
+    afc_ops::check_sizes(args);
     afc_ops::want(bytes != nullptr, "null argument");
     *bytes = afc_ops::grad_bytes(args);
   });

@@ -856,7 +856,9 @@ __global__ __launch_bounds__(256) void k_scan_step4(afc_scan_args P, int tiles) 
   const bool on = n < P.state;  // (a lane without states holds zeros: it takes part in the sums)
   const int64_t g = (unsigned)w / (unsigned)(P.width / P.groups), st = (b0 * P.width + w) * P.state + n, row = P.width * P.state;
   F4 h[R];
-  E x[R], dt[R], z[R], B[R][4], C[R][4];
+  typedef E E4 __attribute__((ext_vector_type(4), aligned(sizeof(E))));  // (from any place: B and C may be slices)
+  E x[R], dt[R], z[R];
+  E4 B[R], C[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     if (r >= rows) continue;
@@ -866,10 +868,10 @@ __global__ __launch_bounds__(256) void k_scan_step4(afc_scan_args P, int tiles) 
     x[r] = ((const E *)P.x.data)[b * P.x.stride_batch + w];
     dt[r] = ((const E *)P.dt.data)[b * P.dt.stride_batch + w];
     if (P.z.data) z[r] = ((const E *)P.z.data)[b * P.z.stride_batch + w];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      B[r][i] = on ? ((const E *)P.b.data)[b * P.b.stride_batch + g * P.b.stride_group + n + i] : (E)0.f;
-      C[r][i] = on ? ((const E *)P.c.data)[b * P.c.stride_batch + g * P.c.stride_group + n + i] : (E)0.f;
+    B[r] = C[r] = (E4)(E)0.f;
+    if (on) {
+      B[r] = *reinterpret_cast<const E4 *>((const E *)P.b.data + b * P.b.stride_batch + g * P.b.stride_group + n);
+      C[r] = *reinterpret_cast<const E4 *>((const E *)P.c.data + b * P.c.stride_batch + g * P.c.stride_group + n);
     }
   }
   F4 a2 = (F4)0.f;
@@ -954,6 +956,7 @@ void check(const afc_scan_args *p, bool grad, bool step) {
     check_seq(p->ddt, p->batch, p->length, 0, "ddt");
     check_seq(p->db, p->batch, p->length, p->groups, "db");
     check_seq(p->dc, p->batch, p->length, p->groups, "dc");
+    want(!p->dz.data || p->z.data, "dz without z");
     if (p->dz.data) check_seq(p->dz, p->batch, p->length, 0, "dz");
     want(p->checkpoints != nullptr, "checkpoints are missing");
   }
@@ -971,18 +974,20 @@ Split split(const afc_scan_args *p) {
 }
 int padded(const afc_scan_args *p) { return split(p).s * split(p).nl; }
 
-Plan plan(const afc_scan_args *p) {
+Plan plan(const afc_scan_args *p, bool grad) {
   Plan t;
   const int cb = 256 / split(p).nl;
   t.tiles = (int)ceil_div(p->width / p->groups, cb);
   t.chunks = (int)ceil_div(p->length, K);
   const int64_t blocks = p->batch * p->groups * t.tiles;
-  // Parts cost a pass of their own for the carries (two thirds of the forward pass), so they are made where rows and channels
-  // give less than two blocks for each of 256 CUs, up to four, and no shorter than 256 positions.  1 x 8191 x 2048 (64 blocks):
-  // 256 us in 4 parts, 179 in 8, 163 in 16; 8 x 2048 x 2048 (512 blocks) forwards and backwards: 813 us whole, 987 in 2 parts.
+  // Parts cost a pass of their own for the carries: two thirds of the forward pass, a fifth of the backward one.  A CU gets
+  // through a chunk of a block in 1.1 us with one block, in 0.76 us each with four (backwards, where registers allow two: 3.3
+  // and 2.4 us), so they are made where there is less than a block for each of 256 CUs (backwards: one and a half).  1 x 8191 x
+  // 2048 (64 blocks) takes 578 us whole, 182 in 8 parts, 160 in 16 and in 32; 5 x 1021 x 1000 with a state of 64 (320 blocks)
+  // 123 us whole and 130 in 4 parts; 4 x 4096 x 2048 (256 blocks) with gradients 1116 us whole and 1033 with two parts backwards.  Shorter than 128 positions a part does not pay.
   int64_t segs = 1;
-  if (blocks < 512)
-    while (blocks * segs < 1024 && t.chunks / (segs * 2) >= 16) segs *= 2;
+  if (blocks < (grad ? 384 : 256))
+    while (blocks * segs < (grad ? 512 : 1024) && t.chunks / (segs * 2) >= 8) segs *= 2;
   t.seg_chunks = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, segs);
   t.segs = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, t.seg_chunks);
   want(blocks * t.segs < (int64_t)1 << 31, "too many blocks");
@@ -1037,7 +1042,7 @@ void check_workspace(const afc_scan_args *p, uint64_t bytes) {
 
 void scan(const afc_scan_args *p, hipStream_t st) {
   check(p, false, false);
-  const Plan t = plan(p);
+  const Plan t = plan(p, false);
   if (p->batch > 0) check_workspace(p, carry_bytes(p, t));
   want((uintptr_t)p->checkpoints % 16 == 0, "checkpoints must be 16-byte aligned");
   OnDevice on(p->device);
@@ -1073,7 +1078,7 @@ Layout layout(const afc_scan_args *p, const Plan &t) {
 
 void scan_grad(const afc_scan_args *p, hipStream_t st) {
   check(p, true, false);
-  const Plan t = plan(p);
+  const Plan t = plan(p, true);
   const Layout o = layout(p, t);
   if (p->batch > 0) check_workspace(p, o.all);
   want((uintptr_t)p->checkpoints % 16 == 0, "checkpoints must be 16-byte aligned");
@@ -1130,8 +1135,9 @@ int lanes(const afc_scan_args *p) {
 template <int DT, int NL>
 void go_step4(const afc_scan_args *p, hipStream_t st) {
   const int64_t tiles = ceil_div(p->width, 256 / NL);
-  // four rows a thread where that leaves four blocks for every CU
-  const int rows = tiles * p->batch >= 4 * 1024 ? 4 : 1;
+  // four rows a thread where that leaves four blocks for every CU: 131 x 4096 x 16 bf16 takes 15.6 us with four and 18.3 with
+  // one, 1024 x 256 x 16 f32 9.4 and 9.8; below, one row keeps the chip busier
+  const int rows = tiles * p->batch >= 4096 ? 4 : 1;
   const int64_t n = tiles * ceil_div(p->batch, rows);
   want(n < (int64_t)1 << 31, "too many blocks");
   const dim3 grid((unsigned)n);
@@ -1184,10 +1190,10 @@ int afc_scan_workspace(const afc_scan_args *args, uint64_t *checkpoint_bytes, ui
     using namespace afc_ops;
     want(args && checkpoint_bytes && scan_bytes && grad_bytes, "null argument");
     check_sizes(args);
-    const Plan t = plan(args);
+    const Plan t = plan(args, false), g = plan(args, true);
     *checkpoint_bytes = up256((uint64_t)args->batch * t.chunks * args->width * padded(args) * 4);
     *scan_bytes = carry_bytes(args, t);
-    *grad_bytes = layout(args, t).all;
+    *grad_bytes = layout(args, g).all;
   });
 }
 }

@@ -3,11 +3,12 @@ C ABI's own checks (which refuse before any device is touched)."""
 import ctypes as C
 import os
 import re
+import shutil
 
 import pytest
 import torch
 
-from rlfluidcontrol_amd import build, ops
+from rlfluidcontrol_amd import build, codeobj, ops
 from tests import ops_abi as abi
 from tests import ops_reference as ref
 from tests.conftest import ROOT
@@ -287,7 +288,8 @@ def test_c_abi_refuses_bad_arguments(lib):
     for kw in (dict(dtype=3), dict(state=0), dict(state=65), dict(groups=0), dict(groups=3), dict(width=0), dict(a=0), dict(batch=-1), dict(length=-1),
                dict(x=abi.Seq()), dict(dt=abi.Seq()), dict(b=abi.Seq()), dict(c=abi.Seq(4096, 1, 1, big)), dict(z=abi.Seq(4096, 1, -1, 0)), dict(y=abi.Seq())):
         bad(lib.afc_scan, fake_scan(**kw))
-    for kw in (dict(dx=abi.Seq()), dict(ddt=abi.Seq()), dict(db=abi.Seq()), dict(dc=abi.Seq()), dict(checkpoints=0), dict()):  # the last: no workspace
+    for kw in (dict(dx=abi.Seq()), dict(ddt=abi.Seq()), dict(db=abi.Seq()), dict(dc=abi.Seq()), dict(checkpoints=0), dict(dz=abi.Seq(4096, 20, 4, 0)),
+               dict()):  # the last: no workspace
         bad(lib.afc_scan_grad, fake_scan(**kw))
     bad(lib.afc_scan_step, fake_scan(length=1))
 
@@ -309,6 +311,28 @@ def test_c_abi_refuses_bad_arguments(lib):
               clip([a, a], [4, 4], outs=[a, a]), clip([a, a + 8], [4, 4], outs=[a, a + 8]), clip([a], [4], outs=[a + 4]), clip([a, b], [4, 4], outs=[b, a]),
               clip([a, b], [4, 4], outs=[b + 64, b + 68])):
         bad(lib.afc_clip, p)
+
+
+def test_workspaces_need_sizes_only(lib):
+    p = abi.ConvArgs()
+    p.taps, p.batch, p.length, p.width = 4, 2, 100, 24
+    n = (C.c_uint64 * 3)()
+    at = [C.cast(C.byref(n, 8 * k), C.POINTER(C.c_uint64)) for k in range(3)]
+    assert lib.afc_conv_workspace(C.byref(p), at[0]) == 0 and n[0] >= 5 * 24 * 4
+    q = abi.ScanArgs()
+    q.state, q.batch, q.length, q.width, q.groups = 16, 2, 100, 24, 2
+    assert lib.afc_scan_workspace(C.byref(q), *at) == 0 and n[0] >= 2 * 7 * 24 * 16 * 4 and n[2] > 0
+    q.length = 0
+    assert lib.afc_scan_workspace(C.byref(q), *at) == 0
+    assert lib.afc_scan_workspace(C.byref(q), None, at[0], at[1]) == -1 and lib.afc_conv_workspace(C.byref(p), None) == -1
+
+
+@pytest.mark.skipif(not os.path.exists(os.path.join(codeobj.LLVM, "clang-offload-bundler")) or shutil.which("objcopy") is None, reason="ROCm LLVM tools not available")
+def test_kernels_use_scalar_float_arithmetic_and_no_scratch(lib):
+    path = build.build_ops()
+    assert not re.search(r"v_pk_(add|mul|fma)_f32", codeobj.disassembly(path))
+    for name, r in codeobj.kernel_resources(path).items():
+        assert r["private_segment_fixed_size"] == 0, name
 
 
 def test_no_cpu_fallback_of_the_library(lib):
