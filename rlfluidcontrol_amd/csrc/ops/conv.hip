@@ -5,8 +5,10 @@
 
 namespace afc_ops {
 
+// V neighbouring elements at any address that suits one: the memory pipeline takes accesses that start anywhere, so rows of odd
+// widths and slices need no other path
 template <int DT, int V>
-using Vec = Elem<DT> __attribute__((ext_vector_type(V)));
+using Vec = Elem<DT> __attribute__((ext_vector_type(V), aligned(sizeof(Elem<DT>))));
 
 template <int DT, int V>
 __device__ inline void load(float (&f)[V], const Elem<DT> *p) {
@@ -57,8 +59,9 @@ __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
   blk /= T.tiles_c;
   const int64_t lt = blk % T.tiles_l, b = blk / T.tiles_l;
   const int cx = 1 << T.log_cx;
-  const int64_t c = (ct * cx + (threadIdx.x & (cx - 1))) * V;
+  int64_t c = (ct * cx + (threadIdx.x & (cx - 1))) * V;
   if (c >= P.width) return;
+  c = min(c, P.width - V);  // (the last vector ends with the row: what two lanes share both write, the same)
   const int64_t l0 = (lt * (256 >> T.log_cx) + (threadIdx.x >> T.log_cx)) * T.run;
   const int len = row_length(P.lengths, b, P.length);
   const E *x = (const E *)P.x.data + b * P.x.stride_batch + c;
@@ -157,13 +160,15 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
   const int64_t lt = blk % T.tiles_l, b = blk / T.tiles_l;
   const int cx = 1 << T.log_cx, ty = 256 >> T.log_cx;
   const int lane_c = threadIdx.x & (cx - 1), lane_l = threadIdx.x >> T.log_cx;
-  const int64_t c = (ct * cx + lane_c) * V;
+  int64_t c = (ct * cx + lane_c) * V;
+  const bool inside = c < P.width;
+  c = inside ? min(c, P.width - V) : c;  // (the last vector ends with the row: what two lanes share both write, the same)
   const int64_t s = (lt * ty + lane_l) * (int64_t)T.run;
   const int len = row_length(P.lengths, b, P.length);
   float dw[K + 1][V];
   for (int k = 0; k <= K; ++k)
     for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
-  if (c < P.width && (s < P.length || s == 0)) {
+  if (inside && (s < P.length || s == 0)) {
     const int64_t e = s + T.run < P.length ? s + T.run : P.length;
     const E *x = (const E *)P.x.data + b * P.x.stride_batch + c;
     const E *dy = (const E *)P.dy.data + b * P.dy.stride_batch + c;
@@ -249,7 +254,7 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
     __syncthreads();
     for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = dw[k][i];
     __syncthreads();
-    if (lane_l == 0 && c < P.width) {
+    if (lane_l == 0 && inside) {
       for (int i = 0; i < V; ++i) {
         float a = 0.f;
         for (int r = 0; r < ty; ++r) a += red[((r << T.log_cx) + lane_c) * V + i];
@@ -304,17 +309,6 @@ void check(const afc_conv_args *p, bool grad, bool step) {
   }
 }
 
-// vectors of 16 bytes along the channels where every row starts on one
-bool vectors(const afc_conv_args *p, std::initializer_list<const afc_seq *> seqs, std::initializer_list<const void *> states) {
-  const int e = elem_bytes(p->dtype), v = 16 / e;
-  if (p->width % v) return false;
-  for (const afc_seq *s : seqs)
-    if ((uintptr_t)s->data % 16 || s->stride_batch % v || s->stride_length % v) return false;
-  for (const void *s : states)
-    if ((uintptr_t)s % 16) return false;
-  return true;
-}
-
 Tiling tiling(const afc_conv_args *p, int v, int run) {
   Tiling t;
   const int64_t lanes = ceil_div(p->width, v);
@@ -337,7 +331,7 @@ Tiling run_tiling(const afc_conv_args *p, int v, int run) {
   while (run > 8 && p->batch * t.tiles_l * t.tiles_c < 1024) t = tiling(p, v, run /= 2);
   return t;
 }
-// Channels of a gradient thread where rows are aligned.  Eight 16-bit ones would make 16 bytes a load, but with the windows of
+// Channels of a gradient thread.  Eight 16-bit ones would make 16 bytes a load, but with the windows of
 // inputs and of dp, the filter and its gradient they need 288 registers: 275 us against 250 for 3 x 8191 x 4096 forwards and
 // backwards.
 constexpr int kGradVector = 4;
@@ -366,8 +360,9 @@ static void conv(const afc_conv_args *p, hipStream_t st) {
   check(p, false, false);
   OnDevice on(p->device);
   if (p->batch == 0 || (p->length == 0 && !p->final_state)) return;
-  const bool wide = vectors(p, {&p->x, &p->y}, {p->initial_state, p->final_state});
-  const Tiling t = run_tiling(p, wide ? 16 / elem_bytes(p->dtype) : 1, 32);
+  const int v = 16 / elem_bytes(p->dtype);
+  const bool wide = p->width >= v;
+  const Tiling t = run_tiling(p, wide ? v : 1, 32);
   const dim3 grid((unsigned)blocks(p, t));
 #define CONV_GO(DT, V, K, S, ...) (k_conv<DT, V, K, S><<<grid, 256, 0, st>>>(*p, t), 0)
   (void)CONV_TYPES(wide, 4, 8);
@@ -379,8 +374,9 @@ static void conv_step(const afc_conv_args *p, hipStream_t st) {
   check(p, false, true);
   OnDevice on(p->device);
   if (p->batch == 0) return;
-  const bool wide = vectors(p, {&p->x, &p->y}, {p->final_state});
-  const int64_t n = ceil_div(p->batch * (p->width / (wide ? 16 / elem_bytes(p->dtype) : 1)), 256);
+  const int v = 16 / elem_bytes(p->dtype);
+  const bool wide = p->width % v == 0;  // (the state is updated in place: no two lanes may share a channel)
+  const int64_t n = ceil_div(p->batch * (p->width / (wide ? v : 1)), 256);
   want(n < (int64_t)1 << 31, "too many blocks");
   const dim3 grid((unsigned)n);
 #define CONV_GO(DT, V, K, S, ...) (k_conv_step<DT, V, K, S><<<grid, 256, 0, st>>>(*p), 0)
@@ -393,7 +389,7 @@ static void conv_grad(const afc_conv_args *p, hipStream_t st) {
   check(p, true, false);
   OnDevice on(p->device);
   const bool params = p->dweight || p->dbias;
-  const bool wide = vectors(p, {&p->x, &p->dy, &p->dx}, {p->initial_state, p->dfinal_state, p->dinitial_state});
+  const bool wide = p->width >= kGradVector;
   const Tiling t = grad_tiling(p, wide ? kGradVector : 1);
   float *part = params ? (float *)p->workspace : nullptr;
   const int64_t rows = p->batch * t.tiles_l;

@@ -101,37 +101,38 @@ __device__ inline float sum_channels(float *v, int lane) {
   return mine + dpp<kXor1>(other);
 }
 
-// E neighbouring elements in the form in which they were loaded (converted where they are used, so that loads stay in flight)
-template <int DT, int E, bool VEC>
+// E neighbouring elements in the form in which they were loaded (converted where they are used, so that loads stay in flight).
+// They are loaded and stored together from any address that suits one element: the memory pipeline takes accesses that start
+// anywhere, so rows of odd widths and slices need no scalar path.  WHOLE: n is E or 0, as where E divides a group's channels
+// (without the branches for a last piece that is cut, 8 x 2048 x 2048 takes 812 us forwards and backwards, with them 892).
+template <int DT, int E, bool WHOLE>
 struct Piece {
-  Elem<DT> v[E];
-  __device__ inline void load(const Elem<DT> *p, int n) {
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = i < n ? p[i] : (Elem<DT>)0.f;
-  }
-  __device__ inline float operator[](int i) const { return (float)v[i]; }
-};
-template <int DT, int E>
-struct Piece<DT, E, true> {
   typedef Elem<DT> V __attribute__((ext_vector_type(E)));
+  typedef Elem<DT> Any __attribute__((ext_vector_type(E), aligned(sizeof(Elem<DT>))));
   V v;
   __device__ inline void load(const Elem<DT> *p, int n) {
     v = (V)(Elem<DT>)0.f;
-    if (n > 0) v = *reinterpret_cast<const V *>(p);
+    if (WHOLE ? n > 0 : n == E) {
+      v = *reinterpret_cast<const Any *>(p);
+    } else if (!WHOLE && n > 0) {
+#pragma unroll
+      for (int i = 0; i + 1 < E; ++i)
+        if (i < n) v[i] = p[i];
+    }
   }
   __device__ inline float operator[](int i) const { return (float)v[i]; }
 };
-template <int DT, int E, bool VEC>
+template <int DT, int E, bool WHOLE>
 __device__ inline void store(Elem<DT> *p, const float *f, int n) {
-  if constexpr (VEC) {
-    typename Piece<DT, E, true>::V v;
+  typename Piece<DT, E, WHOLE>::V v;
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = (Elem<DT>)f[i];
-    if (n > 0) *reinterpret_cast<typename Piece<DT, E, true>::V *>(p) = v;
-  } else {
+  for (int i = 0; i < E; ++i) v[i] = (Elem<DT>)f[i];
+  if (WHOLE ? n > 0 : n == E) {
+    *reinterpret_cast<typename Piece<DT, E, WHOLE>::Any *>(p) = v;
+  } else if (!WHOLE && n > 0) {
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-      if (i < n) p[i] = (Elem<DT>)f[i];
+    for (int i = 0; i + 1 < E; ++i)
+      if (i < n) p[i] = v[i];
   }
 }
 template <int S>
@@ -317,7 +318,7 @@ __device__ inline void take_carries(float *h, const float *a2, const Carry &carr
 // the step sizes of chunk i + 1 (into the other half of LDS), finish the outputs of chunk i - 1 and have the loads of chunk
 // i + 2 in flight: the chains of the recurrence leave issue slots that the rest fills, also with a single wave on each SIMD.
 // CARRY: only the carries are computed (of all parts but the last)
-template <int DT, int S, int NL, bool VEC, bool CARRY>
+template <int DT, int S, int NL, bool WHOLE, bool CARRY>
 __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry carry) {
   typedef Shape<S, NL> H;
   constexpr int E = H::E;
@@ -342,7 +343,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
     D[i] = P.d && i < at.n ? P.d[at.w0 + at.q + i] : 0.f;
   }
   const int first = at.first_chunk(T), live = at.live_end(T), end = at.end_chunk(T);
-  Piece<DT, E, VEC> x{}, dt{}, z{}, xa{}, dta{}, za{};  // of the chunk whose step sizes come next, and of the one after it
+  Piece<DT, E, WHOLE> x{}, dt{}, z{}, xa{}, dta{}, za{};  // of the chunk whose step sizes come next, and of the one after it
   const int64_t l0 = (int64_t)first * K;
   Rows<DT, S, NL> rb(P.b, at, l0), rc(P.c, at, l0);
   Stream<DT> xs(P.x, at.b, l0 + at.r, at.w0 + at.q), dts(P.dt, at.b, l0 + at.r, at.w0 + at.q), zs(P.z, at.b, l0 + at.r, at.w0 + at.q),
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
     rb.put(bs[half]);
     if (!CARRY) rc.put(cs[half]);
   };
-  Piece<DT, E, VEC> x1{}, z1{}, x2{}, z2{};  // of the chunk in the recurrence, and of the one before it
+  Piece<DT, E, WHOLE> x1{}, z1{}, x2{}, z2{};  // of the chunk in the recurrence, and of the one before it
   float y[E];
   auto finish = [&](int i) {
     const float v = __builtin_fmaf(D[i], x2[i], y[i]), gated = v * silu(z2[i]);
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
     if (l >= P.length) return;
 #pragma unroll
     for (int i = 0; i < E; ++i) y[i] = l < at.len ? y[i] : 0.f;
-    store<DT, E, VEC>(out.p, y, at.n);
+    store<DT, E, WHOLE>(out.p, y, at.n);
     out.next();
   };
   if (first < live) {
@@ -453,7 +454,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
   }
   for (int ch = live; ch < end; ++ch, out.next()) {
     const float zero[E] = {};
-    if (ch * K + at.r < P.length) store<DT, E, VEC>(out.p, zero, at.n);
+    if (ch * K + at.r < P.length) store<DT, E, WHOLE>(out.p, zero, at.n);
   }
   if (at.seg == T.segs - 1) put_state<S, NL>(P.final_state, h, P, at);
 }
@@ -466,7 +467,7 @@ struct Sums {
 };
 
 // What a part hands on to the one before it, from a zero adjoint behind it (of all parts but the first)
-template <int DT, int S, int NL, bool VEC>
+template <int DT, int S, int NL, bool WHOLE>
 __global__ __launch_bounds__(256) void k_scan_grad_carry(afc_scan_args P, Plan T, Carry carry) {
   typedef Shape<S, NL> H;
   constexpr int E = H::E;
@@ -481,7 +482,7 @@ __global__ __launch_bounds__(256) void k_scan_grad_carry(afc_scan_args P, Plan T
 #pragma unroll
   for (int i = 0; i < E; ++i) bias[i] = P.dt_bias && i < at.n ? P.dt_bias[at.w0 + at.q + i] : 0.f;
   const int first = at.first_chunk(T), live = at.live_end(T);
-  Piece<DT, E, VEC> dt{}, z{}, dout{}, dta{}, za{}, douta{};
+  Piece<DT, E, WHOLE> dt{}, z{}, dout{}, dta{}, za{}, douta{};
   const int64_t l0 = (int64_t)(live - 1) * K;
   Rows<DT, S, NL> rc(P.c, at, l0);
   Stream<DT> dts(P.dt, at.b, l0 + at.r, at.w0 + at.q), zs(P.z, at.b, l0 + at.r, at.w0 + at.q), douts(P.dy, at.b, l0 + at.r, at.w0 + at.q);
@@ -549,7 +550,7 @@ __global__ __launch_bounds__(256) void k_scan_grad_carry(afc_scan_args P, Plan T
 
 // A chunk is run forwards again from its checkpoint with the states and decays of its K positions in registers (beside it, the
 // outputs of the chunk behind it are finished), then backwards (beside it, the chunk in front of it is prepared).
-template <int DT, int S, int NL, bool VEC>
+template <int DT, int S, int NL, bool WHOLE>
 __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carry carry, Sums sums) {
   typedef Shape<S, NL> H;
   constexpr int E = H::E, V = 2 * S, SET = H::CPW > V ? H::CPW : V, NO = (K * 2 * H::NP + 255) / 256;
@@ -574,7 +575,7 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
   for (int s = 0; s < S; ++s) sum_a[s] = 0.f;
   const int first = at.first_chunk(T), live = at.live_end(T), end = at.end_chunk(T);
   const bool gate = P.z.data, soft = P.softplus;
-  Piece<DT, E, VEC> x{}, dt{}, z{}, dout{}, xa{}, dta{}, za{}, douta{};  // of the chunk that is prepared next, and of the one in front of it
+  Piece<DT, E, WHOLE> x{}, dt{}, z{}, dout{}, xa{}, dta{}, za{}, douta{};  // of the chunk that is prepared next, and of the one in front of it
   const int64_t l0 = (int64_t)(live - 1) * K, lr = l0 + at.r, wq = at.w0 + at.q;
   Rows<DT, S, NL> rb(P.b, at, l0), rc(P.c, at, l0);
   Stream<DT> xs(P.x, at.b, lr, wq), dts(P.dt, at.b, lr, wq), zs(P.z, at.b, lr, wq), douts(P.dy, at.b, lr, wq), dxs(P.dx, at.b, lr, wq), ddts(P.ddt, at.b, lr, wq),
@@ -616,7 +617,7 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
   };
   // the chunk in the recurrence, and the one behind it
   struct Kept {
-    Piece<DT, E, VEC> x, dt, z, dout;
+    Piece<DT, E, WHOLE> x, dt, z, dout;
     float step[E], dy[E];
   } k1{}, k2{};
   auto keep = [&] {
@@ -658,9 +659,9 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
         sum_d[i] = __builtin_fmaf(k2.dy[i], k2.x[i], sum_d[i]);
         sum_b[i] += ddt[i];
       }
-      store<DT, E, VEC>(dxs.p, dx, at.n);
-      store<DT, E, VEC>(ddts.p, ddt, at.n);
-      if (P.dz.data) store<DT, E, VEC>(dzs.p, dz, at.n);
+      store<DT, E, WHOLE>(dxs.p, dx, at.n);
+      store<DT, E, WHOLE>(ddts.p, ddt, at.n);
+      if (P.dz.data) store<DT, E, WHOLE>(dzs.p, dz, at.n);
     }
     dxs.back(), ddts.back(), dzs.back();
   };
@@ -669,9 +670,9 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
     for (int ch = live; ch < end; ++ch) {
       dxs.next(), ddts.next(), dzs.next();
       if (ch * K + at.r < P.length) {
-        store<DT, E, VEC>(dxs.p, zero, at.n);
-        store<DT, E, VEC>(ddts.p, zero, at.n);
-        if (P.dz.data) store<DT, E, VEC>(dzs.p, zero, at.n);
+        store<DT, E, WHOLE>(dxs.p, zero, at.n);
+        store<DT, E, WHOLE>(ddts.p, zero, at.n);
+        if (P.dz.data) store<DT, E, WHOLE>(dzs.p, zero, at.n);
       }
       for (int i = threadIdx.x; i < K * 2 * H::NP; i += 256)
         if (ch * K + i / (2 * H::NP) < P.length) sums.bc[(bc_tile + ch * K) * 2 * H::NP + i] = 0.f;
@@ -970,6 +971,10 @@ struct Split {
 };
 Split split(const afc_scan_args *p) {
   const int n = p->state;
+  const int64_t wg = p->width / p->groups;
+  // groups of few channels: more lanes a channel instead of idle ones (37 x 7197 x 7, four groups, state 1: XXX us against 324)
+  if (n <= 16 && wg <= 16) return Split{1, 16};
+  if (n <= 8 && wg <= 32) return Split{1, 8};
   return n <= 4 ? Split{1, 4} : n <= 8 ? Split{1, 8} : n <= 16 ? Split{2, 8} : n <= 32 ? Split{2, 16} : Split{4, 16};
 }
 int padded(const afc_scan_args *p) { return split(p).s * split(p).nl; }
@@ -994,36 +999,28 @@ Plan plan(const afc_scan_args *p, bool grad) {
   return t;
 }
 
-// vectors of E elements along the channels where every row and every tile starts on one
-bool vectors(const afc_scan_args *p, std::initializer_list<const afc_seq *> seqs) {
-  const int v = 16 / split(p).nl, e = p->dtype == AFC_F32 ? 4 : 2;
-  if (p->width / p->groups % v) return false;
-  for (const afc_seq *s : seqs)
-    if (s->data && ((uintptr_t)s->data % (v * e) || s->stride_batch % v || s->stride_length % v)) return false;
-  return true;
-}
-
-#define SCAN_SHAPE(DT, VEC, C)                \
-  switch (split(p).s * 100 + split(p).nl) {   \
-    case 104: SCAN_GO(DT, 1, 4, VEC, C); break;  \
-    case 108: SCAN_GO(DT, 1, 8, VEC, C); break;  \
-    case 208: SCAN_GO(DT, 2, 8, VEC, C); break;  \
-    case 216: SCAN_GO(DT, 2, 16, VEC, C); break; \
-    default: SCAN_GO(DT, 4, 16, VEC, C); break;  \
+#define SCAN_SHAPE(DT, WHOLE, C)                 \
+  switch (split(p).s * 100 + split(p).nl) {      \
+    case 104: SCAN_GO(DT, 1, 4, WHOLE, C); break;  \
+    case 108: SCAN_GO(DT, 1, 8, WHOLE, C); break;  \
+    case 116: SCAN_GO(DT, 1, 16, true, C); break;  \
+    case 208: SCAN_GO(DT, 2, 8, WHOLE, C); break;  \
+    case 216: SCAN_GO(DT, 2, 16, true, C); break;  \
+    default: SCAN_GO(DT, 4, 16, true, C); break;   \
   }
-#define SCAN_VEC(DT, C)          \
-  if (wide) {                    \
-    SCAN_SHAPE(DT, true, C)      \
-  } else {                       \
-    SCAN_SHAPE(DT, false, C)     \
+#define SCAN_WHOLE(DT, C)                                        \
+  if (p->width / p->groups % (16 / split(p).nl) == 0) {          \
+    SCAN_SHAPE(DT, true, C)                                      \
+  } else {                                                       \
+    SCAN_SHAPE(DT, false, C)                                     \
   }
-#define SCAN_ALL(C)              \
-  if (p->dtype == AFC_F32) {     \
-    SCAN_VEC(AFC_F32, C)         \
+#define SCAN_ALL(C)                  \
+  if (p->dtype == AFC_F32) {         \
+    SCAN_WHOLE(AFC_F32, C)           \
   } else if (p->dtype == AFC_BF16) { \
-    SCAN_VEC(AFC_BF16, C)        \
-  } else {                       \
-    SCAN_VEC(AFC_F16, C)         \
+    SCAN_WHOLE(AFC_BF16, C)          \
+  } else {                           \
+    SCAN_WHOLE(AFC_F16, C)           \
   }
 
 uint64_t carry_bytes(const afc_scan_args *p, const Plan &t) {
@@ -1047,10 +1044,9 @@ void scan(const afc_scan_args *p, hipStream_t st) {
   want((uintptr_t)p->checkpoints % 16 == 0, "checkpoints must be 16-byte aligned");
   OnDevice on(p->device);
   if (p->batch == 0) return;
-  const bool wide = vectors(p, {&p->x, &p->dt, &p->z, &p->y});
   const Carry carry = carry_at(p, t);
   const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
-#define SCAN_GO(DT, S, NL, VEC, C) k_scan<DT, S, NL, VEC, C><<<grid, 256, 0, st>>>(*p, t, carry)
+#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan<DT, S, NL, WHOLE, C><<<grid, 256, 0, st>>>(*p, t, carry)
   if (t.segs > 1) {
     SCAN_ALL(true)
     launched("k_scan (carry)");
@@ -1087,15 +1083,14 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   const Carry carry = carry_at(p, t);
   const Sums sums = {(float *)(ws + o.bc), (float *)(ws + o.a), (float *)(ws + o.d), (float *)(ws + o.bias)};
   if (p->batch > 0) {
-    const bool wide = vectors(p, {&p->x, &p->dt, &p->z, &p->dy, &p->dx, &p->ddt, &p->dz});
-    const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
+      const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
     if (t.segs > 1) {
-#define SCAN_GO(DT, S, NL, VEC, C) k_scan_grad_carry<DT, S, NL, VEC><<<grid, 256, 0, st>>>(*p, t, carry)
+#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan_grad_carry<DT, S, NL, WHOLE><<<grid, 256, 0, st>>>(*p, t, carry)
       SCAN_ALL(0)
 #undef SCAN_GO
       launched("k_scan_grad_carry");
     }
-#define SCAN_GO(DT, S, NL, VEC, C) k_scan_grad<DT, S, NL, VEC><<<grid, 256, 0, st>>>(*p, t, carry, sums)
+#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan_grad<DT, S, NL, WHOLE><<<grid, 256, 0, st>>>(*p, t, carry, sums)
     SCAN_ALL(0)
 #undef SCAN_GO
     launched("k_scan_grad");
