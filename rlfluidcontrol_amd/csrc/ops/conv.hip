@@ -265,17 +265,12 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
 }
 
 // dweight, dbias: the partial rows summed in their order
-__global__ __launch_bounds__(256) void k_conv_params(const float *part, int64_t rows, int64_t width, int taps, float *dweight,
-                                                     float *dbias) {
-  __shared__ float red[256];
+__global__ __launch_bounds__(1024) void k_conv_params(const float *part, int64_t rows, int64_t width, int taps, float *dweight,
+                                                      float *dbias) {
+  __shared__ float red[1024];
   const int64_t cols = (taps + 1) * width, col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  float a = 0.f;
-  if (col < cols)
-    for (int64_t r = threadIdx.x >> 6; r < rows; r += 4) a += part[r * cols + col];
-  red[threadIdx.x] = a;
-  __syncthreads();
+  const float a = column_sum(part, rows, cols, col, red);
   if (threadIdx.x >= 64 || col >= cols) return;
-  a = (red[threadIdx.x] + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]);
   const int64_t k = col / width, w = col - k * width;
   if (k < taps) {
     if (dweight) dweight[w * taps + k] = a;
@@ -404,7 +399,7 @@ static void conv_grad(const afc_conv_args *p, hipStream_t st) {
   }
   if (params) {
     const dim3 grid((unsigned)ceil_div((p->taps + 1) * p->width, 64));
-    k_conv_params<<<grid, 256, 0, st>>>(part, rows, p->width, p->taps, p->dweight, p->dbias);
+    k_conv_params<<<grid, 1024, 0, st>>>(part, rows, p->width, p->taps, p->dweight, p->dbias);
     launched("k_conv_params");
   }
 }

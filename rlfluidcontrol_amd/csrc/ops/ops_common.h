@@ -114,6 +114,26 @@ __device__ inline float softplus(float v) {
   return fmaxf(v, 0.f) + (dw == 0.f ? e : l);
 }
 
+// Sum of a column over many rows by a block of 1024: 64 columns, 16 interleaved runs of rows with four sums each in flight, added
+// up in a fixed order.  The threads below 64 get it.  (Four runs: 68 us for 1107 rows of 288 columns, which make only five
+// blocks.)
+__device__ inline float column_sum(const float *from, int64_t rows, int64_t cols, int64_t col, float *red) {
+  float a[4] = {};
+  if (col < cols) {
+    int64_t r = threadIdx.x >> 6;
+    for (; r + 48 < rows; r += 64)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) a[k] += from[(r + 16 * k) * cols + col];
+    for (; r < rows; r += 16) a[0] += from[r * cols + col];
+  }
+  red[threadIdx.x] = (a[0] + a[1]) + (a[2] + a[3]);
+  __syncthreads();
+  float sum = 0.f;
+  if (threadIdx.x < 64)
+    for (int k = 0; k < 16; ++k) sum += red[threadIdx.x + 64 * k];
+  return sum;
+}
+
 __device__ inline int row_length(const int32_t *lengths, int64_t b, int64_t length) {
   if (!lengths) return (int)length;
   const int n = lengths[b];

@@ -120,6 +120,7 @@ struct Piece {
         if (i < n) v[i] = p[i];
     }
   }
+  __device__ inline void load_all(const Elem<DT> *p) { v = *reinterpret_cast<const Any *>(p); }
   __device__ inline float operator[](int i) const { return (float)v[i]; }
 };
 template <int DT, int E, bool WHOLE>
@@ -191,6 +192,8 @@ struct Place {
     r = threadIdx.x >> 4, q = (threadIdx.x & 15) * H::E;
     n = max(0, min(H::E, nw - q));
   }
+  // where the thread may read rows: a thread without channels reads the block's first ones, and what it reads counts as zero
+  __device__ int64_t readable() const { return w0 + (n > 0 ? q : 0); }
   __device__ int first_chunk(const Plan &T) const { return seg * T.seg_chunks; }
   __device__ int end_chunk(const Plan &T) const { return min((seg + 1) * T.seg_chunks, T.chunks); }
   __device__ int live_end(const Plan &T) const { return max(first_chunk(T), min(end_chunk(T), (len + K - 1) / K)); }
@@ -204,18 +207,24 @@ struct Rows {
   const Elem<DT> *p;
   int64_t stride, step;
   int k, n;
+  bool on;  // (of a padded state the thread reads the first one's value and puts zero)
   Elem<DT> v[H::NB], ahead[H::NB];
-  __device__ Rows(const afc_seq &s, const Place<S, NL> &at, int64_t l0)
-      : stride(s.stride_length * R), step(K * s.stride_length), k(threadIdx.x / H::NP), n(threadIdx.x % H::NP) {
-    p = (const Elem<DT> *)s.data + at.b * s.stride_batch + (l0 + k) * s.stride_length + at.g * s.stride_group + n;
+  __device__ Rows(const afc_seq &s, const Place<S, NL> &at, int64_t l0, int N)
+      : stride(s.stride_length * R), step(K * s.stride_length), k(threadIdx.x / H::NP), n(threadIdx.x % H::NP), on(n < N) {
+    p = (const Elem<DT> *)s.data + at.b * s.stride_batch + (l0 + k) * s.stride_length + at.g * s.stride_group + (on ? n : 0);
+  }
+  __device__ inline void load_all() {
+#pragma unroll
+    for (int i = 0; i < H::NB; ++i)
+      if (K * H::NP >= 256 * (i + 1) || k + i * R < K) ahead[i] = p[i * stride];
   }
   __device__ void next() { p += step; }
   __device__ void back() { p -= step; }
-  __device__ inline void load(int left, int N) {  // left: positions of the chunk within the row
+  __device__ inline void load(int left) {  // left: positions of the chunk within the row
 #pragma unroll
     for (int i = 0; i < H::NB; ++i) {
       ahead[i] = (Elem<DT>)0.f;
-      if (k + i * R < (left < K ? left : K) && n < N) ahead[i] = p[i * stride];
+      if (k + i * R < (left < K ? left : K)) ahead[i] = p[i * stride];
     }
   }
   __device__ inline void take() {
@@ -225,7 +234,7 @@ struct Rows {
   __device__ inline void put(float *to) const {
 #pragma unroll
     for (int i = 0; i < H::NB; ++i)
-      if (K * H::NP >= 256 * (i + 1) || threadIdx.x + 256 * i < K * H::NP) to[threadIdx.x + 256 * i] = (float)v[i];
+      if (K * H::NP >= 256 * (i + 1) || threadIdx.x + 256 * i < K * H::NP) to[threadIdx.x + 256 * i] = on ? (float)v[i] : 0.f;
   }
 };
 
@@ -344,18 +353,26 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
   }
   const int first = at.first_chunk(T), live = at.live_end(T), end = at.end_chunk(T);
   Piece<DT, E, WHOLE> x{}, dt{}, z{}, xa{}, dta{}, za{};  // of the chunk whose step sizes come next, and of the one after it
-  const int64_t l0 = (int64_t)first * K;
-  Rows<DT, S, NL> rb(P.b, at, l0), rc(P.c, at, l0);
-  Stream<DT> xs(P.x, at.b, l0 + at.r, at.w0 + at.q), dts(P.dt, at.b, l0 + at.r, at.w0 + at.q), zs(P.z, at.b, l0 + at.r, at.w0 + at.q),
-      out(P.y, at.b, l0 + at.r, at.w0 + at.q);
+  const int64_t l0 = (int64_t)first * K, lr = l0 + at.r, wq = at.readable();
+  Rows<DT, S, NL> rb(P.b, at, l0, P.state), rc(P.c, at, l0, P.state);
+  Stream<DT> xs(P.x, at.b, lr, wq), dts(P.dt, at.b, lr, wq), zs(P.z, at.b, lr, wq), out(P.y, at.b, lr, at.w0 + at.q);
   const bool gate = !CARRY && P.z.data, soft = P.softplus;
   auto fetch = [&](int ch) {
-    const int n = ch < live && ch * K + at.r < at.len ? at.n : 0, rows = ch < live ? at.len - ch * K : 0;
-    xa.load(xs.p, n);
-    dta.load(dts.p, n);
-    if (!CARRY) za.load(zs.p, gate ? n : 0);
-    rb.load(rows, P.state);
-    if (!CARRY) rc.load(rows, P.state);
+    if (ch >= live) return;  // (what is there stays, unused)
+    if (WHOLE && (ch + 1) * K <= at.len) {
+      xa.load_all(xs.p);
+      dta.load_all(dts.p);
+      if (gate) za.load_all(zs.p);
+      rb.load_all();
+      if (!CARRY) rc.load_all();
+    } else {
+      const int n = ch * K + at.r < at.len ? at.n : 0, rows = at.len - ch * K;
+      xa.load(xs.p, n);
+      dta.load(dts.p, n);
+      if (gate) za.load(zs.p, n);
+      rb.load(rows);
+      if (!CARRY) rc.load(rows);
+    }
     xs.next(), dts.next(), zs.next(), rb.next(), rc.next();
   };
   auto take = [&] {
@@ -369,7 +386,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
   float step[E];
   auto put = [&](int half) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) steps[half][at.r][at.q + i] = make_float2(step[i], step[i] * x[i]);
+    for (int i = 0; i < E; ++i) steps[half][at.r][at.q + i] = make_float2(step[i], i < at.n ? step[i] * x[i] : 0.f);
     rb.put(bs[half]);
     if (!CARRY) rc.put(cs[half]);
   };
@@ -484,15 +501,24 @@ __global__ __launch_bounds__(256) void k_scan_grad_carry(afc_scan_args P, Plan T
   const int first = at.first_chunk(T), live = at.live_end(T);
   Piece<DT, E, WHOLE> dt{}, z{}, dout{}, dta{}, za{}, douta{};
   const int64_t l0 = (int64_t)(live - 1) * K;
-  Rows<DT, S, NL> rc(P.c, at, l0);
-  Stream<DT> dts(P.dt, at.b, l0 + at.r, at.w0 + at.q), zs(P.z, at.b, l0 + at.r, at.w0 + at.q), douts(P.dy, at.b, l0 + at.r, at.w0 + at.q);
+  Rows<DT, S, NL> rc(P.c, at, l0, P.state);
+  const int64_t lr = l0 + at.r, wq = at.readable();
+  Stream<DT> dts(P.dt, at.b, lr, wq), zs(P.z, at.b, lr, wq), douts(P.dy, at.b, lr, wq);
   const bool gate = P.z.data, soft = P.softplus;
   auto fetch = [&](int ch) {
-    const int n = ch >= first && ch * K + at.r < at.len ? at.n : 0;
-    dta.load(dts.p, n);
-    za.load(zs.p, gate ? n : 0);
-    douta.load(douts.p, n);
-    rc.load(ch >= first ? at.len - ch * K : 0, P.state);
+    if (ch < first) return;
+    if (WHOLE && (ch + 1) * K <= at.len) {
+      dta.load_all(dts.p);
+      if (gate) za.load_all(zs.p);
+      douta.load_all(douts.p);
+      rc.load_all();
+    } else {
+      const int n = ch * K + at.r < at.len ? at.n : 0;
+      dta.load(dts.p, n);
+      if (gate) za.load(zs.p, n);
+      douta.load(douts.p, n);
+      rc.load(at.len - ch * K);
+    }
     dts.back(), zs.back(), douts.back(), rc.back();
   };
   auto take = [&] {
@@ -503,7 +529,7 @@ __global__ __launch_bounds__(256) void k_scan_grad_carry(afc_scan_args P, Plan T
   auto prepare = [&](int i, int ch) {
     const float v = dt[i] + bias[i], soft_v = softplus(v), d = dout[i], gated = d * silu(z[i]);
     step[i] = ch * K + at.r < at.len && i < at.n ? (soft ? soft_v : v) : 0.f;
-    dy[i] = gate ? gated : d;
+    dy[i] = i < at.n ? (gate ? gated : d) : 0.f;
   };
   auto put = [&](int half) {
 #pragma unroll
@@ -576,18 +602,28 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
   const int first = at.first_chunk(T), live = at.live_end(T), end = at.end_chunk(T);
   const bool gate = P.z.data, soft = P.softplus;
   Piece<DT, E, WHOLE> x{}, dt{}, z{}, dout{}, xa{}, dta{}, za{}, douta{};  // of the chunk that is prepared next, and of the one in front of it
-  const int64_t l0 = (int64_t)(live - 1) * K, lr = l0 + at.r, wq = at.w0 + at.q;
-  Rows<DT, S, NL> rb(P.b, at, l0), rc(P.c, at, l0);
-  Stream<DT> xs(P.x, at.b, lr, wq), dts(P.dt, at.b, lr, wq), zs(P.z, at.b, lr, wq), douts(P.dy, at.b, lr, wq), dxs(P.dx, at.b, lr, wq), ddts(P.ddt, at.b, lr, wq),
-      dzs(P.dz, at.b, lr, wq);
+  const int64_t l0 = (int64_t)(live - 1) * K, lr = l0 + at.r, wq = at.readable(), wo = at.w0 + at.q;
+  Rows<DT, S, NL> rb(P.b, at, l0, P.state), rc(P.c, at, l0, P.state);
+  Stream<DT> xs(P.x, at.b, lr, wq), dts(P.dt, at.b, lr, wq), zs(P.z, at.b, lr, wq), douts(P.dy, at.b, lr, wq), dxs(P.dx, at.b, lr, wo), ddts(P.ddt, at.b, lr, wo),
+      dzs(P.dz, at.b, lr, wo);
   auto fetch = [&](int ch) {
-    const int n = ch >= first && ch * K + at.r < at.len ? at.n : 0, rows = ch >= first ? at.len - ch * K : 0;
-    xa.load(xs.p, n);
-    dta.load(dts.p, n);
-    za.load(zs.p, gate ? n : 0);
-    douta.load(douts.p, n);
-    rb.load(rows, P.state);
-    rc.load(rows, P.state);
+    if (ch < first) return;
+    if (WHOLE && (ch + 1) * K <= at.len) {
+      xa.load_all(xs.p);
+      dta.load_all(dts.p);
+      if (gate) za.load_all(zs.p);
+      douta.load_all(douts.p);
+      rb.load_all();
+      rc.load_all();
+    } else {
+      const int n = ch * K + at.r < at.len ? at.n : 0, rows = at.len - ch * K;
+      xa.load(xs.p, n);
+      dta.load(dts.p, n);
+      if (gate) za.load(zs.p, n);
+      douta.load(douts.p, n);
+      rb.load(rows);
+      rc.load(rows);
+    }
     xs.back(), dts.back(), zs.back(), douts.back(), rb.back(), rc.back();
   };
   auto take = [&] {
@@ -604,12 +640,12 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
   auto prepare = [&](int i, int ch) {
     const float v = dt[i] + bias[i], soft_v = softplus(v), d = dout[i], gated = d * silu(z[i]);
     step[i] = ch * K + at.r < at.len && i < at.n ? (soft ? soft_v : v) : 0.f;
-    dy[i] = gate ? gated : d;
+    dy[i] = i < at.n ? (gate ? gated : d) : 0.f;
   };
   auto put = [&](int half) {
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      steps[half][at.r][at.q + i] = make_float2(step[i], step[i] * x[i]);
+      steps[half][at.r][at.q + i] = make_float2(step[i], i < at.n ? step[i] * x[i] : 0.f);
       dys[half][at.r][at.q + i] = dy[i];
     }
     rb.put(bs[half]);
@@ -656,7 +692,7 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
         dx[i] = on ? dx[i] : 0.f;
         ddt[i] = on ? ddt[i] : 0.f;
         dz[i] = on ? dz[i] : 0.f;
-        sum_d[i] = __builtin_fmaf(k2.dy[i], k2.x[i], sum_d[i]);
+        sum_d[i] = __builtin_fmaf(k2.dy[i], i < at.n ? k2.x[i] : 0.f, sum_d[i]);
         sum_b[i] += ddt[i];
       }
       store<DT, E, WHOLE>(dxs.p, dx, at.n);
@@ -805,25 +841,21 @@ __global__ __launch_bounds__(256) void k_scan_bc(afc_scan_args P, Plan T, const 
   if (n >= P.state) return;
   const float *from = bc + (row * T.tiles * P.length + l) * per + c * NP + n;
   float a = 0.f;
+#pragma unroll 8
   for (int t = 0; t < T.tiles; ++t) a += from[t * P.length * per];
   const afc_seq &s = c ? P.dc : P.db;
   ((E *)s.data)[b * s.stride_batch + l * s.stride_length + g * s.stride_group + n] = (E)a;
 }
 
-// da, dd, ddt_bias: the sums over rows and parts, 64 columns and four interleaved runs of rows in a block
-__global__ __launch_bounds__(256) void k_scan_params(afc_scan_args P, Sums sums, int64_t rows, int NP) {
-  __shared__ float red[256];
+// da, dd, ddt_bias: the sums over rows and parts, 64 columns a block
+__global__ __launch_bounds__(1024) void k_scan_params(afc_scan_args P, Sums sums, int64_t rows, int NP) {
+  __shared__ float red[1024];
   const int64_t na = P.width * NP, col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
   const int which = col < na ? 0 : col < na + P.width ? 1 : 2;
   const int64_t at = which == 0 ? col : col - na - (which - 1) * P.width, cols = which == 0 ? na : P.width;
   const float *from = which == 0 ? sums.a : which == 1 ? sums.d : sums.bias;
-  float a = 0.f;
-  if (at < cols)
-    for (int64_t r = threadIdx.x >> 6; r < rows; r += 4) a += from[r * cols + at];
-  red[threadIdx.x] = a;
-  __syncthreads();
+  const float a = column_sum(from, rows, cols, at, red);
   if (threadIdx.x >= 64 || at >= cols) return;
-  a = (red[threadIdx.x] + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]);
   if (which == 0) {
     if (P.da && at % NP < P.state) P.da[at / NP * P.state + at % NP] = a;
   } else if (which == 1) {
@@ -972,7 +1004,7 @@ struct Split {
 Split split(const afc_scan_args *p) {
   const int n = p->state;
   const int64_t wg = p->width / p->groups;
-  // groups of few channels: more lanes a channel instead of idle ones (37 x 7197 x 7, four groups, state 1: XXX us against 324)
+  // groups of few channels: more lanes a channel instead of idle ones (37 x 7197 x 7, four groups, state 1: 193 us against 324)
   if (n <= 16 && wg <= 16) return Split{1, 16};
   if (n <= 8 && wg <= 32) return Split{1, 8};
   return n <= 4 ? Split{1, 4} : n <= 8 ? Split{1, 8} : n <= 16 ? Split{2, 8} : n <= 32 ? Split{2, 16} : Split{4, 16};
@@ -1106,7 +1138,7 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   }
   if (p->da || p->dd || p->ddt_bias) {
     const dim3 gp((unsigned)ceil_div(p->width * (padded(p) + 2), 64));
-    k_scan_params<<<gp, 256, 0, st>>>(*p, sums, p->batch * t.segs, padded(p));
+    k_scan_params<<<gp, 1024, 0, st>>>(*p, sums, p->batch * t.segs, padded(p));
     launched("k_scan_params");
   }
 }

@@ -340,3 +340,26 @@ def test_no_cpu_fallback_of_the_library(lib):
         pytest.skip("GPU present")
     assert lib.afc_conv(C.byref(fake_conv()), None) == -2 and b"no HIP device" in lib.afc_ops_last_error()
     assert lib.afc_scan(C.byref(fake_scan()), None) == -2
+
+
+def test_overlaps_are_found_among_any_tensors(lib):
+    """the library's check of a few random ranges against every pair; an accepted call goes on to look for a device"""
+    import random
+    rng = random.Random(3)
+    seen = set()
+    for _ in range(400):
+        n = rng.randint(1, 4)
+        numel = [rng.randint(0, 6) for _ in range(n)]
+        ins = [4096 + 4 * rng.randint(0, 40) for _ in range(n)]
+        outs = [a if rng.random() < 0.4 else 4096 + 4 * rng.randint(0, 40) for a in ins]
+        spans = [(o, o + 4 * k, i, True) for i, (o, k) in enumerate(zip(outs, numel)) if k]
+        spans += [(a, a + 4 * k, i, False) for i, (a, o, k) in enumerate(zip(ins, outs, numel)) if k and a != o]
+        bad = any(p[0] < q[1] and q[0] < p[1] and (p[3] or q[3]) for x, p in enumerate(spans) for q in spans[:x])
+        keep = [(C.c_void_p * n)(*ins), (C.c_int64 * n)(*numel), (C.c_int32 * n)(), (C.c_void_p * n)(*outs)]
+        p = abi.ClipArgs()
+        p.device, p.count, p.norm, p.workspace, p.workspace_bytes, p.max_norm = 1 << 20, n, 4096, 1 << 30, 1 << 30, 1.0  # (no such device)
+        p.inp, p.numel, p.in_dtype, p.out, p.out_dtype = (C.addressof(keep[k]) for k in (0, 1, 2, 3, 2))
+        assert lib.afc_clip(C.byref(p), None) != 0
+        assert (b"overlap" in lib.afc_ops_last_error()) == bad, (ins, outs, numel)
+        seen.add(bad)
+    assert seen == {True, False}
