@@ -277,8 +277,7 @@ struct Scan : torch::autograd::Function<Scan> {
     const Tensor s = dense(state), n = dense(lengths);
     Tensor checkpoints;
     variable_list out = scan_forward(in, s, n, softplus, want_last, &checkpoints);
-    ctx->save_for_backward({in.x, in.dt, in.A, in.B, in.C, in.D, in.z, in.dt_bias, s, n});
-    ctx->saved_data["checkpoints"] = checkpoints;
+    ctx->save_for_backward({in.x, in.dt, in.A, in.B, in.C, in.D, in.z, in.dt_bias, s, n, checkpoints});
     ctx->saved_data["softplus"] = softplus;
     ctx->saved_data["wanted"] = wanted(x, dt, A, B, C, D, z, dt_bias, state);
     ctx->set_materialize_grads(false);
@@ -291,7 +290,7 @@ struct Scan : torch::autograd::Function<Scan> {
     if (!dy.defined() && !dlast.defined()) return out;
     const variable_list v = ctx->get_saved_variables();
     const ScanInputs in = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-    const Tensor &x = in.x, &state = v[8], &lengths = v[9], checkpoints = ctx->saved_data["checkpoints"].toTensor();
+    const Tensor &x = in.x, &state = v[8], &lengths = v[9], &checkpoints = v[10];
     dy = dy.defined() ? last_contiguous(dy) : at::zeros(x.sizes(), x.options());
     if (dlast.defined()) dlast = dlast.contiguous();
     out[0] = fresh(x), out[1] = fresh(in.dt), out[3] = fresh(in.B), out[4] = fresh(in.C);

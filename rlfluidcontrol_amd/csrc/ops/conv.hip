@@ -49,7 +49,8 @@ struct Tiling {
 
 // A thread takes T.run positions of V channels (16 bytes of a row): the filter and the last K - 1 inputs stay in registers, and
 // the next U positions are in flight while U are computed.  It reads and writes each element once (and K - 1 in front of each
-// run, mostly from cache): memory bounds it.
+// run, mostly from cache): memory bounds it.  3 x 8191 x 4096 bf16: 81 us, 5.0 TB/s (a copy: 5.1; runs of 8 positions loaded at
+// once and filters read for each, 124 us; 8 positions in flight, 90 us).
 template <int DT, int V, int K, bool SILU>
 __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
   typedef Elem<DT> E;
@@ -149,7 +150,9 @@ __global__ __launch_bounds__(256) void k_conv_step(afc_conv_args P) {
 
 // A thread takes T.run positions [s, e) of V channels.  It walks over the positions q = s .. e + K - 2 whose outputs its dx
 // depend on, with windows of the last K inputs and of the last K dp = dy f'(pre) in registers; dx[q - K + 1] is complete
-// when dp[q] is known.  dweight and dbias: sums of the thread, then of the block, one partial row for each block.
+// when dp[q] is known.  dweight and dbias: sums of the thread, then of the block, one partial row for each block, so that no
+// order of additions depends on timing.  Reads x and dy and writes dx once: 150 us for 3 x 8191 x 4096 bf16, 4.0 TB/s (without
+// the loads ahead 208 us, with four positions ahead 165: the windows of V channels and the filter's gradient fill the registers).
 template <int DT, int V, int K, bool SILU>
 __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, float *part) {
   typedef Elem<DT> E;

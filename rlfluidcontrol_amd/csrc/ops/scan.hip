@@ -5,10 +5,13 @@
 //   g[l] = dy C + exp(delta A)[l+1] g[l+1]     du = <g, B>     t = g exp(delta A) h[l-1]
 //   dx = du delta + D dy     ddelta = du x + <t, A>     dA = sum t delta     dB = sum_w g delta x     dC = sum_w dy h
 //
-// What bounds it: each of batch x length x width x state decays takes an exponential (16 clocks of a SIMD for 64 of them) and
-// four multiply-adds forwards, eight more backwards, while the tensors that are read and written are state times smaller.  So
-// the states stay in registers, everything that is the same for several states is computed once per position and channel and
-// handed over through LDS, and no instruction is spent on a state but the recurrence.
+// What bounds it: each of the batch x length x width x state decays takes an exponential (8 clocks of a SIMD for 64 of them) and
+// four other instructions (4 clocks each) forwards, and 3 + 8 and another exponential backwards, while the tensors that are read
+// and written are `state` times smaller.  So the states stay in registers, everything that is the same for several states is
+// computed once per position and channel and handed over through LDS, and little is spent on a state but the recurrence.
+// 8 x 2048 x 2048 x 16 in bf16: forwards 226 us, 2.4e12 states/s (the instructions above alone: 85 us; VALU busy 70 % at 2.3
+// GHz, 1.8 TB/s with the checkpoints), backwards 590 us (200 us; VALU busy 75 % at 2.2 GHz).  What both have to read and write
+// would take 106 us at a copy's rate.
 #include <stdexcept>
 
 #include "ops_common.h"
@@ -140,10 +143,6 @@ template <int S>
 struct States {
   typedef float V __attribute__((ext_vector_type(S)));
 };
-template <>
-struct States<1> {
-  typedef float V __attribute__((ext_vector_type(1)));
-};
 template <int S>
 __device__ inline void load_states(float *h, const float *p) {
   const typename States<S>::V v = *reinterpret_cast<const typename States<S>::V *>(p);
@@ -237,19 +236,6 @@ struct Rows {
       if (K * H::NP >= 256 * (i + 1) || threadIdx.x + 256 * i < K * H::NP) to[threadIdx.x + 256 * i] = on ? (float)v[i] : 0.f;
   }
 };
-
-// (all E of them side by side: a chain of transcendentals leaves room for three others)
-template <int E, class P>
-__device__ inline void step_sizes(float *step, const P &dt, const float *bias, bool soft, int n) {
-#pragma unroll
-  for (int i = 0; i < E; ++i) step[i] = dt[i] + bias[i];
-  if (soft) {
-#pragma unroll
-    for (int i = 0; i < E; ++i) step[i] = softplus(step[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < E; ++i) step[i] = i < n ? step[i] : 0.f;
-}
 
 // decays are computed as 2^(delta A log2 e)
 template <int S, int NL>
