@@ -385,7 +385,7 @@ def grads_of(sizes, dtypes, seed=0, scale=1.0):
 
 
 @pytest.mark.parametrize("dtypes", [[F32], [BF16], [F16], [F32, BF16, F16]])
-@pytest.mark.parametrize("sizes", [[1], [0, 3], [5, 64, 1, 0, 257], [1000, 33333, 7], [70001], [3] * 250 + [100000], [300001, 2, 65536, 65537], [0] + [17] * 110 + [0], [9000, 5] * 300])
+@pytest.mark.parametrize("sizes", [[1], [0, 3], [5, 64, 1, 0, 257], [1000, 33333, 7], [70001], [3] * 250 + [100000], [300001, 2, 65536, 65537], [0] + [17] * 110 + [0], [17] * 120, [17] * 121, [9000, 5] * 300])
 def test_clip(dtypes, sizes):
     grads = grads_of(sizes, dtypes)
     before = [g.clone() for g in grads]
