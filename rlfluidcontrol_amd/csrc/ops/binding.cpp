@@ -71,6 +71,28 @@ void no_grad(const T &...t) {
   TORCH_CHECK_VALUE(!wants_grad(t...), "a step has no gradient: call it under torch.no_grad(), or the whole-sequence form");
 }
 
+Tensor value(const Maybe &t) { return t ? *t : Tensor(); }
+// the bytes from a tensor's first element to its last
+struct Span {
+  uintptr_t from, to;
+  explicit Span(const Tensor &t) : from((uintptr_t)t.data_ptr()), to(from) {
+    if (t.numel() == 0) return;
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    to += (uintptr_t)(last + 1) * t.element_size();
+  }
+};
+// a state that is updated in place is read and written by many threads at once
+void own_memory(const Tensor &state, const char *name, const Tensor &t) {
+  if (!t.defined()) return;
+  const Span a(state), b(t);
+  TORCH_CHECK_VALUE(a.to <= b.from || b.to <= a.from, "state shares memory with ", name);
+}
+// what a kernel has written behind autograd's back: a graph that saved the old values refuses to use them
+void written(const Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor dense(const Maybe &t) { return t ? t->contiguous() : Tensor(); }
 Tensor last_contiguous(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
 template <class T = void>
@@ -97,7 +119,6 @@ afc_seq token(const Tensor &t) {  // [batch, width] or [batch, groups, state]
 Tensor fresh(const Tensor &like) { return at::empty(like.sizes(), like.options()); }
 Tensor fresh_if(const Tensor &like, bool wanted) { return like.defined() && wanted ? fresh(like) : Tensor(); }
 Tensor space(const Tensor &x, uint64_t bytes) { return at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)); }
-Tensor value(const Maybe &t) { return t ? *t : Tensor(); }
 
 void first_order_only() {
   TORCH_CHECK(!at::GradMode::is_enabled(), "the gradients of these operators have no gradient of their own (create_graph=True)");
@@ -187,6 +208,7 @@ Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weig
   check_filter(weight, bias, x.size(1), x.device());
   tensor("state", state, {x.size(0), weight.size(1) - 1, x.size(1)}, x.scalar_type(), x.device());
   TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous");
+  own_memory(state, "x", x), own_memory(state, "weight", weight), own_memory(state, "bias", value(bias));
   no_grad(x, state, weight, bias);
   const Tensor w = weight.contiguous(), b = dense(bias), y = at::empty(x.sizes(), x.options());
   afc_conv_args p = {};
@@ -199,6 +221,7 @@ Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weig
   p.weight = ptr<float>(w), p.bias = ptr<float>(b);
   p.initial_state = p.final_state = ptr(state);
   ok(afc_conv_step(&p, stream_of(x)));
+  written(state);
   return y;
 }
 
@@ -330,6 +353,8 @@ Tensor selective_scan_step(const Tensor &x, const Tensor &dt, const Tensor &A, c
   check_scan(in);
   tensor("state", state, {x.size(0), x.size(1), A.size(1)}, at::kFloat, x.device());
   TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous");
+  own_memory(state, "x", x), own_memory(state, "dt", dt), own_memory(state, "B", in.B), own_memory(state, "C", in.C), own_memory(state, "z", in.z);
+  own_memory(state, "A", A), own_memory(state, "D", in.D), own_memory(state, "dt_bias", in.dt_bias);
   no_grad(x, dt, A, B, C, state, D, z, dt_bias);
   const Tensor a = A.contiguous(), d = dense(D), bias = dense(dt_bias), y = at::empty(x.sizes(), x.options());
   afc_scan_args p = {};
@@ -342,6 +367,7 @@ Tensor selective_scan_step(const Tensor &x, const Tensor &dt, const Tensor &A, c
   p.a = ptr<float>(a), p.d = ptr<float>(d), p.dt_bias = ptr<float>(bias);
   p.initial_state = p.final_state = ptr<float>(state);
   ok(afc_scan_step(&p, stream_of(x)));
+  written(state);
   return y;
 }
 
@@ -387,6 +413,8 @@ Tensor clip(const std::vector<Tensor> &grads, double max_norm, const std::option
   const Tensor ws = space(norm, p.workspace_bytes);
   p.workspace = ptr(ws);
   ok(afc_clip(&p, stream_of(norm)));
+  if (scale)
+    for (const Tensor &t : out ? *out : grads) written(t);
   return norm;
 }
 

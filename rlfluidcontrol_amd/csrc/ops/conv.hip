@@ -290,8 +290,7 @@ void check_sizes(const afc_conv_args *p) {
   want(p != nullptr, "null arguments");
   want(p->dtype >= AFC_F32 && p->dtype <= AFC_F16, "dtype must be AFC_F32, AFC_BF16 or AFC_F16");
   want(p->taps >= 2 && p->taps <= 4, "taps must be 2, 3 or 4");
-  want(p->batch >= 0 && p->length >= 0 && p->width >= 1, "batch, length or width");
-  want(p->length < kMostAxis && p->width < kMostAxis && p->batch < kMostAxis, "an axis of 2^30 or more");
+  check_axes(p->batch, p->length, p->width);
 }
 
 void check(const afc_conv_args *p, bool grad, bool step) {

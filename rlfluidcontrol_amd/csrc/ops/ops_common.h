@@ -70,6 +70,14 @@ constexpr int64_t kMostAxis = (int64_t)1 << 30;  // indices along an axis, round
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline uint64_t up256(uint64_t n) { return (n + 255) & ~(uint64_t)255; }
 
+// Everything that is counted or laid out (blocks, partial sums, checkpoints: at most 512 bytes for an element of the sequence) stays
+// inside 63 bits
+inline void check_axes(int64_t batch, int64_t length, int64_t width) {
+  want(batch >= 0 && length >= 0 && width >= 1, "batch, length or width");
+  want(length < kMostAxis && width < kMostAxis && batch < kMostAxis, "an axis of 2^30 or more");
+  want((__int128)batch * (length > 0 ? length : 1) * width < (__int128)1 << 48, "more than 2^48 elements");
+}
+
 // a sequence tensor whose last element's offset stays far inside 63 bits
 inline void check_seq(const afc_seq &s, int64_t batch, int64_t length, int64_t groups, const char *why) {
   want(s.data != nullptr && s.stride_batch >= 0 && s.stride_length >= 0 && s.stride_group >= 0, why);
@@ -99,6 +107,12 @@ template <int DT>
 using Elem = typename ElemT<DT>::type;
 
 __device__ inline float exp_(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896341f); }
+// log2 e times a decay rate, finite from below: a rate of -inf forgets everything at any step size but zero, which is that of a
+// position behind a row's end
+__device__ inline float rate2(float a) {
+  const float r = a * 1.44269504088896341f;
+  return r < -3.4e38f ? -3.4e38f : r;
+}
 __device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + exp_(-v)); }
 __device__ inline float silu(float v) { return v * sigmoid(v); }
 // d/dv v sigmoid(v), with s = sigmoid(v)

@@ -243,7 +243,7 @@ __device__ inline void decay_rates(float *a2, const afc_scan_args &P, const Plac
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     const int n = at.nl * S + s;
-    a2[s] = at.cb < at.nw && n < P.state ? P.a[(at.w0 + at.cb) * P.state + n] * 1.44269504088896341f : 0.f;
+    a2[s] = at.cb < at.nw && n < P.state ? rate2(P.a[(at.w0 + at.cb) * P.state + n]) : 0.f;
   }
 }
 template <int S, int NL>
@@ -669,7 +669,8 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
 #pragma unroll
     for (int j = 0; j < NO; ++j) {
       const int i = threadIdx.x + 256 * j;
-      if (i < K * 2 * H::NP && ch * K + i / (2 * H::NP) < P.length) sums.bc[(bc_tile + ch * K) * 2 * H::NP + i] = bc[j];
+      const int lj = ch * K + i / (2 * H::NP);
+      if (i < K * 2 * H::NP && lj < P.length) sums.bc[(bc_tile + ch * K) * 2 * H::NP + i] = lj < at.len ? bc[j] : 0.f;
     }
     if (l < P.length) {
 #pragma unroll
@@ -895,7 +896,8 @@ __global__ __launch_bounds__(256) void k_scan_step4(afc_scan_args P, int tiles) 
   }
   F4 a2 = (F4)0.f;
   if (on) a2 = *reinterpret_cast<const F4 *>(P.a + w * P.state + n);
-  a2 *= 1.44269504088896341f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a2[i] = rate2(a2[i]);
   const float bias = P.dt_bias ? P.dt_bias[w] : 0.f, D = P.d ? P.d[w] : 0.f;
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -936,7 +938,7 @@ __global__ __launch_bounds__(64) void k_scan_step(afc_scan_args P) {
   if (mine) {
     const float B = (float)((const E *)P.b.data)[b * P.b.stride_batch + g * P.b.stride_group + n];
     const float C = (float)((const E *)P.c.data)[b * P.c.stride_batch + g * P.c.stride_group + n];
-    h = __builtin_fmaf(exp_(delta * P.a[w * P.state + n]), P.final_state[st], delta * x * B);
+    h = __builtin_fmaf(__builtin_amdgcn_exp2f(delta * rate2(P.a[w * P.state + n])), P.final_state[st], delta * x * B);
     P.final_state[st] = h;
     yc = C * h;
   }
@@ -953,8 +955,7 @@ void check_sizes(const afc_scan_args *p) {
   want(p != nullptr, "null arguments");
   want(p->dtype >= AFC_F32 && p->dtype <= AFC_F16, "dtype must be AFC_F32, AFC_BF16 or AFC_F16");
   want(p->state >= 1 && p->state <= 64, "state must be 1..64");
-  want(p->batch >= 0 && p->length >= 0 && p->width >= 1, "batch, length or width");
-  want(p->length < kMostAxis && p->width < kMostAxis && p->batch < kMostAxis, "an axis of 2^30 or more");
+  check_axes(p->batch, p->length, p->width);
   want(p->groups >= 1 && p->width % p->groups == 0, "groups must divide width");
 }
 
@@ -1007,7 +1008,8 @@ Plan plan(const afc_scan_args *p, bool grad) {
   // through a chunk of a block in 1.1 us with one block, in 0.76 us each with four (backwards, where registers allow two: 3.3
   // and 2.4 us), so they are made where there is less than a block for each of 256 CUs (backwards: one and a half).  1 x 8191 x
   // 2048 (64 blocks) takes 578 us whole, 182 in 8 parts, 160 in 16 and in 32; 5 x 1021 x 1000 with a state of 64 (320 blocks)
-  // 123 us whole and 130 in 4 parts; 4 x 4096 x 2048 (256 blocks) with gradients 1116 us whole and 1033 with two parts backwards.  Shorter than 128 positions a part does not pay.
+  // 123 us whole and 130 in 4 parts; 4 x 4096 x 2048 (256 blocks) with gradients 1116 us whole and 1033 with two parts backwards.  Shorter
+  // than 128 positions a part does not pay.
   int64_t segs = 1;
   if (blocks < (grad ? 384 : 256))
     while (blocks * segs < (grad ? 512 : 1024) && t.chunks / (segs * 2) >= 8) segs *= 2;
@@ -1094,6 +1096,8 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   check(p, true, false);
   const Plan t = plan(p, true);
   const Layout o = layout(p, t);
+  const int64_t n = ceil_div(p->batch * p->length * p->groups * 2 * padded(p), 256);
+  want(n < (int64_t)1 << 31, "too many blocks");
   if (p->batch > 0) check_workspace(p, o.all);
   want((uintptr_t)p->checkpoints % 16 == 0, "checkpoints must be 16-byte aligned");
   OnDevice on(p->device);
@@ -1101,7 +1105,7 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   const Carry carry = carry_at(p, t);
   const Sums sums = {(float *)(ws + o.bc), (float *)(ws + o.a), (float *)(ws + o.d), (float *)(ws + o.bias)};
   if (p->batch > 0) {
-      const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
+    const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
     if (t.segs > 1) {
 #define SCAN_GO(DT, S, NL, WHOLE, C) k_scan_grad_carry<DT, S, NL, WHOLE><<<grid, 256, 0, st>>>(*p, t, carry)
       SCAN_ALL(0)
@@ -1112,8 +1116,6 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
     SCAN_ALL(0)
 #undef SCAN_GO
     launched("k_scan_grad");
-    const int64_t n = ceil_div(p->batch * p->length * p->groups * 2 * padded(p), 256);
-    want(n < (int64_t)1 << 31, "too many blocks");
     if (n) {
       const dim3 gb((unsigned)n);
       if (p->dtype == AFC_F32) k_scan_bc<AFC_F32><<<gb, 256, 0, st>>>(*p, t, sums.bc, padded(p));

@@ -89,6 +89,22 @@ def _no_grad(*tensors):
             "a step has no gradient: call it under torch.no_grad(), or the whole-sequence form")
 
 
+def _span(t):
+    """the bytes from a tensor's first element to its last"""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _own_memory(state, **others):
+    lo, hi = _span(state)
+    for name, t in others.items():
+        if t is not None:
+            a, b = _span(t)
+            _refuse(hi <= a or b <= lo, "state shares memory with %s", name)
+
+
 # ---- short causal convolution ----
 
 def causal_conv(x, weight, bias=None, silu=False, initial_state=None, lengths=None, return_final_state=False):
@@ -121,7 +137,7 @@ def _filter(weight, bias, W, device):
 
 def causal_conv_step(x, state, weight, bias=None, silu=False):
     """One position of causal_conv for every row: x [batch, width] -> y [batch, width]; state [batch, taps-1, width]
-    (contiguous, x's type) moves on by x in place.  No gradient."""
+    (contiguous, x's type, memory of its own) moves on by x in place.  No gradient."""
     if _on_gpu(x):
         return _gpu().causal_conv_step(x, state, weight, bias, silu)
     _input(x, 2)
@@ -129,6 +145,7 @@ def causal_conv_step(x, state, weight, bias=None, silu=False):
     _filter(weight, bias, x.shape[1], x.device)
     _tensor("state", state, (x.shape[0], weight.shape[1] - 1, x.shape[1]), x.dtype, x.device)
     _refuse(state.is_contiguous(), "state must be contiguous")
+    _own_memory(state, x=x, weight=weight, bias=bias)
     _no_grad(x, state, weight, bias)
     y, last = _plain_conv(x[:, None], weight, bias, silu, state, None)
     state.copy_(last)
@@ -144,7 +161,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False,
 
     x, dt, z [batch, length, width]; A [width, state] float32, state 1..64; B, C [batch, length, state] or
     [batch, length, groups, state] of x's type, groups dividing width (channel w uses group g = w // (width // groups));
-    D, dt_bias [width] float32; initial_state [batch, width, state] float32 (default: zeros); lengths: see the module.
+    D, dt_bias [width] float32; initial_state [batch, width, state] float32 (default: zeros); lengths: see the module.  A rate
+    of -inf forgets everything at every step size but zero.
     Returns y, or (y, final_state).  Differentiable in everything but lengths, through y and final_state; a forward pass that
     will be differentiated also keeps states for the backward pass."""
     if _on_gpu(x):
@@ -187,13 +205,15 @@ def _scan_inputs(x, dt, A, B, C, D, z, dt_bias):
 
 def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, softplus=False):
     """One position of selective_scan for every row: x, dt, z [batch, width], B, C [batch, state] or [batch, groups, state]
-    -> y [batch, width]; state [batch, width, state] (contiguous, float32) moves on in place.  No gradient."""
+    -> y [batch, width]; state [batch, width, state] (contiguous, float32, memory of its own) moves on in place.  No
+    gradient."""
     if _on_gpu(x):
         return _gpu().selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, softplus)
     _input(x, 2)
     B, C, N = _scan_inputs(x, dt, A, B, C, D, z, dt_bias)
     _tensor("state", state, (x.shape[0], x.shape[1], N), torch.float32, x.device)
     _refuse(state.is_contiguous(), "state must be contiguous")
+    _own_memory(state, x=x, dt=dt, B=B, C=C, z=z, A=A, D=D, dt_bias=dt_bias)
     _no_grad(x, dt, A, B, C, state, D, z, dt_bias)
     y, last = _plain_scan(x[:, None], dt[:, None], A, B[:, None], C[:, None], D, z[:, None] if z is not None else None, dt_bias, softplus, state, None)
     state.copy_(last)
@@ -256,7 +276,21 @@ def _clip(grads, max_norm, out):
     for g, o in zip(grads, out or ()):
         _refuse(g.shape == o.shape and g.stride() == o.stride(), "an output has shape %s and strides %s, its gradient %s and %s",
                 tuple(o.shape), o.stride(), tuple(g.shape), g.stride())
+    if max_norm is not None:
+        _check_overlaps(grads, out or grads)
     return _plain_clip(grads, max_norm, out)
+
+
+def _check_overlaps(grads, out):
+    """as the library does: no element is written twice, or read after it was written"""
+    spans = sorted([_span(o) + (True,) for o in out] + [_span(g) + (False,) for g, o in zip(grads, out) if g.data_ptr() != o.data_ptr()])
+    end = {True: 0, False: 0}  # of the outputs and of the inputs so far
+    for lo, hi, written in spans:
+        if lo == hi:
+            continue
+        if lo < end[True] or (written and lo < end[False]):
+            raise OpsError("two tensors overlap")
+        end[written] = max(end[written], hi)
 
 
 # ---- the same formulas in plain torch, for tensors on the CPU ----
@@ -290,6 +324,7 @@ def _plain_scan(x, dt, A, B, C_, D, z, dt_bias, softplus, state, lengths):
     delta = _mask(lengths, L, v)
     per = W // B.shape[2]
     Bf, Cf = (_mask(lengths, L, t.float()).repeat_interleave(per, dim=2) for t in (B, C_))
+    A = torch.where(A < -3e38, -3e38, A)  # a rate of -inf forgets all at any step size but zero (behind a row's end)
     h = state if state is not None else xf.new_zeros(Bn, W, A.shape[1])
     ys = []
     for t in range(L):

@@ -4,7 +4,8 @@ import torch
 
 from rlfluidcontrol_amd import ops
 from tests import ops_reference as ref
-from tests.test_ops import check_conv, check_scan, conv_case, refusals_of_clip, refusals_of_conv, refusals_of_scan, scan_case
+from tests.test_ops import (check_conv, check_scan, conv_case, infinite_adjoints, rates_without_memory, refusals_of_clip, refusals_of_conv, refusals_of_scan,
+                            scan_case, states_of_their_own, updates_in_place)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -459,3 +460,21 @@ def test_clip_same_bits_every_time():
     grads = grads_of([1 << 20, 12345, 7], [F32, BF16])
     first = ops.grad_norm(grads)
     assert all(torch.equal(ops.grad_norm(grads), first) for _ in range(5))
+
+
+# ---- what shares memory, what is infinite ----
+
+def test_a_rate_without_memory():
+    rates_without_memory(DEV)
+
+
+def test_infinite_adjoints_stay_within_their_rows():
+    infinite_adjoints(DEV)
+
+
+def test_states_have_memory_of_their_own():
+    states_of_their_own(DEV)
+
+
+def test_autograd_sees_what_is_updated_in_place():
+    updates_in_place(DEV)

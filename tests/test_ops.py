@@ -363,3 +363,109 @@ def test_overlaps_are_found_among_any_tensors(lib):
         assert (b"overlap" in lib.afc_ops_last_error()) == bad, (ins, outs, numel)
         seen.add(bad)
     assert seen == {True, False}
+
+
+def test_more_elements_than_can_be_laid_out(lib):
+    n = C.c_uint64()
+    for axes, ok in (((1 << 29, 1 << 10, 1 << 9), False), ((1 << 20, 1 << 10, 1 << 18), False), ((1 << 29, 0, 1 << 20), False), ((1 << 10, 1 << 18, 1 << 10), True)):
+        a = abi.ConvArgs()
+        a.taps, a.batch, a.length, a.width = (4,) + axes
+        assert (lib.afc_conv_workspace(C.byref(a), C.byref(n)) == 0) == ok, axes
+    keep = [(C.c_void_p * 9)(*[4096] * 9), (C.c_int64 * 9)(*[(1 << 45) - 1] * 9), (C.c_int32 * 9)()]
+    for count, ok in ((8, True), (9, False)):
+        a = abi.ClipArgs()
+        a.count, a.inp, a.numel, a.in_dtype = (count,) + tuple(C.addressof(k) for k in keep)
+        assert (lib.afc_clip_workspace(C.byref(a), C.byref(n)) == 0) == ok, count
+
+
+# ---- what shares memory, what is infinite (on either device) ----
+
+def scan_results(c, softplus=True):
+    names = [n for n in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "state") if c[n] is not None]
+    leaves = {n: c[n].detach().clone().requires_grad_() for n in names}
+    args = [leaves.get(n) for n in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")]
+    y, last = ops.selective_scan(*args, softplus=softplus, initial_state=leaves.get("state"), lengths=c["lengths"], return_final_state=True)
+    grads = torch.autograd.grad([y, last], [leaves[n] for n in names], [c["dy"], c["dlast"]])
+    return dict(y=y.detach(), last=last.detach(), **{"d" + n: g for n, g in zip(names, grads)})
+
+
+def rates_without_memory(device):
+    """a rate of -inf is one so large that no step size leaves anything; behind a row's end the step size is zero, and the state stays"""
+    for N, W, L in ((16, 40, 37), (3, 8, 20), (64, 20, 300)):
+        c = scan_case(N, 3, L, W, N, device=device, lengths=[L, L - 5, 0])
+        big, inf = c["A"].clone(), c["A"].clone()
+        big[::3, ::2], inf[::3, ::2] = -1e30, float("-inf")
+        want, got = scan_results(dict(c, A=big)), scan_results(dict(c, A=inf))
+        for k in want:
+            assert bool(torch.isfinite(got[k]).all()) and torch.equal(want[k], got[k]), k
+        tokens = [c[k][:, 0] if c[k] is not None else None for k in ("x", "dt", "B", "C", "z")]
+        tokens[1] = torch.where(torch.arange(W, device=device) % 2 == 0, -1000.0, tokens[1])  # step sizes of zero
+        outs = []
+        for A in (big, inf):
+            h = c["state"].clone()
+            x, dt, B, Cm, z = tokens
+            outs.append((ops.selective_scan_step(x, dt, A, B, Cm, h, c["D"], z, c["dt_bias"], True), h))
+        assert all(bool(torch.isfinite(b).all()) and torch.equal(a, b) for a, b in zip(*outs))
+
+
+def infinite_adjoints(device):
+    c = scan_case(5, 2, 21, 16, 16, device=device, lengths=[4, 18])
+    c["dlast"][:, 0] = float("inf")
+    c["state"][0, 0, 0] = float("inf")
+    got = scan_results(c)
+    for k in ("dx", "ddt", "dB", "dC", "dz"):
+        for b, n in enumerate((4, 18)):
+            assert not bool(got[k][b, n:].any()) and not bool(got[k][b, n:].isnan().any()), k
+
+
+def states_of_their_own(device):
+    x, w = torch.randn(2, 8, device=device), torch.randn(8, 4, device=device)
+    memory = torch.randn(2, 3, 8, device=device)
+    keep = memory.clone()
+    for bad in (memory[:, 0], memory[:, 2], memory.view(-1)[1:17].view(2, 8)):
+        with pytest.raises(ValueError, match="state shares memory with x"):
+            ops.causal_conv_step(bad, memory, w)
+    with pytest.raises(ValueError, match="state shares memory with bias"):
+        ops.causal_conv_step(x, memory, w, memory.view(-1)[:8])
+    flat = torch.randn(200, device=device)
+    h, B = flat[:64].view(2, 8, 4), flat[64:72].view(2, 4)
+    A = -torch.rand(8, 4, device=device)
+    for kw, name in ((dict(B=flat[60:68].view(2, 4)), "B"), (dict(C=flat[:8].view(2, 4)), "C"), (dict(x=flat[:16].view(2, 8)), "x"), (dict(A=flat[32:64].view(8, 4)), "A"),
+                     (dict(D=flat[8:16]), "D"), (dict(z=flat[1:17].view(2, 8)), "z")):
+        with pytest.raises(ValueError, match="state shares memory with %s" % name):
+            ops.selective_scan_step(**{**dict(x=x, dt=x, A=A, B=B, C=B, state=h), **kw})
+    ops.selective_scan_step(x, x, A, B, B, h)  # neighbours in one buffer are no neighbours' memory
+    assert torch.equal(memory, keep)
+
+
+def updates_in_place(device):
+    x, w = torch.randn(2, 8, device=device), torch.randn(8, 4, device=device)
+    scale = torch.ones((), device=device, requires_grad=True)
+    token = torch.randn(2, 4, device=device)
+    for state, update in ((torch.randn(2, 3, 8, device=device), lambda s: ops.causal_conv_step(x, s, w)),
+                          (torch.randn(2, 8, 4, device=device), lambda s: ops.selective_scan_step(x, x, -w.abs(), token, token, s)),
+                          (torch.randn(50, device=device), lambda s: ops.clip_grad_norm([s], 0.1))):
+        saved = (state * scale).sum()  # the backward pass needs the state as it is
+        with torch.no_grad():
+            update(state)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.backward()
+    with torch.inference_mode():
+        state = torch.zeros(2, 3, 8, device=device)
+        ops.causal_conv_step(x, state, w)
+        assert torch.equal(state[:, -1], x)
+
+
+@pytest.mark.parametrize("which", [rates_without_memory, infinite_adjoints, states_of_their_own, updates_in_place])
+def test_on_the_cpu(which):
+    which("cpu")
+
+
+def test_plain_clip_refuses_tensors_that_overlap():
+    a = torch.ones(100)
+    for grads, out in (([a, a], None), ([a[:60], a[50:]], None), ([a[:50]], [a[25:75]])):
+        with pytest.raises(ops.OpsError, match="overlap"):
+            ops.clip_grad_norm(grads, 1.0, out=out)
+    assert torch.equal(a, torch.ones(100))
+    ops.clip_grad_norm([a[50:], a[:50], a[50:50]], 1.0)
+    assert abs(float(a.norm()) - 1) < 1e-5 and abs(float(ops.grad_norm([a, a])) - 2 ** 0.5) < 1e-5
