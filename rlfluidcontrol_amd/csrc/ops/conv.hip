@@ -1,5 +1,6 @@
 // conv.hip -- short causal convolution along the sequence (afc_conv, afc_conv_grad, afc_conv_step)
 #include <stdexcept>
+#include <type_traits>
 
 #include "ops_common.h"
 
@@ -38,6 +39,7 @@ struct Raw {
     v = (Vec<DT, V>)(Elem<DT>)0.f;
     if (on) v = *reinterpret_cast<const Vec<DT, V> *>(p);
   }
+  __device__ inline void load_all(const Elem<DT> *p) { v = *reinterpret_cast<const Vec<DT, V> *>(p); }
   __device__ inline float operator[](int i) const { return (float)v[i]; }
 };
 
@@ -151,8 +153,10 @@ __global__ __launch_bounds__(256) void k_conv_step(afc_conv_args P) {
 // A thread takes T.run positions [s, e) of V channels.  It walks over the positions q = s .. e + K - 2 whose outputs its dx
 // depend on, with windows of the last K inputs and of the last K dp = dy f'(pre) in registers; dx[q - K + 1] is complete
 // when dp[q] is known.  dweight and dbias: sums of the thread, then of the block, one partial row for each block, so that no
-// order of additions depends on timing.  Reads x and dy and writes dx once: 150 us for 3 x 8191 x 4096 bf16, 4.0 TB/s (without
-// the loads ahead 208 us, with four positions ahead 165: the windows of V channels and the filter's gradient fill the registers).
+// order of additions depends on timing.  Reads x and dy and writes dx once: 148 us for 3 x 8191 x 4096 bf16, 4.1 TB/s (the
+// 21 instructions an element would take some 65 us; without the loads ahead 208 us, with one or four positions ahead 160 and 152,
+// half or twice the run or the four waves side by side 148 to 160).  Positions whose neighbours all lie inside the run and the
+// row go without conditions: 40 instructions an element fall to 21, the time by 2 us of 150 where memory bounds it.
 template <int DT, int V, int K, bool SILU>
 __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, float *part) {
   typedef Elem<DT> E;
@@ -166,13 +170,13 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
   int64_t c = (ct * cx + lane_c) * V;
   const bool inside = c < P.width;
   c = inside ? min(c, P.width - V) : c;  // (the last vector ends with the row: what two lanes share both write, the same)
-  const int64_t s = (lt * ty + lane_l) * (int64_t)T.run;
+  const int64_t s64 = (lt * ty + lane_l) * (int64_t)T.run;
   const int len = row_length(P.lengths, b, P.length);
   float dw[K + 1][V];
   for (int k = 0; k <= K; ++k)
     for (int i = 0; i < V; ++i) dw[k][i] = 0.f;
-  if (inside && (s < P.length || s == 0)) {
-    const int64_t e = s + T.run < P.length ? s + T.run : P.length;
+  if (inside && (s64 < P.length || s64 == 0)) {
+    const int s = (int)s64, e = (int)min(s64 + T.run, P.length);
     const E *x = (const E *)P.x.data + b * P.x.stride_batch + c;
     const E *dy = (const E *)P.dy.data + b * P.dy.stride_batch + c;
     E *dx = (E *)P.dx.data + b * P.dx.stride_batch + c;
@@ -187,7 +191,7 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
 #pragma unroll
     for (int j = 0; j < K; ++j) {
       for (int i = 0; i < V; ++i) xw[j][i] = dp[j][i] = 0.f;
-      const int64_t p = s + j - K;  // xw[1..K-1]: positions s-K+1 .. s-1 (moved down by one at the first step)
+      const int p = s + j - K;  // xw[1..K-1]: positions s-K+1 .. s-1 (moved down by one at the first step)
       if (j > 0 && p < 0) {
         if (s0) load<DT, V>(xw[j], s0 + (p + K - 1) * P.width);
       } else if (j > 0 && p < len) {
@@ -195,30 +199,36 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
       }
     }
     constexpr int U = 2;
-    const int64_t last = e + K - 1;
+    const int last = e + K - 1, loads = min(len, last), inner = min(len, e);
     const E *xq = x + s * P.x.stride_length, *dq = dy + s * P.dy.stride_length;
+    E *dxl = dx + (int64_t)(s - (K - 1)) * P.dx.stride_length;
     Raw<DT, V> xa[U], da[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      xa[j].load(xq + j * P.x.stride_length, s + j < len && s + j < last);
-      da[j].load(dq + j * P.dy.stride_length, s + j < len && s + j < last);
+      xa[j].load(xq + j * P.x.stride_length, s + j < loads);
+      da[j].load(dq + j * P.dy.stride_length, s + j < loads);
     }
-    for (int64_t q0 = s; q0 < last; q0 += U) {
+    auto positions = [&](auto whole, int q0) {
+      constexpr bool WHOLE = decltype(whole)::value;
       xq += U * P.x.stride_length, dq += U * P.dy.stride_length;
       Raw<DT, V> xn[U], dn[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) xn[j] = xa[j], dn[j] = da[j];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        xa[j].load(xq + j * P.x.stride_length, q0 + U + j < len && q0 + U + j < last);
-        da[j].load(dq + j * P.dy.stride_length, q0 + U + j < len && q0 + U + j < last);
+        if (WHOLE) {
+          xa[j].load_all(xq + j * P.x.stride_length);
+          da[j].load_all(dq + j * P.dy.stride_length);
+        } else {
+          xa[j].load(xq + j * P.x.stride_length, q0 + U + j < loads);
+          da[j].load(dq + j * P.dy.stride_length, q0 + U + j < loads);
+        }
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int64_t q = q0 + j, l = q - (K - 1), jf = l - len + K - 1;
-        const bool live = q < len;
+        const int q = q0 + j, l = q - (K - 1), jf = q - len;
         float v[V] = {};
-        if (df && jf >= 0 && jf < K - 1 && q < last) load<DT, V>(v, df + jf * P.width);
+        if (!WHOLE && df && jf >= 0 && jf < K - 1 && q < last) load<DT, V>(v, df + jf * P.width);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -233,21 +243,27 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
             for (int k = 0; k < K; ++k) a = __builtin_fmaf(w[k][i], xw[k][i], a);
             d *= silu_slope(a, sigmoid(a));
           }
-          d = live ? d : 0.f;
+          d = WHOLE || q < len ? d : 0.f;
           dp[K - 1][i] = d;
-          const float own = q < e ? d : 0.f;
+          const float own = WHOLE || q < e ? d : 0.f;
           for (int k = 0; k < K; ++k) dw[k][i] = __builtin_fmaf(own, xw[k][i], dw[k][i]);
           dw[K][i] += own;
-          for (int k = 0; k < K; ++k) v[i] = __builtin_fmaf(w[k][i], dp[K - 1 - k][i], v[i]);
-          v[i] = l < len ? v[i] : 0.f;
+          for (int k = 0; k < K; ++k) v[i] = WHOLE && k == 0 ? w[0][i] * dp[K - 1][i] : __builtin_fmaf(w[k][i], dp[K - 1 - k][i], v[i]);
+          v[i] = WHOLE || l < len ? v[i] : 0.f;
         }
-        if (q >= last || (l < s && (l >= 0 || s > 0))) continue;
-        if (l < 0) {
+        if (WHOLE || (q < last && l >= s)) {
+          store<DT, V>(dxl, v);
+        } else if (q < last && l < 0 && s == 0) {
           if (ds) store<DT, V>(ds + (l + K - 1) * P.width, v);
-        } else {
-          store<DT, V>(dx + l * P.dx.stride_length, v);
         }
+        dxl += P.dx.stride_length;
       }
+    };
+    for (int q0 = s; q0 < last; q0 += U) {
+      if (q0 >= s + K - 1 && q0 + 2 * U <= inner)
+        positions(std::true_type(), q0);
+      else
+        positions(std::false_type(), q0);
     }
   }
   if (!part) return;
