@@ -121,11 +121,17 @@ __device__ inline float silu_slope(float v, float s) { return s * __builtin_fmaf
 // log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1].  Step sizes near 1e-3 come out of e near 1e-3, where
 // log(1 + e) would keep only the digits of e that 1 + e keeps (relative error 6e-5): Kahan's log1p, log(w) e / (w - 1) with
 // w = 1 + e as rounded, has the full 24 bits.  No threshold is needed: for large v the sum is v.
-__device__ inline float softplus(float v) {
+// `slope`: sigmoid(v), out of the same exponential.
+__device__ inline float softplus(float v, float &slope) {
   const float e = exp_(-__builtin_fabsf(v));
   const float w = 1.f + e, dw = w - 1.f;
   const float l = __builtin_amdgcn_logf(w) * 0.693147180559945309f * (e * __builtin_amdgcn_rcpf(dw));
+  slope = __builtin_amdgcn_rcpf(w) * (v < 0.f ? e : 1.f);
   return fmaxf(v, 0.f) + (dw == 0.f ? e : l);
+}
+__device__ inline float softplus(float v) {
+  float slope;
+  return softplus(v, slope);
 }
 
 // Sum of a column over many rows by a block of 1024: 64 columns, 16 interleaved runs of rows with four sums each in flight, added

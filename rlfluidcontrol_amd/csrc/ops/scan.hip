@@ -9,8 +9,8 @@
 // four other instructions (4 clocks each) forwards, and 3 + 8 and another exponential backwards, while the tensors that are read
 // and written are `state` times smaller.  So the states stay in registers, everything that is the same for several states is
 // computed once per position and channel and handed over through LDS, and little is spent on a state but the recurrence.
-// 8 x 2048 x 2048 x 16 in bf16: forwards 226 us, 2.4e12 states/s (the instructions above alone: 85 us; VALU busy 70 % at 2.3
-// GHz, 1.8 TB/s with the checkpoints), backwards 590 us (200 us; VALU busy 75 % at 2.2 GHz).  What both have to read and write
+// 8 x 2048 x 2048 x 16 in bf16: forwards 212 to 225 us, 2.4e12 states/s (the instructions above alone: 85 us; VALU busy 70 % at 2.3
+// GHz, 1.8 TB/s with the checkpoints), backwards 545 to 585 us (200 us; VALU busy 78 % at 2.2 GHz).  What both have to read and write
 // would take 106 us at a copy's rate.
 #include <stdexcept>
 
@@ -622,9 +622,11 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
     for (int s = 0; s < S; ++s) h0[s] = 0.f;
     if (ch >= first && at.cb < at.nw) load_states<S>(h0, P.checkpoints + (((int64_t)at.b * T.chunks + ch) * P.width + w) * H::NP + at.nl * S);
   };
-  float step[E], dy[E];
+  float step[E], dy[E], sz[E], slope[E];  // sz: sigmoid(z); slope: of the softplus
   auto prepare = [&](int i, int ch) {
-    const float v = dt[i] + bias[i], soft_v = softplus(v), d = dout[i], gated = d * silu(z[i]);
+    const float v = dt[i] + bias[i], soft_v = softplus(v, slope[i]), d = dout[i];
+    sz[i] = sigmoid(z[i]);
+    const float gated = d * z[i] * sz[i];
     step[i] = ch * K + at.r < at.len && i < at.n ? (soft ? soft_v : v) : 0.f;
     dy[i] = i < at.n ? (gate ? gated : d) : 0.f;
   };
@@ -639,22 +641,24 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
   };
   // the chunk in the recurrence, and the one behind it
   struct Kept {
-    Piece<DT, E, WHOLE> x, dt, z, dout;
-    float step[E], dy[E];
+    Piece<DT, E, WHOLE> x, z, dout;
+    float step[E], dy[E], sz[E], slope[E];
   } k1{}, k2{};
   auto keep = [&] {
     k2 = k1;
-    k1.x = x, k1.dt = dt, k1.z = z, k1.dout = dout;
+    k1.x = x, k1.z = z, k1.dout = dout;
 #pragma unroll
-    for (int i = 0; i < E; ++i) k1.step[i] = step[i], k1.dy[i] = dy[i];
+    for (int i = 0; i < E; ++i) {
+      k1.step[i] = step[i], k1.dy[i] = dy[i], k1.sz[i] = sz[i], k1.slope[i] = slope[i];
+    }
   };
   float dx[E], ddt[E], dz[E], bc[NO];
   auto finish = [&](int i, int half) {
     const float du = dus[at.r][at.q + i], ta = tas[at.r][at.q + i], y = ys[half][at.r][at.q + i], xi = k2.x[i], zi = k2.z[i];
-    const float slope = sigmoid(k2.dt[i] + bias[i]), d = __builtin_fmaf(du, xi, ta * 0.693147180559945309f);
+    const float d = __builtin_fmaf(du, xi, ta * 0.693147180559945309f);
     dx[i] = __builtin_fmaf(du, k2.step[i], D[i] * k2.dy[i]);
-    ddt[i] = soft ? slope * d : d;
-    dz[i] = k2.dout[i] * __builtin_fmaf(D[i], xi, y) * silu_slope(zi, sigmoid(zi));
+    ddt[i] = soft ? k2.slope[i] * d : d;
+    dz[i] = k2.dout[i] * __builtin_fmaf(D[i], xi, y) * silu_slope(zi, k2.sz[i]);
   };
   auto finish_bc = [&] {
 #pragma unroll
@@ -663,30 +667,37 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
       bc[j] = K * 2 * H::NP >= 256 * (j + 1) || i < K * 2 * H::NP ? (part[0][i] + part[1][i]) + (part[2][i] + part[3][i]) : 0.f;
     }
   };
-  const int64_t bc_tile = (((int64_t)at.b * P.groups + at.g) * T.tiles + at.tile) * P.length;
+  const int length = (int)P.length;
+  float *const bc_rows = sums.bc + (((int64_t)at.b * P.groups + at.g) * T.tiles + at.tile) * P.length * 2 * H::NP + threadIdx.x;
+  float *bc_to = bc_rows + (int64_t)(live - 1) * K * 2 * H::NP;
+  const bool gate_grad = P.dz.data;
   auto put_grads = [&](int ch) {
     const int l = ch * K + at.r;
+    if ((ch + 1) * K > at.len) {  // the row ends here: what lies behind it is zero
 #pragma unroll
-    for (int j = 0; j < NO; ++j) {
-      const int i = threadIdx.x + 256 * j;
-      const int lj = ch * K + i / (2 * H::NP);
-      if (i < K * 2 * H::NP && lj < P.length) sums.bc[(bc_tile + ch * K) * 2 * H::NP + i] = lj < at.len ? bc[j] : 0.f;
-    }
-    if (l < P.length) {
+      for (int j = 0; j < NO; ++j) bc[j] = ch * K + (int)(threadIdx.x + 256 * j) / (2 * H::NP) < at.len ? bc[j] : 0.f;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        const bool on = l < at.len;
-        dx[i] = on ? dx[i] : 0.f;
-        ddt[i] = on ? ddt[i] : 0.f;
-        dz[i] = on ? dz[i] : 0.f;
-        sum_d[i] = __builtin_fmaf(k2.dy[i], i < at.n ? k2.x[i] : 0.f, sum_d[i]);
-        sum_b[i] += ddt[i];
+        dx[i] = l < at.len ? dx[i] : 0.f;
+        ddt[i] = l < at.len ? ddt[i] : 0.f;
+        dz[i] = l < at.len ? dz[i] : 0.f;
       }
-      store<DT, E, WHOLE>(dxs.p, dx, at.n);
-      store<DT, E, WHOLE>(ddts.p, ddt, at.n);
-      if (P.dz.data) store<DT, E, WHOLE>(dzs.p, dz, at.n);
     }
+    const int left = length - ch * K;  // positions that the tensors have
+#pragma unroll
+    for (int j = 0; j < NO; ++j)
+      if ((int)threadIdx.x + 256 * j < (left < K ? left : K) * 2 * H::NP) bc_to[256 * j] = bc[j];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      sum_d[i] = __builtin_fmaf(k2.dy[i], i < at.n ? k2.x[i] : 0.f, sum_d[i]);
+      sum_b[i] += ddt[i];
+    }
+    const int n = at.r < left ? at.n : 0;
+    store<DT, E, WHOLE>(dxs.p, dx, n);
+    store<DT, E, WHOLE>(ddts.p, ddt, n);
+    if (gate_grad) store<DT, E, WHOLE>(dzs.p, dz, n);
     dxs.back(), ddts.back(), dzs.back();
+    bc_to -= K * 2 * H::NP;
   };
   {  // behind the row's end
     const float zero[E] = {};
@@ -695,10 +706,10 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
       if (ch * K + at.r < P.length) {
         store<DT, E, WHOLE>(dxs.p, zero, at.n);
         store<DT, E, WHOLE>(ddts.p, zero, at.n);
-        if (P.dz.data) store<DT, E, WHOLE>(dzs.p, zero, at.n);
+        if (gate_grad) store<DT, E, WHOLE>(dzs.p, zero, at.n);
       }
       for (int i = threadIdx.x; i < K * 2 * H::NP; i += 256)
-        if (ch * K + i / (2 * H::NP) < P.length) sums.bc[(bc_tile + ch * K) * 2 * H::NP + i] = 0.f;
+        if (ch * K + i / (2 * H::NP) < length) bc_rows[(int64_t)ch * K * 2 * H::NP + i - threadIdx.x] = 0.f;
     }
     for (int ch = live; ch < end; ++ch) dxs.back(), ddts.back(), dzs.back();
   }
