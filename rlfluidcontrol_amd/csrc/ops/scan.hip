@@ -1015,15 +1015,27 @@ Plan plan(const afc_scan_args *p, bool grad) {
   t.tiles = (int)ceil_div(p->width / p->groups, cb);
   t.chunks = (int)ceil_div(p->length, K);
   const int64_t blocks = p->batch * p->groups * t.tiles;
-  // Parts cost a pass of their own for the carries: two thirds of the forward pass, a fifth of the backward one.  A CU gets
-  // through a chunk of a block in 1.1 us with one block, in 0.76 us each with four (backwards, where registers allow two: 3.3
-  // and 2.4 us), so they are made where there is less than a block for each of 256 CUs (backwards: one and a half).  1 x 8191 x
-  // 2048 (64 blocks) takes 578 us whole, 182 in 8 parts, 160 in 16 and in 32; 5 x 1021 x 1000 with a state of 64 (320 blocks)
-  // 123 us whole and 130 in 4 parts; 4 x 4096 x 2048 (256 blocks) with gradients 1116 us whole and 1033 with two parts backwards.  Shorter
-  // than 128 positions a part does not pay.
+  // Parts run at the same time, and cost a pass of their own for the carries.  Their number is what an estimate likes best, in us:
+  // a chunk of each of n blocks on a CU takes 0.45 + 0.65 n (up to four at once), backwards 1.8 + 1.5 n (two, or one with four
+  // states a lane, whose registers fill a SIMD); the carries add two thirds of the forward pass and a quarter of the backward one,
+  // 5 and 7 for another launch and start, and 0.2 for each part that the last one has to take up.
+  //   1 x 8191 x 2048 (64 blocks) forwards: 578 us whole, 182 in 8 parts, 160 in 16 and in 32
+  //   1 x 8191 x 32 (1 block) forwards: 41 us in 256 parts, 29 in 64 and in 128
+  //   1 x 1000 x 1024 (32 blocks) both ways: 112 us in 4 parts, 70 in 8, 60 in 16
+  //   8 x 128 x 256 (64 blocks) both ways: 43 us whole, 41 in 2 parts, 31 in 4
+  //   8 x 128 x 700 (176 blocks) both ways: 48 us whole, 57 in 2 parts
+  //   3 x 900 x 1500 (141 blocks) both ways: 239 us whole, 197 in 8 and 4 parts
+  //   4 x 4096 x 2048 (256 blocks) both ways: 1116 us whole, 1033 with two parts backwards
+  const int64_t most = grad ? 512 : 1024, resident = !grad ? 4 : split(p).s == 4 ? 1 : 2;
+  const auto chunk = [&](int64_t n) { return n == 0 ? 0. : grad ? 1.8 + 1.5 * (double)n : 0.45 + 0.65 * (double)n; };
+  const auto estimate = [&](int64_t segs) {
+    const int64_t n = ceil_div(blocks * segs, 256);
+    const double whole = (double)ceil_div(t.chunks, segs) * ((double)(n / resident) * chunk(resident) + chunk(n % resident));
+    return segs == 1 ? whole : (grad ? whole * 1.25 + 7 : whole * 1.67 + 5) + 0.2 * (double)segs;
+  };
   int64_t segs = 1;
-  if (blocks < (grad ? 384 : 256))
-    while (blocks * segs < (grad ? 512 : 1024) && t.chunks / (segs * 2) >= 8) segs *= 2;
+  for (int64_t s = 2; blocks * (s / 2) < most && t.chunks / s >= 2; s *= 2)
+    if (estimate(s) < estimate(segs)) segs = s;
   t.seg_chunks = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, segs);
   t.segs = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, t.seg_chunks);
   want(blocks * t.segs < (int64_t)1 << 31, "too many blocks");

@@ -142,6 +142,14 @@ def test_scan_long(B, L, W, N, G, lengths):
     check_scan(scan_case(L, B, L, W, N, G, F32, DEV, lengths), True)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("B,L,W,N,G,lengths", [(1, 520, 17, 16, 1, [519]), (4, 260, 24, 12, 2, [260, 17, 16, 0]), (2, 200, 33, 64, 1, [200, 33]), (1, 4100, 8, 2, 1, None),
+                                               (7, 97, 40, 5, 1, [97, 96, 32, 31, 33, 1, 64]), (1, 2100, 32, 64, 1, [1500])])
+def test_scan_in_short_parts(dtype, B, L, W, N, G, lengths):
+    """few rows: the length is cut into parts of few chunks, of which some lie behind a row's end"""
+    check_scan(scan_case(L + N, B, L, W, N, G, dtype, DEV, lengths), True)
+
+
 def test_scan_of_no_length_and_no_rows():
     c = scan_case(3, 2, 0, 8, 4, 1, F32, DEV)
     r = check_scan(c, True)
