@@ -486,3 +486,45 @@ def test_states_have_memory_of_their_own():
 
 def test_autograd_sees_what_is_updated_in_place():
     updates_in_place(DEV)
+
+
+def test_calls_from_several_threads():
+    """each thread on a stream of its own, with refused calls in between: results and messages are the thread's own"""
+    import threading
+    cases = [(conv_case(k, 2, 30 + k, 40, 4, F32, DEV), scan_case(k, 2, 30 + k, 40, 16, 1, F32, DEV)) for k in range(4)]
+
+    def work(k):
+        c, s = cases[k]
+        x = s["x"].detach().clone().requires_grad_()
+        y = ops.selective_scan(x, s["dt"], s["A"], s["B"], s["C"], s["D"], s["z"], s["dt_bias"], True, s["state"])
+        dx, = torch.autograd.grad(y, [x], [s["dy"]])
+        g = [c["dy"].clone(), dx.clone()]
+        return [ops.causal_conv(c["x"], c["weight"], c["bias"], True, c["state"]), y.detach(), dx, ops.clip_grad_norm(g, 0.1)] + g
+
+    want = [work(k) for k in range(4)]
+    torch.cuda.synchronize()
+    got, failures = [None] * 4, []
+
+    def run(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    out = work(k)
+                    with pytest.raises(ops.OpsError, match="overlap"):
+                        ops.clip_grad_norm([out[1], out[1]], 1.0)
+                    with pytest.raises(ValueError, match="weight"):
+                        ops.causal_conv(cases[k][0]["x"], cases[k][0]["weight"][:, :1])
+            stream.synchronize()
+            got[k] = out
+        except BaseException as e:  # noqa: B902  (a thread's failure is the test's)
+            failures.append(e)
+
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
