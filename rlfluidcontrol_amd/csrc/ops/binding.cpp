@@ -86,7 +86,7 @@ struct Span {
 void own_memory(const Tensor &state, const char *name, const Tensor &t) {
   if (!t.defined()) return;
   const Span a(state), b(t);
-  TORCH_CHECK_VALUE(a.to <= b.from || b.to <= a.from, "state shares memory with ", name);
+  TORCH_CHECK_VALUE(a.from == a.to || b.from == b.to || a.to <= b.from || b.to <= a.from, "state shares memory with ", name);
 }
 // what a kernel has written behind autograd's back: a graph that saved the old values refuses to use them
 void written(const Tensor &t) {

@@ -27,15 +27,17 @@ struct Part {
 // The tables of pointers travel in kernel arguments (at most 4 KB a launch): no copy that would have to outlive the call, and a
 // captured launch carries its own.  Up to kTensors tensors go with the launches that use them; of more, launches of k_table lay
 // down a table in the workspace first, so that one launch each runs over all of them (678 tensors of 40 x 40 and smaller:
-// 134 us a call against 142 with a pair of launches for every 110, most of it the host's 0.1 us a tensor).
-constexpr int kTensors = 120;
+// 134 us a call against 142 with a pair of launches for every 110, most of it the host's 0.1 us a tensor).  Up to kFew tensors take
+// a small table: 4 KB of arguments cost the host half a microsecond a launch (12 tensors: 10.6 us a call against 11.4).
+constexpr int kTensors = 120, kFew = 24;
 
+template <int MOST>
 struct Batch {
-  const void *in[kTensors];
-  void *out[kTensors];
-  int64_t numel[kTensors];
-  int32_t first[kTensors + 1];  // the first block of each tensor
-  uint8_t in_dtype[kTensors], out_dtype[kTensors];
+  const void *in[MOST];
+  void *out[MOST];
+  int64_t numel[MOST];
+  int32_t first[MOST + 1];  // the first block of each tensor
+  uint8_t in_dtype[MOST], out_dtype[MOST];
   int32_t count;
   int64_t chunk;  // elements of a block
 
@@ -73,7 +75,7 @@ struct Table {
 };
 
 // one block for each tensor of a batch
-__global__ __launch_bounds__(64) void k_table(Batch B, Table T, int base, int first) {
+__global__ __launch_bounds__(64) void k_table(Batch<kTensors> B, Table T, int base, int first) {
   const int t = blockIdx.x;
   if (threadIdx.x == 0) T.entries[base + t] = {B.in[t], B.out[t], B.numel[t], first + B.first[t], B.in_dtype[t], B.out_dtype[t]};
   for (int i = B.first[t] + threadIdx.x; i < B.first[t + 1]; i += 64) T.tensor_of[first + i] = base + t;
@@ -283,19 +285,20 @@ Layout layout(const afc_clip_args *p) {
   return o;
 }
 
-std::vector<Batch> batches(const afc_clip_args *p) {
-  std::vector<Batch> all;
+template <int MOST>
+std::vector<Batch<MOST>> batches(const afc_clip_args *p) {
+  std::vector<Batch<MOST>> all;
   const int64_t chunk = chunk_of(p);
   int64_t blocks = 0;
   for (int i = 0; i < p->count; ++i) {
     if (p->numel[i] == 0) continue;
-    if (all.empty() || all.back().count == kTensors) {
+    if (all.empty() || all.back().count == MOST) {
       all.emplace_back();
       all.back().count = 0;
       all.back().chunk = chunk;
       blocks = 0;
     }
-    Batch &t = all.back();
+    Batch<MOST> &t = all.back();
     const int k = t.count++;
     t.in[k] = p->in[i];
     t.out[k] = p->out ? p->out[i] : nullptr;
@@ -342,11 +345,15 @@ void clip(const afc_clip_args *p, hipStream_t st) {
   want(p->workspace && p->workspace_bytes >= o.all && (uintptr_t)p->workspace % 256 == 0, "workspace is missing, too small or not 256-byte aligned");
   OnDevice on(p->device);
   char *ws = (char *)p->workspace;
-  const std::vector<Batch> all = batches(p);
+  if (p->count > 0 && p->count <= kFew) {
+    const std::vector<Batch<kFew>> few = batches<kFew>(p);
+    if (!few.empty()) return passes(p, few[0], few[0].first[few[0].count], ws, o, st);
+  }
+  const std::vector<Batch<kTensors>> all = batches<kTensors>(p);
   if (all.size() > 1) {
     const Table table = {(Entry *)(ws + o.entries), (int32_t *)(ws + o.tensor_of), all[0].chunk};
     int base = 0, first = 0;
-    for (const Batch &b : all) {
+    for (const Batch<kTensors> &b : all) {
       k_table<<<dim3((unsigned)b.count), 64, 0, st>>>(b, table, base, first);
       launched("k_table");
       base += b.count, first += b.first[b.count];

@@ -973,7 +973,7 @@ void check_sizes(const afc_scan_args *p) {
 void check(const afc_scan_args *p, bool grad, bool step) {
   check_sizes(p);
   want(p->a != nullptr, "a is missing");
-  if (step) want(p->length == 1 && !p->lengths && p->final_state && p->final_state == p->initial_state, "a step takes length 1, no lengths, and its state as initial_state and final_state");
+  if (step) want(p->length == 1 && !p->lengths && (p->final_state || p->batch == 0) && p->final_state == p->initial_state, "a step takes length 1, no lengths, and its state as initial_state and final_state");
   if (p->batch == 0 || p->length == 0) return;
   check_seq(p->x, p->batch, p->length, 0, "x");
   check_seq(p->dt, p->batch, p->length, 0, "dt");

@@ -102,7 +102,7 @@ def _own_memory(state, **others):
     for name, t in others.items():
         if t is not None:
             a, b = _span(t)
-            _refuse(hi <= a or b <= lo, "state shares memory with %s", name)
+            _refuse(lo == hi or a == b or hi <= a or b <= lo, "state shares memory with %s", name)
 
 
 # ---- short causal convolution ----

@@ -5,7 +5,7 @@ import torch
 from rlfluidcontrol_amd import ops
 from tests import ops_reference as ref
 from tests.test_ops import (check_conv, check_scan, conv_case, infinite_adjoints, rates_without_memory, refusals_of_clip, refusals_of_conv, refusals_of_scan,
-                            scan_case, states_of_their_own, updates_in_place)
+                            scan_case, states_of_their_own, steps_of_no_rows, updates_in_place)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -394,7 +394,7 @@ def grads_of(sizes, dtypes, seed=0, scale=1.0):
 
 
 @pytest.mark.parametrize("dtypes", [[F32], [BF16], [F16], [F32, BF16, F16]])
-@pytest.mark.parametrize("sizes", [[1], [0, 3], [5, 64, 1, 0, 257], [1000, 33333, 7], [70001], [3] * 250 + [100000], [300001, 2, 65536, 65537], [0] + [17] * 110 + [0], [17] * 120, [17] * 121, [9000, 5] * 300])
+@pytest.mark.parametrize("sizes", [[1], [0, 3], [5, 64, 1, 0, 257], [1000, 33333, 7], [70001], [3] * 250 + [100000], [300001, 2, 65536, 65537], [0] + [17] * 110 + [0], [17] * 120, [17] * 121, [5] * 24, [5] * 25, [9000, 5] * 300])
 def test_clip(dtypes, sizes):
     grads = grads_of(sizes, dtypes)
     before = [g.clone() for g in grads]
@@ -482,6 +482,10 @@ def test_infinite_adjoints_stay_within_their_rows():
 
 def test_states_have_memory_of_their_own():
     states_of_their_own(DEV)
+
+
+def test_steps_of_no_rows():
+    steps_of_no_rows(DEV)
 
 
 def test_autograd_sees_what_is_updated_in_place():

@@ -434,6 +434,7 @@ def states_of_their_own(device):
                      (dict(D=flat[8:16]), "D"), (dict(z=flat[1:17].view(2, 8)), "z")):
         with pytest.raises(ValueError, match="state shares memory with %s" % name):
             ops.selective_scan_step(**{**dict(x=x, dt=x, A=A, B=B, C=B, state=h), **kw})
+    ops.causal_conv_step(x[:0], x.view(-1)[5:5].view(0, 3, 8), w)  # nothing is shared where there is nothing
     ops.selective_scan_step(x, x, A, B, B, h)  # neighbours in one buffer are no neighbours' memory
     assert torch.equal(memory, keep)
 
@@ -456,7 +457,18 @@ def updates_in_place(device):
         assert torch.equal(state[:, -1], x)
 
 
-@pytest.mark.parametrize("which", [rates_without_memory, infinite_adjoints, states_of_their_own, updates_in_place])
+def steps_of_no_rows(device):
+    w, A = torch.randn(8, 4, device=device), -torch.rand(8, 4, device=device)
+
+    def none(*axes):
+        return torch.empty(0, *axes, device=device)
+
+    assert ops.causal_conv_step(none(8), none(3, 8), w).shape == (0, 8)
+    assert ops.selective_scan_step(none(8), none(8), A, none(4), none(4), none(8, 4), torch.ones(8, device=device), none(8)).shape == (0, 8)
+    assert float(ops.clip_grad_norm([none(3), none(2, 2)], 1.0)) == 0 and ops.grad_norm([]) == 0
+
+
+@pytest.mark.parametrize("which", [rates_without_memory, infinite_adjoints, states_of_their_own, updates_in_place, steps_of_no_rows])
 def test_on_the_cpu(which):
     which("cpu")
 
