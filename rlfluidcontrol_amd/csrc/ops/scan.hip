@@ -463,7 +463,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
 }
 
 // ---- backwards ----
-// sums that are finished by k_scan_bc and k_scan_params: bc [batch, groups, tiles, length, 2, NP], a [batch, segs, width, NP], d
+// sums that are finished by k_scan_sums: bc [batch, groups, tiles, length, 2, NP], a [batch, segs, width, NP], d
 // and bias [batch, segs, width]
 struct Sums {
   float *bc, *a, *d, *bias;
@@ -828,27 +828,29 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
   }
 }
 
-// db and dc: the sums over a group's tiles.  One thread for each value.
+// The sums that the blocks of k_scan_grad leave, in one launch (two cost 1 to 4 us more: 8 x 64 x 256 both ways
+// 28.9 against 27.8, 1 x 8191 x 512 164 against 160), in blocks of 1024.
+// The first bc_blocks: db and dc, sums over a group's tiles, one thread for each value.  The others: da, dd and ddt_bias, sums
+// over rows and parts, 64 columns a block.
 template <int DT>
-__global__ __launch_bounds__(256) void k_scan_bc(afc_scan_args P, Plan T, const float *bc, int NP) {
+__global__ __launch_bounds__(1024) void k_scan_sums(afc_scan_args P, Plan T, Sums sums, int NP, int64_t bc_blocks) {
   typedef Elem<DT> E;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = 2 * NP;
-  if (i >= P.batch * P.groups * P.length * per) return;
-  const int64_t row = i / (P.length * per), l = i / per % P.length, b = row / P.groups, g = row % P.groups;
-  const int n = (int)(i % NP), c = (int)(i % per) / NP;
-  if (n >= P.state) return;
-  const float *from = bc + (row * T.tiles * P.length + l) * per + c * NP + n;
-  float a = 0.f;
-#pragma unroll 8
-  for (int t = 0; t < T.tiles; ++t) a += from[t * P.length * per];
-  const afc_seq &s = c ? P.dc : P.db;
-  ((E *)s.data)[b * s.stride_batch + l * s.stride_length + g * s.stride_group + n] = (E)a;
-}
-
-// da, dd, ddt_bias: the sums over rows and parts, 64 columns a block
-__global__ __launch_bounds__(1024) void k_scan_params(afc_scan_args P, Sums sums, int64_t rows, int NP) {
   __shared__ float red[1024];
-  const int64_t na = P.width * NP, col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  if (blockIdx.x < bc_blocks) {
+    const int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x, per = 2 * NP;
+    if (i >= P.batch * P.groups * P.length * per) return;
+    const int64_t row = i / (P.length * per), l = i / per % P.length, b = row / P.groups, g = row % P.groups;
+    const int n = (int)(i % NP), c = (int)(i % per) / NP;
+    if (n >= P.state) return;
+    const float *from = sums.bc + (row * T.tiles * P.length + l) * per + c * NP + n;
+    float a = 0.f;
+#pragma unroll 8
+    for (int t = 0; t < T.tiles; ++t) a += from[t * P.length * per];
+    const afc_seq &s = c ? P.dc : P.db;
+    ((E *)s.data)[b * s.stride_batch + l * s.stride_length + g * s.stride_group + n] = (E)a;
+    return;
+  }
+  const int64_t rows = P.batch * T.segs, na = P.width * NP, col = ((int64_t)blockIdx.x - bc_blocks) * 64 + (threadIdx.x & 63);
   const int which = col < na ? 0 : col < na + P.width ? 1 : 2;
   const int64_t at = which == 0 ? col : col - na - (which - 1) * P.width, cols = which == 0 ? na : P.width;
   const float *from = which == 0 ? sums.a : which == 1 ? sums.d : sums.bias;
@@ -1119,8 +1121,8 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   check(p, true, false);
   const Plan t = plan(p, true);
   const Layout o = layout(p, t);
-  const int64_t n = ceil_div(p->batch * p->length * p->groups * 2 * padded(p), 256);
-  want(n < (int64_t)1 << 31, "too many blocks");
+  const int64_t bc = ceil_div(p->batch * p->length * p->groups * 2 * padded(p), 1024);
+  want(bc < (int64_t)1 << 30, "too many blocks");
   if (p->batch > 0) check_workspace(p, o.all);
   want((uintptr_t)p->checkpoints % 16 == 0, "checkpoints must be 16-byte aligned");
   OnDevice on(p->device);
@@ -1139,19 +1141,14 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
     SCAN_ALL(0)
 #undef SCAN_GO
     launched("k_scan_grad");
-    if (n) {
-      const dim3 gb((unsigned)n);
-      if (p->dtype == AFC_F32) k_scan_bc<AFC_F32><<<gb, 256, 0, st>>>(*p, t, sums.bc, padded(p));
-      if (p->dtype == AFC_BF16) k_scan_bc<AFC_BF16><<<gb, 256, 0, st>>>(*p, t, sums.bc, padded(p));
-      if (p->dtype == AFC_F16) k_scan_bc<AFC_F16><<<gb, 256, 0, st>>>(*p, t, sums.bc, padded(p));
-      launched("k_scan_bc");
-    }
   }
-  if (p->da || p->dd || p->ddt_bias) {
-    const dim3 gp((unsigned)ceil_div(p->width * (padded(p) + 2), 64));
-    k_scan_params<<<gp, 1024, 0, st>>>(*p, sums, p->batch * t.segs, padded(p));
-    launched("k_scan_params");
-  }
+  const int64_t params = p->da || p->dd || p->ddt_bias ? ceil_div(p->width * (padded(p) + 2), 64) : 0;
+  if (bc + params == 0) return;
+  const dim3 gs((unsigned)(bc + params));
+  if (p->dtype == AFC_F32) k_scan_sums<AFC_F32><<<gs, 1024, 0, st>>>(*p, t, sums, padded(p), bc);
+  if (p->dtype == AFC_BF16) k_scan_sums<AFC_BF16><<<gs, 1024, 0, st>>>(*p, t, sums, padded(p), bc);
+  if (p->dtype == AFC_F16) k_scan_sums<AFC_F16><<<gs, 1024, 0, st>>>(*p, t, sums, padded(p), bc);
+  launched("k_scan_sums");
 }
 
 int lanes(const afc_scan_args *p) {
