@@ -72,6 +72,15 @@ void no_grad(const T &...t) {
 }
 
 Tensor value(const Maybe &t) { return t ? *t : Tensor(); }
+
+// A kernel knows nothing of forward-mode derivatives: what it writes would have none, which PyTorch takes for zero.
+bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const Maybe &t) { return t && has_tangent(*t); }
+template <class... T>
+void no_tangent(const T &...t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), "these operators have no forward-mode derivative on a GPU (a tensor carries a tangent)");
+}
+
 // the bytes from a tensor's first element to its last
 struct Span {
   uintptr_t from, to;
@@ -120,7 +129,8 @@ Tensor fresh(const Tensor &like) { return at::empty(like.sizes(), like.options()
 Tensor fresh_if(const Tensor &like, bool wanted) { return like.defined() && wanted ? fresh(like) : Tensor(); }
 Tensor space(const Tensor &x, uint64_t bytes) { return at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)); }
 
-void first_order_only() {
+void first_order_only(const Tensor &dy, const Tensor &dlast) {
+  no_tangent(dy, dlast);
   TORCH_CHECK(!at::GradMode::is_enabled(), "the gradients of these operators have no gradient of their own (create_graph=True)");
 }
 
@@ -167,9 +177,9 @@ struct Conv : torch::autograd::Function<Conv> {
     return conv_forward(x, w, b, s, n, silu, want_last);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    first_order_only();
     variable_list out(7);
     Tensor dy = grads[0], dlast = grads.size() > 1 ? grads[1] : Tensor();
+    first_order_only(dy, dlast);
     if (!dy.defined() && !dlast.defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &state = saved[3], &lengths = saved[4];
@@ -193,6 +203,7 @@ struct Conv : torch::autograd::Function<Conv> {
 };
 
 variable_list causal_conv(const Tensor &x, const Tensor &weight, const Maybe &bias, bool silu, const Maybe &state, const Maybe &lengths, bool want_last) {
+  no_tangent(x, weight, bias, state);
   input(x, 3);
   sequence("x", x, x.sizes(), x.scalar_type(), x.device());
   check_filter(weight, bias, x.size(2), x.device());
@@ -203,6 +214,7 @@ variable_list causal_conv(const Tensor &x, const Tensor &weight, const Maybe &bi
 }
 
 Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weight, const Maybe &bias, bool silu) {
+  no_tangent(x, state, weight, bias);
   input(x, 2);
   sequence("x", x, x.sizes(), x.scalar_type(), x.device());
   check_filter(weight, bias, x.size(1), x.device());
@@ -307,9 +319,9 @@ struct Scan : torch::autograd::Function<Scan> {
     return out;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    first_order_only();
     variable_list out(12);
     Tensor dy = grads[0], dlast = grads.size() > 1 ? grads[1] : Tensor();
+    first_order_only(dy, dlast);
     if (!dy.defined() && !dlast.defined()) return out;
     const variable_list v = ctx->get_saved_variables();
     const ScanInputs in = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
@@ -336,6 +348,7 @@ struct Scan : torch::autograd::Function<Scan> {
 
 variable_list selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Maybe &D, const Maybe &z, const Maybe &dt_bias,
                              bool softplus, const Maybe &state, const Maybe &lengths, bool want_last) {
+  no_tangent(x, dt, A, B, C, D, z, dt_bias, state);
   input(x, 3);
   ScanInputs in = {x, dt, A, B, C, value(D), value(z), value(dt_bias)};
   check_scan(in);
@@ -348,6 +361,7 @@ variable_list selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A,
 
 Tensor selective_scan_step(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Tensor &state, const Maybe &D, const Maybe &z,
                            const Maybe &dt_bias, bool softplus) {
+  no_tangent(x, dt, A, B, C, state, D, z, dt_bias);
   input(x, 2);
   ScanInputs in = {x, dt, A, B, C, value(D), value(z), value(dt_bias)};
   check_scan(in);
@@ -378,6 +392,9 @@ bool without_gaps(const Tensor &t) { return t.is_contiguous() || t.is_non_overla
 Tensor clip(const std::vector<Tensor> &grads, double max_norm, const std::optional<std::vector<Tensor>> &out) {
   const bool scale = max_norm >= 0;
   const size_t n = grads.size();
+  for (const Tensor &g : grads) no_tangent(g);
+  if (out)
+    for (const Tensor &o : *out) no_tangent(o);
   TORCH_CHECK_VALUE(n > 0 && (!out || out->size() == n), "out has another number of tensors than grads");
   const at::Device dev = grads[0].device();
   TORCH_CHECK_VALUE(dev.is_cuda(), "gradients are on ", dev, ": a GPU is expected");

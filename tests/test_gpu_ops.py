@@ -5,7 +5,7 @@ import torch
 from rlfluidcontrol_amd import ops
 from tests import ops_reference as ref
 from tests.test_ops import (check_conv, check_scan, conv_case, infinite_adjoints, rates_without_memory, refusals_of_clip, refusals_of_conv, refusals_of_scan,
-                            scan_case, states_of_their_own, steps_of_no_rows, updates_in_place)
+                            scan_case, states_of_their_own, steps_of_no_rows, tangents_are_refused, updates_in_place)
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -532,3 +532,26 @@ def test_calls_from_several_threads():
     assert not failures
     for a, b in zip(got, want):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+# ---- derivatives that the kernels do not compute ----
+
+def test_tangents_are_refused():
+    tangents_are_refused(DEV)
+
+
+def test_adjoints_with_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    c = conv_case(1, 2, 5, 8, 3, F32, DEV)
+    x = c["x"].clone().requires_grad_()
+    y = ops.causal_conv(x, c["weight"])
+    with fwd.dual_level(), pytest.raises(RuntimeError, match="tangent"):
+        torch.autograd.grad(y, [x], [fwd.make_dual(c["dy"], torch.ones_like(c["dy"]))])
+
+
+def test_transformed_tensors_are_refused():
+    x, w = torch.randn(3, 2, 5, 8, device=DEV), torch.randn(8, 3, device=DEV)
+    for f in (lambda: torch.func.vmap(lambda t: ops.causal_conv(t, w))(x), lambda: torch.func.jvp(lambda t: ops.causal_conv(t, w), (x[0],), (x[0],)),
+              lambda: torch.func.grad(lambda t: ops.causal_conv(t, w).sum())(x[0]), lambda: torch.func.functionalize(lambda t: ops.causal_conv(t, w))(x[0])):
+        with pytest.raises(RuntimeError):
+            f()

@@ -481,3 +481,50 @@ def test_plain_clip_refuses_tensors_that_overlap():
     assert torch.equal(a, torch.ones(100))
     ops.clip_grad_norm([a[50:], a[:50], a[50:50]], 1.0)
     assert abs(float(a.norm()) - 1) < 1e-5 and abs(float(ops.grad_norm([a, a])) - 2 ** 0.5) < 1e-5
+
+
+# ---- what the binding refuses before it asks for a GPU ----
+
+def calls_of_the_binding(device="cpu"):
+    """every call of the binding as (name, call, its floating-point tensors); a call takes one of them replaced"""
+    c, v = scan_case(1, 2, 5, 6, 4, device=device), conv_case(1, 2, 5, 6, 3, device=device)
+    m = ops._gpu()
+    one = {k: c[k][:, 0].contiguous() for k in ("x", "dt", "B", "C", "z")}
+    cases = [
+        ("causal_conv", ("x", "weight", "bias", "state"), v, lambda a: m.causal_conv(a["x"], a["weight"], a["bias"], True, a["state"], None, True)[0]),
+        ("causal_conv_step", ("x", "state", "weight", "bias"), dict(v, x=v["x"][:, 0]), lambda a: m.causal_conv_step(a["x"], a["state"], a["weight"], a["bias"], True)),
+        ("selective_scan", ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "state"), c,
+         lambda a: m.selective_scan(a["x"], a["dt"], a["A"], a["B"], a["C"], a["D"], a["z"], a["dt_bias"], True, a["state"], None, True)[0]),
+        ("selective_scan_step", ("x", "dt", "A", "B", "C", "state", "D", "z", "dt_bias"), dict(c, **one),
+         lambda a: m.selective_scan_step(a["x"], a["dt"], a["A"], a["B"], a["C"], a["state"], a["D"], a["z"], a["dt_bias"], True)),
+        ("clip", ("g", "h"), dict(g=torch.randn(4, device=device), h=torch.randn(3, device=device)), lambda a: m.clip([a["g"], a["h"]], 1.0, None)),
+        ("clip", ("out",), dict(g=torch.randn(4, device=device), out=torch.randn(4, device=device)), lambda a: m.clip([a["g"]], 1.0, [a["out"]])),
+        ("norm", ("g",), dict(g=torch.randn(4, device=device)), lambda a: m.clip([a["g"]], -1.0, None)),
+    ]
+    return [(name, names, values, call) for name, names, values, call in cases]
+
+
+def tangents_are_refused(device):
+    import torch.autograd.forward_ad as fwd
+    for name, names, values, call in calls_of_the_binding(device):
+        for n in names:
+            for leaf in (False, True):
+                with fwd.dual_level(), torch.set_grad_enabled(leaf and name in ("causal_conv", "selective_scan")):
+                    t = values[n].clone().requires_grad_(torch.is_grad_enabled())
+                    with pytest.raises(NotImplementedError, match="tangent"):
+                        call(dict(values, **{n: fwd.make_dual(t, torch.ones_like(t))}))
+
+
+def test_the_binding_refuses_tangents(lib):
+    tangents_are_refused("cpu")
+
+
+def test_tangents_on_the_cpu():
+    import torch.autograd.forward_ad as fwd
+    c = conv_case(3, 2, 5, 4, 3)
+    with fwd.dual_level():
+        y = fwd.unpack_dual(ops.causal_conv(fwd.make_dual(c["x"], c["dy"]), c["weight"], None, True))
+    eps = 1e-3
+    a, b = (ops.causal_conv(c["x"] + s * c["dy"], c["weight"], None, True) for s in (eps, -eps))
+    # central differences in 32 bits: values of up to 8 are off by 8 u a few times, over 2 eps; the third derivative by eps^2
+    assert float(((a - b) / (2 * eps) - y.tangent).abs().max()) < 16 * 8 * 2.0 ** -24 / (2 * eps) + 100 * eps ** 2
