@@ -3,6 +3,9 @@
 // In C++ because the calls are short: at the sizes of the learner the kernels of a training step take some 40 us, and the same
 // work in Python took 240.
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -76,6 +79,12 @@ Tensor value(const Maybe &t) { return t ? *t : Tensor(); }
 // A kernel knows nothing of forward-mode derivatives: what it writes would have none, which PyTorch takes for zero.
 bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
 bool has_tangent(const Maybe &t) { return t && has_tangent(*t); }
+// Nor does a tracer see it: torch.jit.trace and make_fx would record the allocation of an output and not what fills it.
+void not_traced() {
+  const bool traced = torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value() ||
+                      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+  TORCH_CHECK_NOT_IMPLEMENTED(!traced, "these operators cannot be traced on a GPU: a tracer sees their outputs' memory and not what fills it");
+}
 template <class... T>
 void no_tangent(const T &...t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), "these operators have no forward-mode derivative on a GPU (a tensor carries a tangent)");
@@ -130,6 +139,7 @@ Tensor fresh_if(const Tensor &like, bool wanted) { return like.defined() && want
 Tensor space(const Tensor &x, uint64_t bytes) { return at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)); }
 
 void first_order_only(const Tensor &dy, const Tensor &dlast) {
+  not_traced();
   no_tangent(dy, dlast);
   TORCH_CHECK(!at::GradMode::is_enabled(), "the gradients of these operators have no gradient of their own (create_graph=True)");
 }
@@ -203,6 +213,7 @@ struct Conv : torch::autograd::Function<Conv> {
 };
 
 variable_list causal_conv(const Tensor &x, const Tensor &weight, const Maybe &bias, bool silu, const Maybe &state, const Maybe &lengths, bool want_last) {
+  not_traced();
   no_tangent(x, weight, bias, state);
   input(x, 3);
   sequence("x", x, x.sizes(), x.scalar_type(), x.device());
@@ -214,6 +225,7 @@ variable_list causal_conv(const Tensor &x, const Tensor &weight, const Maybe &bi
 }
 
 Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weight, const Maybe &bias, bool silu) {
+  not_traced();
   no_tangent(x, state, weight, bias);
   input(x, 2);
   sequence("x", x, x.sizes(), x.scalar_type(), x.device());
@@ -348,6 +360,7 @@ struct Scan : torch::autograd::Function<Scan> {
 
 variable_list selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Maybe &D, const Maybe &z, const Maybe &dt_bias,
                              bool softplus, const Maybe &state, const Maybe &lengths, bool want_last) {
+  not_traced();
   no_tangent(x, dt, A, B, C, D, z, dt_bias, state);
   input(x, 3);
   ScanInputs in = {x, dt, A, B, C, value(D), value(z), value(dt_bias)};
@@ -361,6 +374,7 @@ variable_list selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A,
 
 Tensor selective_scan_step(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Tensor &state, const Maybe &D, const Maybe &z,
                            const Maybe &dt_bias, bool softplus) {
+  not_traced();
   no_tangent(x, dt, A, B, C, state, D, z, dt_bias);
   input(x, 2);
   ScanInputs in = {x, dt, A, B, C, value(D), value(z), value(dt_bias)};
@@ -392,6 +406,7 @@ bool without_gaps(const Tensor &t) { return t.is_contiguous() || t.is_non_overla
 Tensor clip(const std::vector<Tensor> &grads, double max_norm, const std::optional<std::vector<Tensor>> &out) {
   const bool scale = max_norm >= 0;
   const size_t n = grads.size();
+  not_traced();
   for (const Tensor &g : grads) no_tangent(g);
   if (out)
     for (const Tensor &o : *out) no_tangent(o);

@@ -8,6 +8,8 @@ global gradient norm (libafc_ops.so, include/afc_ops.h; no counterpart in the re
 On a GPU every call runs the hand-written kernels on the current stream of the tensors' own device: nothing is copied to the
 host and nothing waits, so the calls may be captured into a graph.  There is no other GPU path; a missing library raises, and so
 does what the kernels do not compute: second derivatives and forward-mode ones (NotImplementedError for a tensor with a tangent).
+A tracer sees no kernel that is called behind PyTorch's back, so calls under torch.jit.trace or make_fx raise NotImplementedError
+(torch.compile breaks its graph around them and runs them as they are).
 Tensors on the CPU take the same formulas in plain torch (the learner runs on either device).
 
 Sequence tensors are [batch, length, width] in float32, bfloat16 or float16, the last axis contiguous, the others free (so
