@@ -85,6 +85,13 @@ void not_traced() {
                       c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
   TORCH_CHECK_NOT_IMPLEMENTED(!traced, "these operators cannot be traced on a GPU: a tracer sees their outputs' memory and not what fills it");
 }
+// x.conj().imag and the like are views whose sign is applied when PyTorch reads them; the memory has the other one
+bool is_negated(const Tensor &t) { return t.defined() && t.is_neg(); }
+bool is_negated(const Maybe &t) { return t && is_negated(*t); }
+template <class... T>
+void as_stored(const T &...t) {
+  TORCH_CHECK_VALUE(!(is_negated(t) || ...), "a tensor is a view that negates its memory (resolve_neg() gives a plain one)");
+}
 template <class... T>
 void no_tangent(const T &...t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(t) || ...), "these operators have no forward-mode derivative on a GPU (a tensor carries a tangent)");
@@ -111,8 +118,9 @@ void written(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-Tensor dense(const Maybe &t) { return t ? t->contiguous() : Tensor(); }
-Tensor last_contiguous(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor dense(const Tensor &t) { return t.resolve_neg().contiguous(); }
+Tensor dense(const Maybe &t) { return t ? dense(*t) : Tensor(); }
+Tensor last_contiguous(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t.resolve_neg() : dense(t); }
 template <class T = void>
 T *ptr(const Tensor &t) {
   return t.defined() ? (T *)t.data_ptr() : nullptr;
@@ -179,7 +187,7 @@ variable_list conv_forward(const Tensor &x, const Tensor &weight, const Tensor &
 struct Conv : torch::autograd::Function<Conv> {
   static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &weight, const Maybe &bias, const Maybe &state, const Maybe &lengths, bool silu,
                                bool want_last) {
-    const Tensor w = weight.contiguous(), b = dense(bias), s = dense(state), n = dense(lengths);
+    const Tensor w = dense(weight), b = dense(bias), s = dense(state), n = dense(lengths);
     ctx->save_for_backward({x, w, b, s, n});
     ctx->saved_data["silu"] = silu;
     ctx->saved_data["wanted"] = wanted(x, weight, bias, state);
@@ -194,7 +202,7 @@ struct Conv : torch::autograd::Function<Conv> {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &state = saved[3], &lengths = saved[4];
     dy = dy.defined() ? last_contiguous(dy) : at::zeros(x.sizes(), x.options());
-    if (dlast.defined()) dlast = dlast.contiguous();
+    if (dlast.defined()) dlast = dense(dlast);
     const int64_t need = ctx->saved_data["wanted"].toInt();
     const Tensor dx = fresh(x), dw = fresh_if(weight, need & 2), db = fresh_if(bias, need & 4), ds = fresh_if(state, need & 8);
     afc_conv_args p = conv_args(x, weight, bias, state, lengths, ctx->saved_data["silu"].toBool());
@@ -215,18 +223,20 @@ struct Conv : torch::autograd::Function<Conv> {
 variable_list causal_conv(const Tensor &x, const Tensor &weight, const Maybe &bias, bool silu, const Maybe &state, const Maybe &lengths, bool want_last) {
   not_traced();
   no_tangent(x, weight, bias, state);
+  as_stored(x);
   input(x, 3);
   sequence("x", x, x.sizes(), x.scalar_type(), x.device());
   check_filter(weight, bias, x.size(2), x.device());
   optional("initial_state", state, {x.size(0), weight.size(1) - 1, x.size(2)}, x.scalar_type(), x.device());
   optional("lengths", lengths, {x.size(0)}, at::kInt, x.device());
   if (wants_grad(x, weight, bias, state)) return Conv::apply(x, weight, bias, state, lengths, silu, want_last);
-  return conv_forward(x, weight.contiguous(), dense(bias), dense(state), dense(lengths), silu, want_last);
+  return conv_forward(x, dense(weight), dense(bias), dense(state), dense(lengths), silu, want_last);
 }
 
 Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weight, const Maybe &bias, bool silu) {
   not_traced();
   no_tangent(x, state, weight, bias);
+  as_stored(x, state);
   input(x, 2);
   sequence("x", x, x.sizes(), x.scalar_type(), x.device());
   check_filter(weight, bias, x.size(1), x.device());
@@ -234,7 +244,7 @@ Tensor causal_conv_step(const Tensor &x, const Tensor &state, const Tensor &weig
   TORCH_CHECK_VALUE(state.is_contiguous(), "state must be contiguous");
   own_memory(state, "x", x), own_memory(state, "weight", weight), own_memory(state, "bias", value(bias));
   no_grad(x, state, weight, bias);
-  const Tensor w = weight.contiguous(), b = dense(bias), y = at::empty(x.sizes(), x.options());
+  const Tensor w = dense(weight), b = dense(bias), y = at::empty(x.sizes(), x.options());
   afc_conv_args p = {};
   p.device = x.device().index();
   p.dtype = dtype_of(x);
@@ -320,7 +330,7 @@ variable_list scan_forward(const ScanInputs &in, const Tensor &state, const Tens
 struct Scan : torch::autograd::Function<Scan> {
   static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Maybe &D, const Maybe &z,
                                const Maybe &dt_bias, const Maybe &state, const Maybe &lengths, bool softplus, bool want_last) {
-    const ScanInputs in = {x, dt, A.contiguous(), B, C, dense(D), value(z), dense(dt_bias)};
+    const ScanInputs in = {x, dt, dense(A), B, C, dense(D), value(z), dense(dt_bias)};
     const Tensor s = dense(state), n = dense(lengths);
     Tensor checkpoints;
     variable_list out = scan_forward(in, s, n, softplus, want_last, &checkpoints);
@@ -339,7 +349,7 @@ struct Scan : torch::autograd::Function<Scan> {
     const ScanInputs in = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
     const Tensor &x = in.x, &state = v[8], &lengths = v[9], &checkpoints = v[10];
     dy = dy.defined() ? last_contiguous(dy) : at::zeros(x.sizes(), x.options());
-    if (dlast.defined()) dlast = dlast.contiguous();
+    if (dlast.defined()) dlast = dense(dlast);
     out[0] = fresh(x), out[1] = fresh(in.dt), out[3] = fresh(in.B), out[4] = fresh(in.C);
     const int64_t need = ctx->saved_data["wanted"].toInt();
     out[2] = fresh_if(in.A, need & 4), out[5] = fresh_if(in.D, need & 32), out[6] = fresh_if(in.z, need & 64);
@@ -362,13 +372,14 @@ variable_list selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A,
                              bool softplus, const Maybe &state, const Maybe &lengths, bool want_last) {
   not_traced();
   no_tangent(x, dt, A, B, C, D, z, dt_bias, state);
+  as_stored(x, dt, B, C, z);
   input(x, 3);
   ScanInputs in = {x, dt, A, B, C, value(D), value(z), value(dt_bias)};
   check_scan(in);
   optional("initial_state", state, {x.size(0), x.size(2), A.size(1)}, at::kFloat, x.device());
   optional("lengths", lengths, {x.size(0)}, at::kInt, x.device());
   if (wants_grad(x, dt, A, B, C, D, z, dt_bias, state)) return Scan::apply(x, dt, A, in.B, in.C, D, z, dt_bias, state, lengths, softplus, want_last);
-  in.A = in.A.contiguous(), in.D = dense(D), in.dt_bias = dense(dt_bias);
+  in.A = dense(in.A), in.D = dense(D), in.dt_bias = dense(dt_bias);
   return scan_forward(in, dense(state), dense(lengths), softplus, want_last, nullptr);
 }
 
@@ -376,6 +387,7 @@ Tensor selective_scan_step(const Tensor &x, const Tensor &dt, const Tensor &A, c
                            const Maybe &dt_bias, bool softplus) {
   not_traced();
   no_tangent(x, dt, A, B, C, state, D, z, dt_bias);
+  as_stored(x, dt, B, C, state, z);
   input(x, 2);
   ScanInputs in = {x, dt, A, B, C, value(D), value(z), value(dt_bias)};
   check_scan(in);
@@ -384,7 +396,7 @@ Tensor selective_scan_step(const Tensor &x, const Tensor &dt, const Tensor &A, c
   own_memory(state, "x", x), own_memory(state, "dt", dt), own_memory(state, "B", in.B), own_memory(state, "C", in.C), own_memory(state, "z", in.z);
   own_memory(state, "A", A), own_memory(state, "D", in.D), own_memory(state, "dt_bias", in.dt_bias);
   no_grad(x, dt, A, B, C, state, D, z, dt_bias);
-  const Tensor a = A.contiguous(), d = dense(D), bias = dense(dt_bias), y = at::empty(x.sizes(), x.options());
+  const Tensor a = dense(A), d = dense(D), bias = dense(dt_bias), y = at::empty(x.sizes(), x.options());
   afc_scan_args p = {};
   p.device = x.device().index();
   p.dtype = dtype_of(x);
@@ -407,9 +419,9 @@ Tensor clip(const std::vector<Tensor> &grads, double max_norm, const std::option
   const bool scale = max_norm >= 0;
   const size_t n = grads.size();
   not_traced();
-  for (const Tensor &g : grads) no_tangent(g);
+  for (const Tensor &g : grads) no_tangent(g), as_stored(g);
   if (out)
-    for (const Tensor &o : *out) no_tangent(o);
+    for (const Tensor &o : *out) no_tangent(o), as_stored(o);
   TORCH_CHECK_VALUE(n > 0 && (!out || out->size() == n), "out has another number of tensors than grads");
   const at::Device dev = grads[0].device();
   TORCH_CHECK_VALUE(dev.is_cuda(), "gradients are on ", dev, ": a GPU is expected");

@@ -31,3 +31,26 @@ def test_the_plain_path_is_traced():
     c = conv_case(3, 2, 5, 4, 3)
     f = torch.jit.trace(lambda x: ops.causal_conv(x, c["weight"], c["bias"], True), (c["x"],))
     assert torch.equal(f(c["dy"]), ops.causal_conv(c["dy"], c["weight"], c["bias"], True))
+
+
+def negated(t):
+    """the values of t, as a view of memory that holds their negatives"""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+# what a kernel reads or updates where it lies (the other operands are copied where they have to be)
+IN_PLACE = {"causal_conv": ("x",), "causal_conv_step": ("x", "state"), "selective_scan": ("x", "dt", "B", "C", "z"),
+            "selective_scan_step": ("x", "dt", "B", "C", "z", "state"), "clip": ("g", "h", "out"), "norm": ("g",)}
+
+
+def negated_views_are_refused(device):
+    for name, names, values, call in calls_of_the_binding(device):
+        for n in set(names) & set(IN_PLACE[name]):
+            with torch.no_grad(), pytest.raises(ValueError, match="resolve_neg"):
+                call(dict(values, **{n: negated(values[n])}))
+
+
+def test_negated_views_are_refused():
+    negated_views_are_refused("cpu")
