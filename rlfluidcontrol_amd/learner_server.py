@@ -25,11 +25,11 @@ class LearnerServer:
 
     def __init__(self, environment="CFD", filter="None", explore_noise="Gaussian", one_action=False, host="localhost",
                  port=8000, device="cpu", seed=None, save_dir="save", data_dir="save_data", eval_dir="save_eval", actor="mlp",
-                 max_grad_norm=None):
+                 max_grad_norm=None, window=64):
         if environment != "CFD":
             raise NotImplementedError("only the CFD environment (server.py:117-118) is served")
         self.learner = td3.BatchedLearner(1, device=device, filter=filter, explore_noise=explore_noise,
-                                          one_action=one_action, seed=seed, actor=actor, max_grad_norm=max_grad_norm)
+                                          one_action=one_action, seed=seed, actor=actor, window=window, max_grad_norm=max_grad_norm)
         self.unfiltered_state_record = []
         self.save_model_dir, self.save_data_dir, self.save_eval_dir = save_dir, data_dir, eval_dir
         self.server = SimpleXMLRPCServer((host, port), logRequests=False, allow_none=True)
@@ -122,12 +122,13 @@ def main(argv=None):
     ap.add_argument("-exn", "--explore_noise", choices=["Gaussian", "Process"], default="Gaussian")
     ap.add_argument("-one", "--one_action", action="store_true")
     ap.add_argument("--actor", choices=["mlp", "memory"], default="mlp")
+    ap.add_argument("--window", type=int, default=64, help="transitions of a training window (--actor memory)")
     ap.add_argument("--max-grad-norm", type=float, default=None)
     ap.add_argument("--port", type=int, default=8000)
     ap.add_argument("--device", default="cuda:0" if torch.cuda.is_available() else "cpu")
     a = ap.parse_args(argv)
     LearnerServer(environment=a.environment, filter=a.filter, explore_noise=a.explore_noise, one_action=a.one_action,
-                  port=a.port, device=a.device, actor=a.actor, max_grad_norm=a.max_grad_norm).start_server()
+                  port=a.port, device=a.device, actor=a.actor, window=a.window, max_grad_norm=a.max_grad_norm).start_server()
 
 
 if __name__ == "__main__":
