@@ -49,13 +49,21 @@ def _ops_deps():
 
 
 def _binding_flags():
-    """(compile, link) flags of _ops_torch.so: host code only, against the torch that imports it"""
+    """(compile, link) flags of _ops_torch.so: host code only, against the torch that imports it; None where there is nothing to
+    build it against (no torch, one without a GPU's runtime, no headers of torch or Python)"""
     import sysconfig
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return None
     inc, lib = os.path.join(os.path.dirname(torch.__file__), "include"), os.path.join(os.path.dirname(torch.__file__), "lib")
+    python = sysconfig.get_paths()["include"]
+    headers = (os.path.join(inc, "torch", "extension.h"), os.path.join(python, "Python.h"))
+    if torch.version.hip is None or not all(map(os.path.exists, headers)):
+        return None
     compile_ = ["-O2", "-std=c++17", "-fPIC", "-x", "c++", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_ops_torch",
                 "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
-    for d in (inc, os.path.join(inc, "torch", "csrc", "api", "include"), "/opt/rocm/include", sysconfig.get_paths()["include"]):
+    for d in (inc, os.path.join(inc, "torch", "csrc", "api", "include"), "/opt/rocm/include", python):
         compile_ += ["-isystem", d]
     return compile_, ["-L" + HERE, "-lafc_ops", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lc10", "-lc10_hip"]
 
@@ -92,19 +100,18 @@ def needs_build():
 
 
 def build(force=False, verbose=False):
-    """Everything; returns the environment's library."""
+    """Everything, the environment's library (returned) first: it needs neither torch nor what is built after it."""
+    path = _build(ENV, force, verbose)
     build_ops(force, verbose)
-    return _build(ENV, force, verbose)
+    return path
 
 
 def build_ops(force=False, verbose=False):
-    """libafc_ops.so (returned) and, where torch is, its binding"""
+    """libafc_ops.so (returned) and, where there is a torch to build it against, its binding"""
     path = _build(OPS, force, verbose)
-    try:
-        flags, link = _binding_flags()
-    except ImportError:
-        return path
-    _build(_Library(BINDING, OPS_CSRC, ["binding.cpp"], _ops_deps, flags, BINDING_STAMP, link), force, verbose)
+    flags = _binding_flags()
+    if flags is not None:
+        _build(_Library(BINDING, OPS_CSRC, ["binding.cpp"], _ops_deps, flags[0], BINDING_STAMP, flags[1]), force, verbose)
     return path
 
 

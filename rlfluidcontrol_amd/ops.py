@@ -42,7 +42,10 @@ def _gpu():
     if _gpu_module is None:
         if not os.path.exists(LIB_PATH):
             raise OpsError("libafc_ops.so is missing: build it with `python -m rlfluidcontrol_amd.build`")
-        from . import _ops_torch
+        try:
+            from . import _ops_torch
+        except ImportError as e:
+            raise OpsError("the torch binding of libafc_ops.so cannot be loaded (%s): build it with `python -m rlfluidcontrol_amd.build`" % e) from e
         _ops_torch.set_error_class(OpsError)
         _gpu_module = _ops_torch
     return _gpu_module
