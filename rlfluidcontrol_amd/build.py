@@ -62,7 +62,8 @@ def _binding_flags():
     if torch.version.hip is None or not all(map(os.path.exists, headers)):
         return None
     compile_ = ["-O2", "-std=c++17", "-fPIC", "-x", "c++", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_ops_torch",
-                "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI]
+                "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+                "-DAFC_BUILT_FOR_TORCH=" + torch.__version__]  # (read by nothing but flag_string(): another torch in the same place is another build)
     for d in (inc, os.path.join(inc, "torch", "csrc", "api", "include"), "/opt/rocm/include", python):
         compile_ += ["-isystem", d]
     return compile_, ["-L" + HERE, "-lafc_ops", "-Wl,-rpath,$ORIGIN", "-L" + lib, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", "-lc10", "-lc10_hip"]

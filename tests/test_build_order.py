@@ -61,3 +61,15 @@ def test_a_missing_binding_is_an_error_of_the_operators(monkeypatch):
     monkeypatch.delattr("rlfluidcontrol_amd._ops_torch", raising=False)
     with pytest.raises(ops.OpsError, match="binding"):
         ops._gpu()
+
+
+def test_another_torch_makes_another_binding(monkeypatch):
+    build.build_ops()
+
+    def stale():
+        flags, link = build._binding_flags()
+        return build._Library(build.BINDING, build.OPS_CSRC, ["binding.cpp"], build._ops_deps, flags, build.BINDING_STAMP, link).needs_build()
+
+    assert not stale()
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".1")
+    assert stale()
