@@ -430,13 +430,18 @@ class Agent:
         q_loss = ((self.main_critic_1(sa1) - y) ** 2).mean() + ((self.main_critic_2(sa1) - y) ** 2).mean()
         return q_loss, y
 
+    def _window_target_actions(self, batch):
+        """The target actor's actions in the next states of windows.  It reads a window's first state too, so that it has seen in
+        state k + 1 what an actor that starts with the window has seen there (obs2[k] is obs1[k + 1])."""
+        seen = torch.cat([batch["obs1"][:, :1], batch["obs2"]], 1)
+        return self.target_actor(seen, batch["lengths"] + 1)[:, 1:]
+
     def window_losses(self, batch):
-        """losses() over windows [batch, length, ...]: the target actor reads each window's next states from its start, and the
-        mean runs over what lies within the windows"""
+        """losses() over windows [batch, length, ...]; the mean runs over what lies within the windows"""
         lengths = batch["lengths"]
         keep = (torch.arange(batch["obs1"].shape[1], device=self.device) < lengths[:, None])[..., None]
         with torch.no_grad():
-            nxt = self.target_actor(batch["obs2"], lengths)
+            nxt = self._window_target_actions(batch)
             noise = torch.clamp(self.criticreg_noise_size * torch.randn(nxt.shape, device=self.device, generator=self.gen),
                                 -self.criticreg_noise_clip, self.criticreg_noise_clip)
             sa2 = torch.cat([batch["obs2"], torch.clamp(nxt + noise, -1, 1)], -1)
