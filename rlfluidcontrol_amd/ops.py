@@ -314,7 +314,8 @@ def _plain_conv(x, weight, bias, silu, state, lengths):
     xf = _mask(lengths, L, x.float())
     front = state.float() if state is not None else xf.new_zeros(B, K - 1, W)
     rows = torch.cat([front, xf], 1)
-    pre = sum(rows[:, k:k + L] * weight[:, k] for k in range(K))
+    # (masked again: a zero adjoint behind a row's end times an infinite input would be NaN in weight's gradient)
+    pre = sum(_mask(lengths, L, rows[:, k:k + L]) * weight[:, k] for k in range(K))
     pre = pre + bias if bias is not None else pre
     y = _mask(lengths, L, pre * torch.sigmoid(pre) if silu else pre)
     n = lengths.clamp(0, L).long() if lengths is not None else torch.full((B,), L)

@@ -4,6 +4,7 @@ import torch
 
 from rlfluidcontrol_amd import ops
 from tests.test_ops import calls_of_the_binding, conv_case, scan_case
+from tests import test_ops_infinities as infinities
 from tests.test_ops_calls import IN_PLACE, negated, negated_views_are_refused, tracing_is_refused
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +43,8 @@ def test_negated_adjoints():
         want = torch.autograd.grad(outs, list(leaves.values()), [case["dy"], case["dlast"]], retain_graph=True)
         got = torch.autograd.grad(outs, list(leaves.values()), [negated(case["dy"]), negated(case["dlast"])])
         assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("which", infinities.CHECKS)
+def test_infinities(which):
+    which(DEV)
