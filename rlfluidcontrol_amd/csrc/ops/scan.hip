@@ -342,7 +342,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
   const int64_t l0 = (int64_t)first * K, lr = l0 + at.r, wq = at.readable();
   Rows<DT, S, NL> rb(P.b, at, l0, P.state), rc(P.c, at, l0, P.state);
   Stream<DT> xs(P.x, at.b, lr, wq), dts(P.dt, at.b, lr, wq), zs(P.z, at.b, lr, wq), out(P.y, at.b, lr, at.w0 + at.q);
-  const bool gate = !CARRY && P.z.data, soft = P.softplus;
+  const bool gate = !CARRY && P.z.data, soft = P.softplus, skip = P.d;
   auto fetch = [&](int ch) {
     if (ch >= live) return;  // (what is there stays, unused)
     if (WHOLE && (ch + 1) * K <= at.len) {
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
   Piece<DT, E, WHOLE> x1{}, z1{}, x2{}, z2{};  // of the chunk in the recurrence, and of the one before it
   float y[E];
   auto finish = [&](int i) {
-    const float v = __builtin_fmaf(D[i], x2[i], y[i]), gated = v * silu(z2[i]);
+    const float with_x = __builtin_fmaf(D[i], x2[i], y[i]), v = skip ? with_x : y[i], gated = v * silu(z2[i]);
     y[i] = gate ? gated : v;
   };
   auto put_y = [&](int ch) {
@@ -586,7 +586,7 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
 #pragma unroll
   for (int s = 0; s < S; ++s) sum_a[s] = 0.f;
   const int first = at.first_chunk(T), live = at.live_end(T), end = at.end_chunk(T);
-  const bool gate = P.z.data, soft = P.softplus;
+  const bool gate = P.z.data, soft = P.softplus, skip = P.d;  // (without D its terms are left out: zero times an infinite input is NaN)
   Piece<DT, E, WHOLE> x{}, dt{}, z{}, dout{}, xa{}, dta{}, za{}, douta{};  // of the chunk that is prepared next, and of the one in front of it
   const int64_t l0 = (int64_t)(live - 1) * K, lr = l0 + at.r, wq = at.readable(), wo = at.w0 + at.q;
   Rows<DT, S, NL> rb(P.b, at, l0, P.state), rc(P.c, at, l0, P.state);
@@ -656,9 +656,10 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
   auto finish = [&](int i, int half) {
     const float du = dus[at.r][at.q + i], ta = tas[at.r][at.q + i], y = ys[half][at.r][at.q + i], xi = k2.x[i], zi = k2.z[i];
     const float d = __builtin_fmaf(du, xi, ta * 0.693147180559945309f);
-    dx[i] = __builtin_fmaf(du, k2.step[i], D[i] * k2.dy[i]);
+    dx[i] = __builtin_fmaf(du, k2.step[i], skip ? D[i] * k2.dy[i] : 0.f);
     ddt[i] = soft ? k2.slope[i] * d : d;
-    dz[i] = k2.dout[i] * __builtin_fmaf(D[i], xi, y) * silu_slope(zi, k2.sz[i]);
+    const float with_x = __builtin_fmaf(D[i], xi, y);
+    dz[i] = k2.dout[i] * (skip ? with_x : y) * silu_slope(zi, k2.sz[i]);
   };
   auto finish_bc = [&] {
 #pragma unroll
@@ -923,7 +924,8 @@ __global__ __launch_bounds__(256) void k_scan_step4(afc_scan_args P, int tiles) 
       y = __builtin_fmaf((float)C[r][i], h[r][i], y);
     }
     if (on) *reinterpret_cast<F4 *>(P.final_state + st + r * row) = h[r];
-    y = __builtin_fmaf(D, xr, sum_side<NL>(y));
+    y = sum_side<NL>(y);
+    if (P.d) y = __builtin_fmaf(D, xr, y);
     if (P.z.data) y *= silu((float)z[r]);
     if (n == 0) ((E *)P.y.data)[(b0 + r) * P.y.stride_batch + w] = (E)y;
   }

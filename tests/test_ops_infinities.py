@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from rlfluidcontrol_amd import ops
-from tests.test_ops import conv_case
+from tests.test_ops import conv_case, scan_case
 
 INF = float("inf")
 
@@ -40,7 +40,47 @@ def an_infinite_input(device):
             assert bool(torch.isfinite(dw[torch.arange(5) != 2]).all())
 
 
-CHECKS = [an_infinite_last_input, an_infinite_input]
+def no_skip(device):
+    """without D there is no term D x: what is infinite stays infinite and does not turn to NaN (a state that a kernel fills up to the next
+    size has zeros there, so that it may be either)"""
+    for N, W in ((16, 20), (64, 6), (4, 37), (8, 70), (3, 8), (5, 70)):
+        def is_infinite(t):
+            return t == INF if N % 4 == 0 else ~torch.isfinite(t)
+
+        c = scan_case(N, 2, 40, W, N, device=device, D=False, z=False)
+        c["B"], c["C"] = c["B"].abs() + 0.1, c["C"].abs() + 0.1
+        x = c["x"].clone()
+        x[1, 21, 2] = INF
+        args = (x, c["dt"], c["A"], c["B"], c["C"])
+        y = ops.selective_scan(*args, dt_bias=c["dt_bias"], softplus=True, initial_state=c["state"])
+        inf = torch.zeros_like(y, dtype=torch.bool)
+        inf[1, 21:, 2] = True
+        assert torch.equal(is_infinite(y), inf) and bool(torch.isfinite(y[~inf]).all()), N
+        state = c["state"].clone()
+        step = ops.selective_scan_step(*(t[:, 21] if t.dim() > 2 else t for t in args), state, dt_bias=c["dt_bias"], softplus=True)
+        assert torch.equal(is_infinite(step), inf[:, 21]) and bool(torch.isfinite(step[~inf[:, 21]]).all()), N
+        leaf, dy = c["x"].detach().clone().requires_grad_(), c["dy"].clone()
+        dy[1, 21, 2] = INF
+        y = ops.selective_scan(leaf, *args[1:], dt_bias=c["dt_bias"], softplus=True, initial_state=c["state"])
+        dx, = torch.autograd.grad(y, [leaf], [dy])
+        inf = torch.zeros_like(inf)
+        inf[1, :22, 2] = True
+        assert torch.equal(is_infinite(dx), inf) and bool(torch.isfinite(dx[~inf]).all()), N
+
+
+def no_skip_with_a_gate(device):
+    c = scan_case(8, 2, 40, 20, 16, device=device, D=False)
+    c["B"], c["C"], c["dy"] = c["B"].abs() + 0.1, c["C"].abs() + 0.1, c["dy"].abs() + 0.1
+    c["z"] = c["z"].abs() + 0.1  # the gate's slope is positive
+    x, z = c["x"].clone(), c["z"].detach().clone().requires_grad_()
+    x[1, 21, 2] = INF
+    y = ops.selective_scan(x, c["dt"], c["A"], c["B"], c["C"], z=z, dt_bias=c["dt_bias"], softplus=True)
+    dz, = torch.autograd.grad(y, [z], [c["dy"]])
+    assert bool((y[1, 21:, 2] == INF).all()) and bool((dz[1, 21:, 2] == INF).all())
+    assert int(torch.isfinite(dz).sum()) == dz.numel() - 19
+
+
+CHECKS = [an_infinite_last_input, an_infinite_input, no_skip, no_skip_with_a_gate]
 
 
 @pytest.mark.parametrize("which", CHECKS)
