@@ -726,6 +726,41 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
     take();
     __syncthreads();
   }
+  // The chunk in which the row ends, the first one here.  Behind the end the step size is zero, but zero times a state or an adjoint
+  // that is not finite is NaN, and the formula's sum does not go there: if it is NaN it is taken again over the row's own positions,
+  // each with the state in front of it from the checkpoint on.
+  auto rates_at_the_end = [&](int ch, int half) {
+    bool again = false;
+#pragma unroll
+    for (int s = 0; s < S; ++s) again |= sum_a[s] != sum_a[s];
+    if (!__any(again)) return;
+    Place<S, NL> my = at;
+    asm volatile("" : "+v"(my.cb), "+v"(my.nl));  // (addresses from here on are not worked out ahead of the loop: up to 6 registers less)
+    float ge[S], he[S], B[S], C[S];
+    state_or_zero<S, NL>(ge, P.dfinal_state, P, my);
+#pragma unroll
+    for (int s = 0; s < S; ++s) sum_a[s] = 0.f;
+#pragma unroll 1
+    for (int k = at.len - ch * K - 1; k >= 0; --k) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) he[s] = 0.f;
+      if (my.cb < my.nw) load_states<S>(he, P.checkpoints + (((int64_t)at.b * T.chunks + ch) * P.width + my.w0 + my.cb) * H::NP + my.nl * S);
+#pragma unroll 1
+      for (int j = 0; j < k; ++j) {
+        const float2 d = steps[half][j][my.cb];
+        load_states<S>(B, bs[half] + j * H::NP + my.nl * S);
+#pragma unroll
+        for (int s = 0; s < S; ++s) he[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(d.x * a2[s]), he[s], d.y * B[s]);
+      }
+      const float delta = steps[half][k][my.cb].x, dyk = dys[half][k][my.cb];
+      load_states<S>(C, cs[half] + k * H::NP + my.nl * S);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        ge[s] = __builtin_amdgcn_exp2f(delta * a2[s]) * __builtin_fmaf(dyk, C[s], ge[s]);
+        sum_a[s] = __builtin_fmaf(ge[s] * he[s], delta, sum_a[s]);
+      }
+    }
+  };
   for (int ch = live - 1; ch >= first; --ch) {
     const int half = (live - 1 - ch) & 1;
 #pragma unroll
@@ -796,6 +831,7 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
 #pragma unroll
       for (int i = k4 / 4 * E / 4; i < (k4 / 4 + 1) * E / 4; ++i) prepare(i, ch - 1);
     }
+    if ((ch + 1) * K > at.len) rates_at_the_end(ch, half);
     put(half ^ 1);
     keep();
     take();

@@ -80,7 +80,43 @@ def no_skip_with_a_gate(device):
     assert int(torch.isfinite(dz).sum()) == dz.numel() - 19
 
 
-CHECKS = [an_infinite_last_input, an_infinite_input, no_skip, no_skip_with_a_gate]
+def a_row_that_ends_in_an_infinite_state(device):
+    """no position of the row comes after that state, so the rates' gradient does not meet it"""
+    for N, W, L, lengths in ((16, 20, 40, [40, 21, 1]), (3, 8, 20, [16, 17, 20]), (64, 6, 300, [299, 33, 32]), (8, 40, 600, [600, 590, 1])):
+        c = scan_case(N, 3, L, W, N, device=device, lengths=lengths)
+        for dlast in (False, True):
+            grads = []
+            for last in (1.0, INF):
+                x = c["x"].clone()
+                for b, n in enumerate(lengths):
+                    x[b, n - 1, 1] = last
+                A, dt = c["A"].detach().clone().requires_grad_(), c["dt"].detach().clone().requires_grad_()
+                y, h = ops.selective_scan(x, dt, A, c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], c["lengths"], return_final_state=True)
+                grads.append(torch.autograd.grad([y] + [h] * dlast, [A, dt], [c["dy"]] + [c["dlast"]] * dlast))
+            assert bool(torch.isfinite(grads[0][0]).all()) and torch.equal(grads[0][0], grads[1][0]), (N, dlast)
+            for b, n in enumerate(lengths):  # and of the step sizes only the last one's does
+                assert torch.equal(grads[0][1][b, :n - 1], grads[1][1][b, :n - 1]) and not bool(grads[1][1][b, n:].any())
+
+
+def an_infinite_adjoint_of_the_final_state(device):
+    """it reaches the rates' gradient through the row's own positions: infinite and not NaN, wherever the row ends"""
+    for N, W, L, lengths in ((16, 20, 40, [40, 21, 2]), (64, 6, 40, [33, 32, 31]), (8, 40, 600, [600, 590, 3])):
+        c = scan_case(N, 3, L, W, N, device=device, lengths=lengths)
+        c["state"] = c["state"].abs() + 0.1  # every state in front of a position is positive
+        c["B"], c["x"] = c["B"].abs(), c["x"].abs()
+        for b in range(3):
+            dlast = c["dlast"].clone()
+            dlast[b, 1, 2] = INF
+            A = c["A"].detach().clone().requires_grad_()
+            A.data[1, 2] = -0.001  # (nothing on the way back through a long row is so small that it comes to zero)
+            y, h = ops.selective_scan(c["x"], c["dt"], A, c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], c["lengths"], return_final_state=True)
+            dA, = torch.autograd.grad([y, h], [A], [c["dy"], dlast])
+            want = torch.zeros_like(dA, dtype=torch.bool)
+            want[1, 2] = True
+            assert torch.equal(dA == INF, want) and bool(torch.isfinite(dA[~want]).all()), (N, b)
+
+
+CHECKS = [an_infinite_adjoint_of_the_final_state, an_infinite_last_input, an_infinite_input, a_row_that_ends_in_an_infinite_state, no_skip, no_skip_with_a_gate]
 
 
 @pytest.mark.parametrize("which", CHECKS)
