@@ -246,8 +246,10 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
           d = WHOLE || q < len ? d : 0.f;
           dp[K - 1][i] = d;
           // (where the run or the row has ended nothing is added, not even zero times an input: that one may be infinite)
-          for (int k = 0; k < K; ++k) dw[k][i] = WHOLE || q < inner ? __builtin_fmaf(d, xw[k][i], dw[k][i]) : dw[k][i];
-          dw[K][i] += WHOLE || q < inner ? d : 0.f;
+          if (WHOLE || q < inner) {
+            for (int k = 0; k < K; ++k) dw[k][i] = __builtin_fmaf(d, xw[k][i], dw[k][i]);
+            dw[K][i] += d;
+          }
           for (int k = 0; k < K; ++k) v[i] = WHOLE && k == 0 ? w[0][i] * dp[K - 1][i] : __builtin_fmaf(w[k][i], dp[K - 1 - k][i], v[i]);
           v[i] = WHOLE || l < len ? v[i] : 0.f;
         }
