@@ -464,10 +464,15 @@ __global__ __launch_bounds__(256) void k_scan(afc_scan_args P, Plan T, Carry car
 
 // ---- backwards ----
 // sums that are finished by k_scan_sums: bc [batch, groups, tiles, length, 2, NP], a [batch, segs, width, NP], d
-// and bias [batch, segs, width]
+// and bias [batch, segs, width]; others [batch, width, NP]: see kLastChunk
 struct Sums {
-  float *bc, *a, *d, *bias;
+  float *bc, *a, *d, *bias, *others;
 };
+
+// Behind a row's end the step size is zero, but zero times a state or an adjoint that is not finite is NaN, where dA's formula has no
+// term at all.  The chunk in which a row ends is the first one that k_scan_grad takes; if its share of dA is NaN the share is left
+// out, the others' sum goes to Sums.others and this NaN to Sums.a, and k_scan_sums takes the share over the row's own positions.
+constexpr unsigned kLastChunk = 0x7fc0afc1u;
 
 // What a part hands on to the one before it, from a zero adjoint behind it (of all parts but the first)
 template <int DT, int S, int NL, bool WHOLE>
@@ -617,6 +622,7 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
     rb.take(), rc.take();
   };
   float h[S], h0[S];
+  bool left_out = false;
   auto fetch_state = [&](int ch) {
 #pragma unroll
     for (int s = 0; s < S; ++s) h0[s] = 0.f;
@@ -726,41 +732,6 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
     take();
     __syncthreads();
   }
-  // The chunk in which the row ends, the first one here.  Behind the end the step size is zero, but zero times a state or an adjoint
-  // that is not finite is NaN, and the formula's sum does not go there: if it is NaN it is taken again over the row's own positions,
-  // each with the state in front of it from the checkpoint on.
-  auto rates_at_the_end = [&](int ch, int half) {
-    bool again = false;
-#pragma unroll
-    for (int s = 0; s < S; ++s) again |= sum_a[s] != sum_a[s];
-    if (!__any(again)) return;
-    Place<S, NL> my = at;
-    asm volatile("" : "+v"(my.cb), "+v"(my.nl));  // (addresses from here on are not worked out ahead of the loop: up to 6 registers less)
-    float ge[S], he[S], B[S], C[S];
-    state_or_zero<S, NL>(ge, P.dfinal_state, P, my);
-#pragma unroll
-    for (int s = 0; s < S; ++s) sum_a[s] = 0.f;
-#pragma unroll 1
-    for (int k = at.len - ch * K - 1; k >= 0; --k) {
-#pragma unroll
-      for (int s = 0; s < S; ++s) he[s] = 0.f;
-      if (my.cb < my.nw) load_states<S>(he, P.checkpoints + (((int64_t)at.b * T.chunks + ch) * P.width + my.w0 + my.cb) * H::NP + my.nl * S);
-#pragma unroll 1
-      for (int j = 0; j < k; ++j) {
-        const float2 d = steps[half][j][my.cb];
-        load_states<S>(B, bs[half] + j * H::NP + my.nl * S);
-#pragma unroll
-        for (int s = 0; s < S; ++s) he[s] = __builtin_fmaf(__builtin_amdgcn_exp2f(d.x * a2[s]), he[s], d.y * B[s]);
-      }
-      const float delta = steps[half][k][my.cb].x, dyk = dys[half][k][my.cb];
-      load_states<S>(C, cs[half] + k * H::NP + my.nl * S);
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        ge[s] = __builtin_amdgcn_exp2f(delta * a2[s]) * __builtin_fmaf(dyk, C[s], ge[s]);
-        sum_a[s] = __builtin_fmaf(ge[s] * he[s], delta, sum_a[s]);
-      }
-    }
-  };
   for (int ch = live - 1; ch >= first; --ch) {
     const int half = (live - 1 - ch) & 1;
 #pragma unroll
@@ -831,7 +802,12 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
 #pragma unroll
       for (int i = k4 / 4 * E / 4; i < (k4 / 4 + 1) * E / 4; ++i) prepare(i, ch - 1);
     }
-    if ((ch + 1) * K > at.len) rates_at_the_end(ch, half);
+    if ((ch + 1) * K > at.len) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) left_out |= sum_a[s] != sum_a[s];
+#pragma unroll
+      for (int s = 0; s < S; ++s) sum_a[s] = left_out ? 0.f : sum_a[s];
+    }
     put(half ^ 1);
     keep();
     take();
@@ -844,6 +820,11 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
     put_grads(first);
   }
   const int64_t row = (int64_t)at.b * T.segs + at.seg;
+  if (left_out && at.cb < at.nw) {
+    store_states<S>(sums.others + ((int64_t)at.b * P.width + w) * H::NP + at.nl * S, sum_a);
+#pragma unroll
+    for (int s = 0; s < S; ++s) sum_a[s] = __builtin_bit_cast(float, kLastChunk);
+  }
   if (at.cb < at.nw) store_states<S>(sums.a + (row * P.width + w) * H::NP + at.nl * S, sum_a);
   if (at.seg == 0) put_state<S, NL>(P.dinitial_state, g, P, at);
   __syncthreads();
@@ -863,6 +844,35 @@ __global__ __launch_bounds__(256) void k_scan_grad(afc_scan_args P, Plan T, Carr
     sums.d[row * P.width + at.w0 + threadIdx.x] = sd;
     sums.bias[row * P.width + at.w0 + threadIdx.x] = sb;
   }
+}
+
+// A row's last chunk's share of dA for one state of one channel, over the row's own positions alone, one after the other, each with the
+// state in front of it from the checkpoint on (only where k_scan_grad has left it out: nothing here is fast).
+template <int DT>
+__device__ inline float last_share(const afc_scan_args &P, const Plan &T, int NP, int64_t b, int64_t w, int n) {
+  typedef Elem<DT> E;
+  const int len = row_length(P.lengths, b, P.length), chunk = (len - 1) / K, l0 = chunk * K;
+  const int64_t g = w / (P.width / P.groups), state = (b * P.width + w) * P.state + n;
+  const float a2 = rate2(P.a[w * P.state + n]), bias = P.dt_bias ? P.dt_bias[w] : 0.f;
+  auto of = [&](const afc_seq &s, int l, int64_t i) { return (float)((const E *)s.data)[b * s.stride_batch + l * s.stride_length + i]; };
+  auto step = [&](int l) {
+    const float v = of(P.dt, l, w) + bias;
+    return P.softplus ? softplus(v) : v;
+  };
+  float adjoint = P.dfinal_state ? P.dfinal_state[state] : 0.f, sum = 0.f;
+#pragma unroll 1
+  for (int l = len - 1; l >= l0; --l) {
+    float h = P.checkpoints[((b * T.chunks + chunk) * P.width + w) * NP + n];
+#pragma unroll 1
+    for (int j = l0; j < l; ++j) {
+      const float delta = step(j);
+      h = __builtin_fmaf(__builtin_amdgcn_exp2f(delta * a2), h, delta * of(P.x, j, w) * of(P.b, j, g * P.b.stride_group + n));
+    }
+    const float delta = step(l), dout = of(P.dy, l, w), dy = P.z.data ? dout * silu(of(P.z, l, w)) : dout;
+    adjoint = __builtin_amdgcn_exp2f(delta * a2) * __builtin_fmaf(dy, of(P.c, l, g * P.c.stride_group + n), adjoint);
+    sum = __builtin_fmaf(adjoint * h, delta, sum);
+  }
+  return sum;
 }
 
 // The sums that the blocks of k_scan_grad leave, in one launch (two cost 1 to 4 us more: 8 x 64 x 256 both ways
@@ -891,10 +901,20 @@ __global__ __launch_bounds__(1024) void k_scan_sums(afc_scan_args P, Plan T, Sum
   const int which = col < na ? 0 : col < na + P.width ? 1 : 2;
   const int64_t at = which == 0 ? col : col - na - (which - 1) * P.width, cols = which == 0 ? na : P.width;
   const float *from = which == 0 ? sums.a : which == 1 ? sums.d : sums.bias;
-  const float a = column_sum(from, rows, cols, at, red);
+  float a = column_sum(from, rows, cols, at, red);
   if (threadIdx.x >= 64 || at >= cols) return;
   if (which == 0) {
-    if (P.da && at % NP < P.state) P.da[at / NP * P.state + at % NP] = a;
+    const int n = (int)(at % NP);
+    if (!P.da || n >= P.state) return;
+    if (a != a) {
+      a = 0.f;
+      for (int64_t r = 0; r < rows; ++r) {
+        const float v = from[r * cols + at];
+        const int64_t b = r / T.segs;
+        a += __builtin_bit_cast(unsigned, v) == kLastChunk ? sums.others[b * cols + at] + last_share<DT>(P, T, NP, b, at / NP, n) : v;
+      }
+    }
+    P.da[at / NP * P.state + n] = a;
   } else if (which == 1) {
     if (P.dd) P.dd[at] = a;
   } else if (P.ddt_bias) {
@@ -1141,7 +1161,7 @@ void scan(const afc_scan_args *p, hipStream_t st) {
 
 // the workspace of the gradients, one part after the other
 struct Layout {
-  uint64_t carry, bc, a, d, bias, all;
+  uint64_t carry, bc, a, d, bias, others, all;
 };
 Layout layout(const afc_scan_args *p, const Plan &t) {
   Layout o;
@@ -1151,7 +1171,8 @@ Layout layout(const afc_scan_args *p, const Plan &t) {
   o.a = o.bc + up256((uint64_t)p->batch * p->groups * t.tiles * p->length * 2 * padded(p) * 4);
   o.d = o.a + up256(rows * padded(p));
   o.bias = o.d + up256(rows);
-  o.all = o.bias + up256(rows);
+  o.others = o.bias + up256(rows);
+  o.all = o.others + up256((uint64_t)p->batch * p->width * padded(p) * 4);
   return o;
 }
 
@@ -1166,7 +1187,7 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   OnDevice on(p->device);
   char *ws = (char *)p->workspace;
   const Carry carry = carry_at(p, t);
-  const Sums sums = {(float *)(ws + o.bc), (float *)(ws + o.a), (float *)(ws + o.d), (float *)(ws + o.bias)};
+  const Sums sums = {(float *)(ws + o.bc), (float *)(ws + o.a), (float *)(ws + o.d), (float *)(ws + o.bias), (float *)(ws + o.others)};
   if (p->batch > 0) {
     const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
     if (t.segs > 1) {
