@@ -212,7 +212,7 @@ namespace {
 
 void check(const afc_clip_args *p) {
   want(p != nullptr, "null arguments");
-  want(p->count >= 0 && p->count < 1 << 24, "count");
+  want(p->count >= 0 && p->count < 1 << 23, "count");  // (with the 4096 blocks that share large ones, 2^24 blocks of 256 in a launch)
   want(p->count == 0 || (p->in && p->numel && p->in_dtype), "an array is missing");
   int64_t all = 0;
   for (int i = 0; i < p->count; ++i) {

@@ -47,6 +47,7 @@ struct Tiling {
   int log_cx;          // lanes side by side along the channels (the others: positions)
   int run;             // positions of a thread
   int64_t tiles_c, tiles_l;
+  int64_t base;        // the slice's first block
 };
 
 // A thread takes T.run positions of V channels (16 bytes of a row): the filter and the last K - 1 inputs stay in registers, and
@@ -57,7 +58,7 @@ template <int DT, int V, int K, bool SILU>
 __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
   typedef Elem<DT> E;
   constexpr int U = 4;
-  int64_t blk = blockIdx.x;
+  int64_t blk = T.base + blockIdx.x;
   const int64_t ct = blk % T.tiles_c;
   blk /= T.tiles_c;
   const int64_t lt = blk % T.tiles_l, b = blk / T.tiles_l;
@@ -129,9 +130,9 @@ __global__ __launch_bounds__(256) void k_conv(afc_conv_args P, Tiling T) {
 }
 
 template <int DT, int V, int K, bool SILU>
-__global__ __launch_bounds__(256) void k_conv_step(afc_conv_args P) {
+__global__ __launch_bounds__(256) void k_conv_step(afc_conv_args P, int64_t base) {
   typedef Elem<DT> E;
-  const int64_t per = P.width / V, t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t per = P.width / V, t = (base + blockIdx.x) * 256 + threadIdx.x;
   if (t >= P.batch * per) return;
   const int64_t b = t / per, c = (t - b * per) * V;
   E *st = (E *)P.final_state + b * (K - 1) * P.width + c;
@@ -161,7 +162,7 @@ template <int DT, int V, int K, bool SILU>
 __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, float *part) {
   typedef Elem<DT> E;
   __shared__ float red[256 * V];
-  int64_t blk = blockIdx.x;
+  int64_t blk = T.base + blockIdx.x;
   const int64_t ct = blk % T.tiles_c;
   blk /= T.tiles_c;
   const int64_t lt = blk % T.tiles_l, b = blk / T.tiles_l;
@@ -287,9 +288,9 @@ __global__ __launch_bounds__(256) void k_conv_grad(afc_conv_args P, Tiling T, fl
 
 // dweight, dbias: the partial rows summed in their order
 __global__ __launch_bounds__(1024) void k_conv_params(const float *part, int64_t rows, int64_t width, int taps, float *dweight,
-                                                      float *dbias) {
+                                                      float *dbias, int64_t base) {
   __shared__ float red[1024];
-  const int64_t cols = (taps + 1) * width, col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int64_t cols = (taps + 1) * width, col = (base + blockIdx.x) * 64 + (threadIdx.x & 63);
   const float a = column_sum(part, rows, cols, col, red);
   if (threadIdx.x >= 64 || col >= cols) return;
   const int64_t k = col / width, w = col - k * width;
@@ -332,11 +333,12 @@ Tiling tiling(const afc_conv_args *p, int v, int run) {
   t.run = run;
   t.tiles_c = ceil_div(lanes, 1 << t.log_cx);
   t.tiles_l = ceil_div(p->length > 0 ? p->length : 1, (int64_t)run * (256 >> t.log_cx));
+  t.base = 0;
   return t;
 }
 int64_t blocks(const afc_conv_args *p, const Tiling &t) {
   const int64_t n = p->batch * t.tiles_l * t.tiles_c;
-  want(n < (int64_t)1 << 31, "too many blocks");
+  want(n < kMostBlocks, "too many blocks");
   return n;
 }
 // Positions of a thread: long runs read the filter and the K - 1 positions that neighbours share less often (and leave fewer
@@ -373,36 +375,37 @@ uint64_t grad_bytes(const afc_conv_args *p) {
 
 static void conv(const afc_conv_args *p, hipStream_t st) {
   check(p, false, false);
-  OnDevice on(p->device);
-  if (p->batch == 0 || (p->length == 0 && !p->final_state)) return;
   const int v = 16 / elem_bytes(p->dtype);
   const bool wide = p->width >= v;
   const Tiling t = run_tiling(p, wide ? v : 1, 32);
-  const dim3 grid((unsigned)blocks(p, t));
-#define CONV_GO(DT, V, K, S, ...) (k_conv<DT, V, K, S><<<grid, 256, 0, st>>>(*p, t), 0)
-  (void)CONV_TYPES(wide, 4, 8);
+  const int64_t n = blocks(p, t);
+  OnDevice on(p->device);
+  if (p->length == 0 && !p->final_state) return;
+  in_slices(n, 256, "k_conv", [&](int64_t base, dim3 grid) {
+    Tiling s = t;
+    s.base = base;
+#define CONV_GO(DT, V, K, S, ...) (k_conv<DT, V, K, S><<<grid, 256, 0, st>>>(*p, s), 0)
+    (void)CONV_TYPES(wide, 4, 8);
 #undef CONV_GO
-  launched("k_conv");
+  });
 }
 
 static void conv_step(const afc_conv_args *p, hipStream_t st) {
   check(p, false, true);
-  OnDevice on(p->device);
-  if (p->batch == 0) return;
   const int v = 16 / elem_bytes(p->dtype);
   const bool wide = p->width % v == 0;  // (the state is updated in place: no two lanes may share a channel)
   const int64_t n = ceil_div(p->batch * (p->width / (wide ? v : 1)), 256);
-  want(n < (int64_t)1 << 31, "too many blocks");
-  const dim3 grid((unsigned)n);
-#define CONV_GO(DT, V, K, S, ...) (k_conv_step<DT, V, K, S><<<grid, 256, 0, st>>>(*p), 0)
-  (void)CONV_TYPES(wide, 4, 8);
+  want(n < kMostBlocks, "too many blocks");
+  OnDevice on(p->device);
+  in_slices(n, 256, "k_conv_step", [&](int64_t base, dim3 grid) {
+#define CONV_GO(DT, V, K, S, ...) (k_conv_step<DT, V, K, S><<<grid, 256, 0, st>>>(*p, base), 0)
+    (void)CONV_TYPES(wide, 4, 8);
 #undef CONV_GO
-  launched("k_conv_step");
+  });
 }
 
 static void conv_grad(const afc_conv_args *p, hipStream_t st) {
   check(p, true, false);
-  OnDevice on(p->device);
   const bool params = p->dweight || p->dbias;
   const bool wide = p->width >= kGradVector;
   const Tiling t = grad_tiling(p, wide ? kGradVector : 1);
@@ -410,18 +413,19 @@ static void conv_grad(const afc_conv_args *p, hipStream_t st) {
   const int64_t rows = p->batch * t.tiles_l;
   if (params)
     want(p->batch == 0 || (part && p->workspace_bytes >= grad_bytes(p) && (uintptr_t)part % 256 == 0), "workspace is missing, too small or not 256-byte aligned");
-  if (p->batch > 0) {
-    const dim3 grid((unsigned)blocks(p, t));
-#define CONV_GO(DT, V, K, S, ...) (k_conv_grad<DT, V, K, S><<<grid, 256, 0, st>>>(*p, t, part), 0)
+  const int64_t n = blocks(p, t);
+  OnDevice on(p->device);
+  in_slices(n, 256, "k_conv_grad", [&](int64_t base, dim3 grid) {
+    Tiling s = t;
+    s.base = base;
+#define CONV_GO(DT, V, K, S, ...) (k_conv_grad<DT, V, K, S><<<grid, 256, 0, st>>>(*p, s, part), 0)
     (void)CONV_TYPES(wide, 4, 4);
 #undef CONV_GO
-    launched("k_conv_grad");
-  }
-  if (params) {
-    const dim3 grid((unsigned)ceil_div((p->taps + 1) * p->width, 64));
-    k_conv_params<<<grid, 1024, 0, st>>>(part, rows, p->width, p->taps, p->dweight, p->dbias);
-    launched("k_conv_params");
-  }
+  });
+  if (params)
+    in_slices(ceil_div((p->taps + 1) * p->width, 64), 1024, "k_conv_params", [&](int64_t base, dim3 grid) {
+      k_conv_params<<<grid, 1024, 0, st>>>(part, rows, p->width, p->taps, p->dweight, p->dbias, base);
+    });
 }
 
 }  // namespace afc_ops

@@ -48,6 +48,18 @@ struct OnDevice {
 
 inline void launched(const char *what) { hip(hipGetLastError(), what); }
 
+// A launch has fewer than 2^32 threads along x, so more blocks than that go in slices: launch(base, blocks of the slice), the kernel's
+// blocks counting from `base`.  (At sizes that real programs have there is one.)
+template <class F>
+void in_slices(int64_t blocks, int threads, const char *what, F &&launch) {
+  const int64_t most = (((int64_t)1 << 32) - 1) / threads;
+  for (int64_t base = 0; base < blocks; base += most) {
+    launch(base, dim3((unsigned)(blocks - base < most ? blocks - base : most)));
+    launched(what);
+  }
+}
+constexpr int64_t kMostBlocks = (int64_t)1 << 31;  // of all slices of a launch
+
 // no exception passes a C entry
 template <class F>
 int entry(const char *name, F &&f) {

@@ -35,6 +35,7 @@ struct Plan {
   int segs;        // parts of the length that run at the same time
   int seg_chunks;  // chunks of a part
   int chunks;
+  unsigned base;   // the slice's first block
 };
 
 template <int CTRL>
@@ -176,7 +177,7 @@ struct Place {
   int r, q, n;                   // before and after it: position r of the chunk, channels q .. q + n of the block
   int64_t w0;                    // the block's first channel
   __device__ Place(const afc_scan_args &P, const Plan &T) {
-    unsigned k = blockIdx.x;
+    unsigned k = T.base + blockIdx.x;
     seg = k % T.segs, k /= T.segs;
     tile = k % T.tiles, k /= T.tiles;
     g = k % (unsigned)P.groups, b = k / (unsigned)P.groups;
@@ -883,8 +884,9 @@ template <int DT>
 __global__ __launch_bounds__(1024) void k_scan_sums(afc_scan_args P, Plan T, Sums sums, int NP, int64_t bc_blocks) {
   typedef Elem<DT> E;
   __shared__ float red[1024];
-  if (blockIdx.x < bc_blocks) {
-    const int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x, per = 2 * NP;
+  const int64_t block = T.base + blockIdx.x;
+  if (block < bc_blocks) {
+    const int64_t i = block * 1024 + threadIdx.x, per = 2 * NP;
     if (i >= P.batch * P.groups * P.length * per) return;
     const int64_t row = i / (P.length * per), l = i / per % P.length, b = row / P.groups, g = row % P.groups;
     const int n = (int)(i % NP), c = (int)(i % per) / NP;
@@ -897,7 +899,7 @@ __global__ __launch_bounds__(1024) void k_scan_sums(afc_scan_args P, Plan T, Sum
     ((E *)s.data)[b * s.stride_batch + l * s.stride_length + g * s.stride_group + n] = (E)a;
     return;
   }
-  const int64_t rows = P.batch * T.segs, na = P.width * NP, col = ((int64_t)blockIdx.x - bc_blocks) * 64 + (threadIdx.x & 63);
+  const int64_t rows = P.batch * T.segs, na = P.width * NP, col = (block - bc_blocks) * 64 + (threadIdx.x & 63);
   const int which = col < na ? 0 : col < na + P.width ? 1 : 2;
   const int64_t at = which == 0 ? col : col - na - (which - 1) * P.width, cols = which == 0 ? na : P.width;
   const float *from = which == 0 ? sums.a : which == 1 ? sums.d : sums.bias;
@@ -936,11 +938,12 @@ __device__ inline float sum_side(float v) {
 }
 
 template <int DT, int NL, int R>
-__global__ __launch_bounds__(256) void k_scan_step4(afc_scan_args P, int tiles) {
+__global__ __launch_bounds__(256) void k_scan_step4(afc_scan_args P, int tiles, unsigned base) {
   typedef Elem<DT> E;
   typedef float F4 __attribute__((ext_vector_type(4)));
-  const int tile = blockIdx.x % tiles;
-  const int64_t b0 = (int64_t)(blockIdx.x / tiles) * R, w = (int64_t)tile * (256 / NL) + threadIdx.x / NL;
+  const unsigned block = base + blockIdx.x;
+  const int tile = block % tiles;
+  const int64_t b0 = (int64_t)(block / tiles) * R, w = (int64_t)tile * (256 / NL) + threadIdx.x / NL;
   const int n = threadIdx.x % NL * 4, rows = (int)min((int64_t)R, P.batch - b0);
   if (w >= P.width) return;
   const bool on = n < P.state;  // (a lane without states holds zeros: it takes part in the sums)
@@ -995,11 +998,11 @@ __device__ inline float sum_lanes(float v) {
 }
 
 template <int DT, int NP>
-__global__ __launch_bounds__(64) void k_scan_step(afc_scan_args P) {
+__global__ __launch_bounds__(64) void k_scan_step(afc_scan_args P, unsigned base) {
   typedef Elem<DT> E;
   const int n = threadIdx.x & (NP - 1);
-  const int64_t tiles = (P.width + 64 / NP - 1) / (64 / NP);
-  const int64_t b = blockIdx.x / tiles, w = (blockIdx.x % tiles) * (64 / NP) + threadIdx.x / NP;
+  const int64_t tiles = (P.width + 64 / NP - 1) / (64 / NP), block = base + blockIdx.x;
+  const int64_t b = block / tiles, w = (block % tiles) * (64 / NP) + threadIdx.x / NP;
   const bool on = w < P.width, mine = on && n < P.state;
   const int64_t g = on ? w / (P.width / P.groups) : 0, st = (b * P.width + w) * P.state + n;
   const float x = on ? (float)((const E *)P.x.data)[b * P.x.stride_batch + w] : 0.f;
@@ -1098,7 +1101,8 @@ Plan plan(const afc_scan_args *p, bool grad) {
     if (estimate(s) < estimate(segs)) segs = s;
   t.seg_chunks = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, segs);
   t.segs = (int)ceil_div(t.chunks > 0 ? t.chunks : 1, t.seg_chunks);
-  want(blocks * t.segs < (int64_t)1 << 31, "too many blocks");
+  want(blocks * t.segs < kMostBlocks, "too many blocks");
+  t.base = 0;
   return t;
 }
 
@@ -1140,6 +1144,15 @@ void check_workspace(const afc_scan_args *p, uint64_t bytes) {
        "workspace is missing, too small or not 256-byte aligned");
 }
 
+template <class F>
+void slices(const afc_scan_args *p, const Plan &t, const char *what, F &&launch) {
+  in_slices(p->batch * p->groups * t.tiles * t.segs, 256, what, [&](int64_t base, dim3 grid) {
+    Plan s = t;
+    s.base = (unsigned)base;
+    launch(s, grid);
+  });
+}
+
 void scan(const afc_scan_args *p, hipStream_t st) {
   check(p, false, false);
   const Plan t = plan(p, false);
@@ -1148,15 +1161,10 @@ void scan(const afc_scan_args *p, hipStream_t st) {
   OnDevice on(p->device);
   if (p->batch == 0) return;
   const Carry carry = carry_at(p, t);
-  const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
-#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan<DT, S, NL, WHOLE, C><<<grid, 256, 0, st>>>(*p, t, carry)
-  if (t.segs > 1) {
-    SCAN_ALL(true)
-    launched("k_scan (carry)");
-  }
-  SCAN_ALL(false)
+#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan<DT, S, NL, WHOLE, C><<<grid, 256, 0, st>>>(*p, s, carry)
+  if (t.segs > 1) slices(p, t, "k_scan (carry)", [&](const Plan &s, dim3 grid) { SCAN_ALL(true) });
+  slices(p, t, "k_scan", [&](const Plan &s, dim3 grid) { SCAN_ALL(false) });
 #undef SCAN_GO
-  launched("k_scan");
 }
 
 // the workspace of the gradients, one part after the other
@@ -1181,33 +1189,27 @@ void scan_grad(const afc_scan_args *p, hipStream_t st) {
   const Plan t = plan(p, true);
   const Layout o = layout(p, t);
   const int64_t bc = ceil_div(p->batch * p->length * p->groups * 2 * padded(p), 1024);
-  want(bc < (int64_t)1 << 30, "too many blocks");
+  want(bc < kMostBlocks, "too many blocks");
   if (p->batch > 0) check_workspace(p, o.all);
   want((uintptr_t)p->checkpoints % 16 == 0, "checkpoints must be 16-byte aligned");
   OnDevice on(p->device);
   char *ws = (char *)p->workspace;
   const Carry carry = carry_at(p, t);
   const Sums sums = {(float *)(ws + o.bc), (float *)(ws + o.a), (float *)(ws + o.d), (float *)(ws + o.bias), (float *)(ws + o.others)};
-  if (p->batch > 0) {
-    const dim3 grid((unsigned)(p->batch * p->groups * t.tiles * t.segs));
-    if (t.segs > 1) {
-#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan_grad_carry<DT, S, NL, WHOLE><<<grid, 256, 0, st>>>(*p, t, carry)
-      SCAN_ALL(0)
+#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan_grad_carry<DT, S, NL, WHOLE><<<grid, 256, 0, st>>>(*p, s, carry)
+  if (t.segs > 1) slices(p, t, "k_scan_grad_carry", [&](const Plan &s, dim3 grid) { SCAN_ALL(0) });
 #undef SCAN_GO
-      launched("k_scan_grad_carry");
-    }
-#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan_grad<DT, S, NL, WHOLE><<<grid, 256, 0, st>>>(*p, t, carry, sums)
-    SCAN_ALL(0)
+#define SCAN_GO(DT, S, NL, WHOLE, C) k_scan_grad<DT, S, NL, WHOLE><<<grid, 256, 0, st>>>(*p, s, carry, sums)
+  slices(p, t, "k_scan_grad", [&](const Plan &s, dim3 grid) { SCAN_ALL(0) });
 #undef SCAN_GO
-    launched("k_scan_grad");
-  }
   const int64_t params = p->da || p->dd || p->ddt_bias ? ceil_div(p->width * (padded(p) + 2), 64) : 0;
-  if (bc + params == 0) return;
-  const dim3 gs((unsigned)(bc + params));
-  if (p->dtype == AFC_F32) k_scan_sums<AFC_F32><<<gs, 1024, 0, st>>>(*p, t, sums, padded(p), bc);
-  if (p->dtype == AFC_BF16) k_scan_sums<AFC_BF16><<<gs, 1024, 0, st>>>(*p, t, sums, padded(p), bc);
-  if (p->dtype == AFC_F16) k_scan_sums<AFC_F16><<<gs, 1024, 0, st>>>(*p, t, sums, padded(p), bc);
-  launched("k_scan_sums");
+  in_slices(bc + params, 1024, "k_scan_sums", [&](int64_t base, dim3 grid) {
+    Plan s = t;
+    s.base = (unsigned)base;
+    if (p->dtype == AFC_F32) k_scan_sums<AFC_F32><<<grid, 1024, 0, st>>>(*p, s, sums, padded(p), bc);
+    if (p->dtype == AFC_BF16) k_scan_sums<AFC_BF16><<<grid, 1024, 0, st>>>(*p, s, sums, padded(p), bc);
+    if (p->dtype == AFC_F16) k_scan_sums<AFC_F16><<<grid, 1024, 0, st>>>(*p, s, sums, padded(p), bc);
+  });
 }
 
 int lanes(const afc_scan_args *p) {
@@ -1233,12 +1235,14 @@ void go_step4(const afc_scan_args *p, hipStream_t st) {
   // one, 1024 x 256 x 16 f32 9.4 and 9.8; below, one row keeps the chip busier
   const int rows = tiles * p->batch >= 4096 ? 4 : 1;
   const int64_t n = tiles * ceil_div(p->batch, rows);
-  want(n < (int64_t)1 << 31, "too many blocks");
-  const dim3 grid((unsigned)n);
-  if (rows == 4)
-    k_scan_step4<DT, NL, 4><<<grid, 256, 0, st>>>(*p, (int)tiles);
-  else
-    k_scan_step4<DT, NL, 1><<<grid, 256, 0, st>>>(*p, (int)tiles);
+  want(n < kMostBlocks, "too many blocks");
+  OnDevice on(p->device);
+  in_slices(n, 256, "k_scan_step4", [&](int64_t base, dim3 grid) {
+    if (rows == 4)
+      k_scan_step4<DT, NL, 4><<<grid, 256, 0, st>>>(*p, (int)tiles, (unsigned)base);
+    else
+      k_scan_step4<DT, NL, 1><<<grid, 256, 0, st>>>(*p, (int)tiles, (unsigned)base);
+  });
 }
 void step4(const afc_scan_args *p, hipStream_t st) {
 #define STEP4(DT)                                                          \
@@ -1247,23 +1251,21 @@ void step4(const afc_scan_args *p, hipStream_t st) {
   if (p->dtype == AFC_F32) STEP4(AFC_F32);
   if (p->dtype == AFC_BF16) STEP4(AFC_BF16);
   if (p->dtype == AFC_F16) STEP4(AFC_F16);
-  launched("k_scan_step4");
 }
 
 void scan_step(const afc_scan_args *p, hipStream_t st) {
   check(p, false, true);
-  OnDevice on(p->device);
-  if (p->batch == 0) return;
   if (p->state % 4 == 0 && (uintptr_t)p->final_state % 16 == 0 && (uintptr_t)p->a % 16 == 0) return step4(p, st);
   const int64_t n = p->batch * ceil_div(p->width, 64 / lanes(p));
-  want(n < (int64_t)1 << 31, "too many blocks");
-  const dim3 grid((unsigned)n);
-#define STEP_GO(DT, NP) k_scan_step<DT, NP><<<grid, 64, 0, st>>>(*p)
-  if (p->dtype == AFC_F32) STEP_STATE(AFC_F32)
-  if (p->dtype == AFC_BF16) STEP_STATE(AFC_BF16)
-  if (p->dtype == AFC_F16) STEP_STATE(AFC_F16)
+  want(n < kMostBlocks, "too many blocks");
+  OnDevice on(p->device);
+  in_slices(n, 64, "k_scan_step", [&](int64_t base, dim3 grid) {
+#define STEP_GO(DT, NP) k_scan_step<DT, NP><<<grid, 64, 0, st>>>(*p, (unsigned)base)
+    if (p->dtype == AFC_F32) STEP_STATE(AFC_F32)
+    if (p->dtype == AFC_BF16) STEP_STATE(AFC_BF16)
+    if (p->dtype == AFC_F16) STEP_STATE(AFC_F16)
 #undef STEP_GO
-  launched("k_scan_step");
+  });
 }
 
 }  // namespace

@@ -54,3 +54,24 @@ def negated_views_are_refused(device):
 
 def test_negated_views_are_refused():
     negated_views_are_refused("cpu")
+
+
+def test_launches_that_could_not_be_made_are_refused():
+    """made-up pointers: the checks come before any device, and before the first launch of a call"""
+    import ctypes as C
+    from tests import ops_abi as abi
+    from tests.test_ops import fake_conv, fake_scan
+    lib = abi.load()
+
+    def many(f, p):
+        assert f(C.byref(p), None) == -1 and b"too many blocks" in lib.afc_ops_last_error()
+
+    rows = (1 << 30) - 1
+    many(lib.afc_scan, fake_scan(batch=rows, length=1, groups=4))  # a block for each row and group
+    many(lib.afc_scan_step, fake_scan(batch=rows, length=1, state=3, width=1 << 12, groups=1, initial_state=4096, final_state=4096))
+    many(lib.afc_conv, fake_conv(batch=rows, length=1, width=1 << 12))
+    many(lib.afc_conv_grad, fake_conv(batch=rows, length=1, width=1 << 12))
+    many(lib.afc_scan_grad, fake_scan(batch=1 << 20, length=1 << 20, width=1, groups=1, state=64))  # 2^40 x 128 partial sums
+    p = abi.ClipArgs()
+    p.count, p.inp, p.numel, p.in_dtype = 1 << 23, 4096, 4096, 4096
+    assert lib.afc_clip_workspace(C.byref(p), C.byref(C.c_uint64())) == -1 and b"count" in lib.afc_ops_last_error()
