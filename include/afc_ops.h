@@ -78,7 +78,8 @@ int afc_conv_step(const afc_conv_args *args, void *hip_stream);
 
 /* delta = dt + dt_bias, or softplus of it;  h[b,l,w,:] = exp(delta a[w,:]) h[b,l-1,w,:] + delta x b[b,l,g(w),:];
  * y = <c[b,l,g(w),:], h> + d[w] x, times silu(z) where z is given;  g(w) = w / (width / groups).
- * The state is held in float.  a = -inf forgets everything at every delta but zero. */
+ * The state is held in float.  a = -inf (taken as -3.4e38) forgets everything at every delta of
+ * 1e-36 and more, and nothing at zero. */
 typedef struct afc_scan_args {
   int32_t device, dtype; /* dtype of x, dt, b, c, z, y and their gradients */
   int32_t softplus;

@@ -119,8 +119,8 @@ template <int DT>
 using Elem = typename ElemT<DT>::type;
 
 __device__ inline float exp_(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896341f); }
-// log2 e times a decay rate, finite from below: a rate of -inf forgets everything at any step size but zero, which is that of a
-// position behind a row's end
+// log2 e times a decay rate, finite from below: a rate of -inf forgets everything at any step size of 1e-36 and more (2^-340 is zero)
+// and nothing at zero, which is that of a position behind a row's end
 __device__ inline float rate2(float a) {
   const float r = a * 1.44269504088896341f;
   return r < -3.4e38f ? -3.4e38f : r;

@@ -168,7 +168,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False,
     x, dt, z [batch, length, width]; A [width, state] float32, state 1..64; B, C [batch, length, state] or
     [batch, length, groups, state] of x's type, groups dividing width (channel w uses group g = w // (width // groups));
     D, dt_bias [width] float32; initial_state [batch, width, state] float32 (default: zeros); lengths: see the module.  A rate
-    of -inf forgets everything at every step size but zero.
+    of -inf forgets everything at every step size of 1e-36 and more, and nothing at zero.
     Returns y, or (y, final_state).  Differentiable in everything but lengths, through y and final_state; a forward pass that
     will be differentiated also keeps states for the backward pass."""
     if _on_gpu(x):
@@ -331,7 +331,7 @@ def _plain_scan(x, dt, A, B, C_, D, z, dt_bias, softplus, state, lengths):
     delta = _mask(lengths, L, v)
     per = W // B.shape[2]
     Bf, Cf = (_mask(lengths, L, t.float()).repeat_interleave(per, dim=2) for t in (B, C_))
-    A = torch.where(A < -3e38, -3e38, A)  # a rate of -inf forgets all at any step size but zero (behind a row's end)
+    A = torch.where(A < -3e38, -3e38, A)  # a rate of -inf forgets all at any step size but the smallest and zero, that behind a row's end
     h = state if state is not None else xf.new_zeros(Bn, W, A.shape[1])
     ys = []
     for t in range(L):

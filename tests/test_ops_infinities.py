@@ -121,7 +121,21 @@ def an_infinite_adjoint_of_the_final_state(device):
             assert torch.equal(dA == INF, want) and bool(torch.isfinite(dA[~want]).all()), (N, b)
 
 
-CHECKS = [an_infinite_adjoint_of_the_final_state, an_infinite_last_input, an_infinite_input, a_row_that_ends_in_an_infinite_state, no_skip, no_skip_with_a_gate]
+def a_rate_without_memory_at_the_smallest_step(device):
+    for N, W in ((16, 20), (3, 8), (64, 6)):
+        for dtype in (torch.float32, torch.bfloat16):
+            x = torch.zeros(2, 3, W, device=device, dtype=dtype)
+            B = torch.ones(2, 3, N, device=device, dtype=dtype)
+            A = torch.full((W, N), -INF, device=device)
+            for delta, left in ((1.01e-36, 0.0), (0.0, 1.0)):  # (1.01: 16 bits round it to above 1e-36)
+                dt, h = torch.full_like(x, delta), torch.ones(2, W, N, device=device)
+                y, last = ops.selective_scan(x, dt, A, B, B, initial_state=h, return_final_state=True)
+                assert bool((last == left).all()) and bool((y == N * left).all()), (N, delta)
+                ops.selective_scan_step(x[:, 0], dt[:, 0], A, B[:, 0], B[:, 0], h)
+                assert bool((h == left).all()), (N, delta)
+
+
+CHECKS = [a_rate_without_memory_at_the_smallest_step, an_infinite_adjoint_of_the_final_state, an_infinite_last_input, an_infinite_input, a_row_that_ends_in_an_infinite_state, no_skip, no_skip_with_a_gate]
 
 
 @pytest.mark.parametrize("which", CHECKS)
