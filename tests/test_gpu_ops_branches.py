@@ -1,0 +1,74 @@
+"""The branches that only larger calls of rlfluidcontrol_amd.ops take: long runs of the convolution, rows of single tokens that are
+no multiple of four, clipping with more blocks and longer ones."""
+import pytest
+import torch
+
+from rlfluidcontrol_amd import ops
+from tests import ops_reference as ref
+from tests.test_gpu_ops import test_clip as check_clip
+from tests.test_ops import check_conv, conv_case, scan_case
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def run_of(B, L, W, v, longest):
+    """how many positions a thread of the convolution takes (run_tiling in conv.hip), and how many threads lie along the length of a block"""
+    v = v if W >= v else 1
+    lanes = -(-W // v)
+    cx = 1
+    while cx < 64 and cx < lanes:
+        cx *= 2
+    run = longest
+    while run > 8 and B * -(-L // (run * (256 // cx))) * -(-lanes // cx) < 1024:
+        run //= 2
+    return run, 256 // cx
+
+
+# (runs forwards and backwards)
+@pytest.mark.parametrize("dtype,B,L,W,K,runs", [
+    (F32, 1030, 200, 5, 4, (32, 64)), (BF16, 1030, 200, 9, 3, (32, 64)), (F32, 200, 130, 260, 4, (16, 16)), (F32, 256, 130, 260, 2, (32, 32)),
+    (F32, 520, 300, 130, 4, (32, 64)), (BF16, 350, 130, 517, 4, (32, 64)), (F16, 180, 130, 519, 3, (16, 32))])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_conv_runs(dtype, B, L, W, K, runs, ragged):
+    (forth, _), (back, along) = run_of(B, L, W, 4 if dtype == F32 else 8, 32), run_of(B, L, W, 4, 64)
+    assert (forth, back) == runs
+    lengths = None
+    if ragged:  # ends on runs and one off them, and anywhere
+        ends = [n for r in (forth, back) for k in range(L // r + 1) for n in (k * r - 1, k * r, k * r + 1) if 0 <= n <= L] + [0, 1, L - 1, L]
+        lengths = (ends + torch.randint(0, L + 1, (B,), generator=torch.Generator().manual_seed(B)).tolist())[:B]
+    c = conv_case(B + W, B, L, W, K, dtype, DEV, lengths)
+    got = check_conv(c, True)
+    # The sums of the filter's gradient are taken in parts: a thread's run, a block's threads, sixteen interleaved runs of four sums over
+    # the blocks' rows.  An element is in no more additions than that, whatever B L is.
+    args = (c["x"], c["weight"], c["bias"], True, c["state"], c["lengths"], c["dy"], c["dlast"])
+    r, m = ref.conv(*args), ref.conv(*args, magnitude=True)
+    k = ref.conv_bounds(m, dtype, c["x"], K, True)
+    rows = B * -(-L // (back * along))
+    for name in ("dweight", "dbias"):
+        assert ref.off(got[name], r[name], m[name], k[name] - B * L + back + along + rows // 64 + 24, F32) <= 1, name
+
+
+@pytest.mark.parametrize("dtype,B,W,N,G", [(BF16, 131, 4096, 16, 1), (F32, 1027, 256, 16, 1), (F16, 129, 4096, 12, 2), (F32, 130, 4100, 16, 1), (BF16, 1367, 700, 4, 1),
+                                           (F32, 241, 2050, 8, 1), (F16, 67, 2000, 32, 5), (F32, 66, 1000, 64, 2)])
+def test_scan_step_rows_in_fours(dtype, B, W, N, G):
+    lanes = next(k for k in (1, 2, 4, 8, 16) if 4 * k >= N)
+    assert -(-W // (256 // lanes)) * B >= 4096 and B % 4
+    c = scan_case(B + W, B, 2, W, N, G, dtype, DEV)
+    args = (c["x"], c["dt"], c["A"], c["B"], c["C"], c["D"], c["z"], c["dt_bias"], True, c["state"], None)
+    r, m = ref.scan(*args), ref.scan(*args, magnitude=True)
+    k = ref.scan_bounds(r, c["x"], N, G)
+    s = c["state"].clone()
+    ys = [ops.selective_scan_step(c["x"][:, l], c["dt"][:, l], c["A"], c["B"][:, l], c["C"][:, l], s, c["D"], c["z"][:, l], c["dt_bias"], True) for l in range(2)]
+    assert ref.off(torch.stack(ys, 1), r["y"], m["y"], k["y"], dtype) <= 1
+    assert ref.off(s, r["last"], m["last"], k["last"], F32) <= 1
+
+
+# more than 1024 blocks of 4096 elements (with tables of up to 24 and 120 tensors, and of more), then more than 2^24 elements
+@pytest.mark.parametrize("dtypes", [[F32], [BF16, F32, F16]])
+@pytest.mark.parametrize("sizes", [[250001] * 20, [50001] * 100, [36001] * 130, [9000001, 8500003, 5, 0, 70001], [180001] * 100, [140001] * 130])
+def test_clip_of_many_elements(dtypes, sizes):
+    blocks, chunk = sum(-(-n // 4096) for n in sizes), max(4096, -(-(-(-sum(sizes) // 4096)) // 2048) * 2048)
+    assert blocks > 1024 and (chunk > 4096) == (sum(sizes) > 1 << 24)
+    check_clip(sizes=sizes, dtypes=dtypes)
