@@ -7,6 +7,7 @@ from rlfluidcontrol_amd import ops
 from tests import ops_reference as ref
 from tests.test_gpu_ops import test_clip as check_clip
 from tests.test_ops import check_conv, conv_case, scan_case
+from tests.test_ops_bounds import LONG, check_long_scan
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -72,3 +73,8 @@ def test_clip_of_many_elements(dtypes, sizes):
     blocks, chunk = sum(-(-n // 4096) for n in sizes), max(4096, -(-(-(-sum(sizes) // 4096)) // 2048) * 2048)
     assert blocks > 1024 and (chunk > 4096) == (sum(sizes) > 1 << 24)
     check_clip(sizes=sizes, dtypes=dtypes)
+
+
+@pytest.mark.parametrize("shape", LONG)
+def test_long_scans_within_bounds_that_follow_the_recurrence(shape):
+    check_long_scan(shape, DEV, 256)
