@@ -75,6 +75,7 @@ void no_grad(const T &...t) {
 }
 
 Tensor value(const Maybe &t) { return t ? *t : Tensor(); }
+Maybe maybe(const Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
 
 // A kernel knows nothing of forward-mode derivatives: what it writes would have none, which PyTorch takes for zero.
 bool has_tangent(const Tensor &t) { return t.defined() && t._fw_grad(0).defined(); }
@@ -118,7 +119,7 @@ void written(const Tensor &t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-Tensor dense(const Tensor &t) { return t.resolve_neg().contiguous(); }
+Tensor dense(const Tensor &t) { return t.defined() ? t.resolve_neg().contiguous() : t; }
 Tensor dense(const Maybe &t) { return t ? dense(*t) : Tensor(); }
 Tensor last_contiguous(const Tensor &t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t.resolve_neg() : dense(t); }
 template <class T = void>
@@ -172,6 +173,13 @@ afc_conv_args conv_args(const Tensor &x, const Tensor &weight, const Tensor &bia
   return p;
 }
 
+void check_conv(const Tensor &x, const Tensor &weight, const Maybe &bias, const Maybe &state, const Maybe &lengths) {
+  sequence("x", x, x.sizes(), x.scalar_type(), x.device());
+  check_filter(weight, bias, x.size(2), x.device());
+  optional("initial_state", state, {x.size(0), weight.size(1) - 1, x.size(2)}, x.scalar_type(), x.device());
+  optional("lengths", lengths, {x.size(0)}, at::kInt, x.device());
+}
+
 variable_list conv_forward(const Tensor &x, const Tensor &weight, const Tensor &bias, const Tensor &state, const Tensor &lengths, bool silu, bool want_last) {
   Tensor y = at::empty(x.sizes(), x.options()), last;
   afc_conv_args p = conv_args(x, weight, bias, state, lengths, silu);
@@ -200,9 +208,15 @@ struct Conv : torch::autograd::Function<Conv> {
     first_order_only(dy, dlast);
     if (!dy.defined() && !dlast.defined()) return out;
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &weight = saved[1], &bias = saved[2], &state = saved[3], &lengths = saved[4];
+    const Tensor &x = saved[0], weight = dense(saved[1]), bias = dense(saved[2]), state = dense(saved[3]), lengths = dense(saved[4]);
+    // (hooks of saved tensors may hand back others than they were given)
+    input(x, 3);
+    as_stored(x);
+    check_conv(x, weight, maybe(bias), maybe(state), maybe(lengths));
     dy = dy.defined() ? last_contiguous(dy) : at::zeros(x.sizes(), x.options());
     if (dlast.defined()) dlast = dense(dlast);
+    tensor("the adjoint of y", dy, x.sizes(), x.scalar_type(), x.device());
+    optional("the adjoint of the final state", maybe(dlast), {x.size(0), weight.size(1) - 1, x.size(2)}, x.scalar_type(), x.device());
     const int64_t need = ctx->saved_data["wanted"].toInt();
     const Tensor dx = fresh(x), dw = fresh_if(weight, need & 2), db = fresh_if(bias, need & 4), ds = fresh_if(state, need & 8);
     afc_conv_args p = conv_args(x, weight, bias, state, lengths, ctx->saved_data["silu"].toBool());
@@ -225,10 +239,7 @@ variable_list causal_conv(const Tensor &x, const Tensor &weight, const Maybe &bi
   no_tangent(x, weight, bias, state);
   as_stored(x);
   input(x, 3);
-  sequence("x", x, x.sizes(), x.scalar_type(), x.device());
-  check_filter(weight, bias, x.size(2), x.device());
-  optional("initial_state", state, {x.size(0), weight.size(1) - 1, x.size(2)}, x.scalar_type(), x.device());
-  optional("lengths", lengths, {x.size(0)}, at::kInt, x.device());
+  check_conv(x, weight, bias, state, lengths);
   if (wants_grad(x, weight, bias, state)) return Conv::apply(x, weight, bias, state, lengths, silu, want_last);
   return conv_forward(x, dense(weight), dense(bias), dense(state), dense(lengths), silu, want_last);
 }
@@ -290,6 +301,11 @@ void check_scan(ScanInputs &in) {
   sequence("C", in.C, shape, type, dev);
 }
 
+void check_scan_rows(const Tensor &x, const Tensor &A, const Maybe &state, const Maybe &lengths) {
+  optional("initial_state", state, {x.size(0), x.size(2), A.size(1)}, at::kFloat, x.device());
+  optional("lengths", lengths, {x.size(0)}, at::kInt, x.device());
+}
+
 afc_scan_args scan_args(const ScanInputs &in, const Tensor &state, const Tensor &lengths, bool softplus) {
   const Tensor &x = in.x;
   afc_scan_args p = {};
@@ -346,10 +362,16 @@ struct Scan : torch::autograd::Function<Scan> {
     first_order_only(dy, dlast);
     if (!dy.defined() && !dlast.defined()) return out;
     const variable_list v = ctx->get_saved_variables();
-    const ScanInputs in = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]};
-    const Tensor &x = in.x, &state = v[8], &lengths = v[9], &checkpoints = v[10];
+    ScanInputs in = {v[0], v[1], dense(v[2]), v[3], v[4], dense(v[5]), v[6], dense(v[7])};
+    const Tensor &x = in.x, state = dense(v[8]), lengths = dense(v[9]), checkpoints = dense(v[10]);
+    input(x, 3);
+    as_stored(x, in.dt, in.B, in.C, in.z);
+    check_scan(in);
+    check_scan_rows(x, in.A, maybe(state), maybe(lengths));
     dy = dy.defined() ? last_contiguous(dy) : at::zeros(x.sizes(), x.options());
     if (dlast.defined()) dlast = dense(dlast);
+    tensor("the adjoint of y", dy, x.sizes(), x.scalar_type(), x.device());
+    optional("the adjoint of the final state", maybe(dlast), {x.size(0), x.size(2), in.A.size(1)}, at::kFloat, x.device());
     out[0] = fresh(x), out[1] = fresh(in.dt), out[3] = fresh(in.B), out[4] = fresh(in.C);
     const int64_t need = ctx->saved_data["wanted"].toInt();
     out[2] = fresh_if(in.A, need & 4), out[5] = fresh_if(in.D, need & 32), out[6] = fresh_if(in.z, need & 64);
@@ -361,6 +383,7 @@ struct Scan : torch::autograd::Function<Scan> {
     p.da = ptr<float>(out[2]), p.dd = ptr<float>(out[5]), p.ddt_bias = ptr<float>(out[7]), p.dinitial_state = ptr<float>(out[8]);
     uint64_t kept, scan;
     ok(afc_scan_workspace(&p, &kept, &scan, &p.workspace_bytes));
+    tensor("the states of the forward pass", checkpoints, {(int64_t)kept}, at::kByte, x.device());
     const Tensor ws = space(x, p.workspace_bytes);
     p.workspace = ptr(ws);
     ok(afc_scan_grad(&p, stream_of(x)));
@@ -376,8 +399,7 @@ variable_list selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A,
   input(x, 3);
   ScanInputs in = {x, dt, A, B, C, value(D), value(z), value(dt_bias)};
   check_scan(in);
-  optional("initial_state", state, {x.size(0), x.size(2), A.size(1)}, at::kFloat, x.device());
-  optional("lengths", lengths, {x.size(0)}, at::kInt, x.device());
+  check_scan_rows(x, A, state, lengths);
   if (wants_grad(x, dt, A, B, C, D, z, dt_bias, state)) return Scan::apply(x, dt, A, in.B, in.C, D, z, dt_bias, state, lengths, softplus, want_last);
   in.A = dense(in.A), in.D = dense(D), in.dt_bias = dense(dt_bias);
   return scan_forward(in, dense(state), dense(lengths), softplus, want_last, nullptr);

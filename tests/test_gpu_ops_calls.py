@@ -48,3 +48,53 @@ def test_negated_adjoints():
 @pytest.mark.parametrize("which", infinities.CHECKS)
 def test_infinities(which):
     which(DEV)
+
+
+def all_grads(case, call, names):
+    leaves = {n: case[n].detach().clone().requires_grad_() for n in names}
+    return torch.autograd.grad(call(leaves), list(leaves.values()), [case["dy"], case["dlast"]])
+
+
+def both_operators():
+    c, s = conv_case(4, 2, 40, 24, 3, device=DEV, lengths=[40, 17]), scan_case(4, 2, 40, 24, 16, device=DEV, lengths=[40, 17])
+    return ((c, lambda a: ops.causal_conv(a["x"], a["weight"], a["bias"], True, a["state"], c["lengths"], return_final_state=True), ("x", "weight", "bias", "state")),
+            (s, lambda a: ops.selective_scan(a["x"], a["dt"], a["A"], a["B"], a["C"], a["D"], a["z"], a["dt_bias"], True, a["state"], s["lengths"], return_final_state=True),
+             ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "state")))
+
+
+def test_saved_tensors_that_travel():
+    """recomputed activations, and saved tensors that wait in host memory"""
+    from torch.utils.checkpoint import checkpoint
+    for case, call, names in both_operators():
+        want = all_grads(case, call, names)
+        again = all_grads(case, lambda a: checkpoint(lambda: call(a), use_reentrant=False), names)
+        assert all(torch.equal(p, q) for p, q in zip(want, again))
+        with torch.autograd.graph.save_on_cpu():
+            leaves = {n: case[n].detach().clone().requires_grad_() for n in names}
+            outs = call(leaves)
+        assert all(torch.equal(p, q) for p, q in zip(want, torch.autograd.grad(outs, list(leaves.values()), [case["dy"], case["dlast"]])))
+
+
+@pytest.mark.parametrize("change", [lambda t: t.bfloat16() if t.dtype == torch.float32 else t, lambda t: t.cpu(), lambda t: t[..., :-1].contiguous(), lambda t: t[:1]])
+def test_saved_tensors_that_come_back_as_others_are_refused(change):
+    for case, call, names in both_operators():
+        for which in range(12):
+            seen = []
+
+            def pack(t):
+                seen.append(t)
+                return t, len(seen) - 1
+
+            def unpack(p):
+                return change(p[0]) if p[1] == which else p[0]
+
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                leaves = {n: case[n].detach().clone().requires_grad_() for n in names}
+                outs = call(leaves)
+            if which >= len(seen):
+                break
+            t = seen[which]
+            if change(t).shape == t.shape and change(t).dtype == t.dtype and change(t).device == t.device:
+                continue
+            with pytest.raises((ValueError, RuntimeError)):
+                torch.autograd.grad(outs, list(leaves.values()), [case["dy"], case["dlast"]])
