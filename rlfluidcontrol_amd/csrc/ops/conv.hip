@@ -348,9 +348,8 @@ Tiling run_tiling(const afc_conv_args *p, int v, int run) {
   while (run > 8 && p->batch * t.tiles_l * t.tiles_c < 1024) t = tiling(p, v, run /= 2);
   return t;
 }
-// Channels of a gradient thread.  Eight 16-bit ones would make 16 bytes a load, but with the windows of
-// inputs and of dp, the filter and its gradient they need 288 registers: 275 us against 250 for 3 x 8191 x 4096 forwards and
-// backwards.
+// Channels of a gradient thread.  Eight 16-bit ones would make 16 bytes a load, but with the windows of inputs and of dp, the filter and
+// its gradient they need 256 registers and more: 265 us against 242 for 3 x 8191 x 4096 forwards and backwards.
 constexpr int kGradVector = 4;
 Tiling grad_tiling(const afc_conv_args *p, int v) { return run_tiling(p, v, 64); }
 uint64_t grad_bytes(const afc_conv_args *p) {

@@ -9,9 +9,9 @@
 // four other instructions (4 clocks each) forwards, and 3 + 8 and another exponential backwards, while the tensors that are read
 // and written are `state` times smaller.  So the states stay in registers, everything that is the same for several states is
 // computed once per position and channel and handed over through LDS, and little is spent on a state but the recurrence.
-// 8 x 2048 x 2048 x 16 in bf16: forwards 212 to 225 us, 2.4e12 states/s (the instructions above alone: 85 us; VALU busy 70 % at 2.3
-// GHz, 1.8 TB/s with the checkpoints), backwards 545 to 585 us (200 us; VALU busy 78 % at 2.2 GHz).  What both have to read and write
-// would take 106 us at a copy's rate.
+// 8 x 2048 x 2048 x 16 in bf16: forwards 211 to 223 us, 2.4e12 states/s (the instructions above alone: 85 us; VALU busy 71 % of the
+// time at 2.3 GHz, 1.8 TB/s with the checkpoints), backwards 536 to 575 us (200 us; VALU busy 77 % at 2.2 GHz).  What both have to
+// read and write would take 106 us at a copy's rate.
 #include <stdexcept>
 
 #include "ops_common.h"
@@ -108,7 +108,7 @@ __device__ inline float sum_channels(float *v, int lane) {
 // E neighbouring elements in the form in which they were loaded (converted where they are used, so that loads stay in flight).
 // They are loaded and stored together from any address that suits one element: the memory pipeline takes accesses that start
 // anywhere, so rows of odd widths and slices need no scalar path.  WHOLE: n is E or 0, as where E divides a group's channels
-// (without the branches for a last piece that is cut, 8 x 2048 x 2048 takes 812 us forwards and backwards, with them 892).
+// (without the branches for a last piece that is cut, 8 x 2048 x 2048 takes 760 us forwards and backwards, with them 880).
 template <int DT, int E, bool WHOLE>
 struct Piece {
   typedef Elem<DT> V __attribute__((ext_vector_type(E)));
@@ -1057,8 +1057,8 @@ void check(const afc_scan_args *p, bool grad, bool step) {
 }
 
 // States of a lane and lanes of a channel.  Few states a lane leave registers for two and more waves on a SIMD and make more of
-// them: a state of 16 in 8 lanes of 2, 4 of 4 and 16 of 1 takes 813, 836 and 1010 us at 8 x 2048 x 2048 bf16 forwards and
-// backwards (VALU 75 % busy at 2 waves a SIMD, 67 % at 1), and 33 us, 44 us and 30 us at 8 x 64 x 256 f32.
+// them: a state of 16 in 8 lanes of 2, 4 of 4 and 16 of 1 takes 762, 840 and 962 us at 8 x 2048 x 2048 bf16 forwards and backwards.
+// (At 8 x 64 x 256 f32 the kernels take 30, 40 and 25 us, of a call of 100.)
 struct Split {
   int s, nl;
 };
@@ -1089,6 +1089,8 @@ Plan plan(const afc_scan_args *p, bool grad) {
   //   8 x 128 x 700 (176 blocks) both ways: 48 us whole, 57 in 2 parts
   //   3 x 900 x 1500 (141 blocks) both ways: 239 us whole, 197 in 8 and 4 parts
   //   4 x 4096 x 2048 (256 blocks) both ways: 1116 us whole, 1033 with two parts backwards
+  // All of these have a state of 16; other states go by the same constants, untimed.  (Their kernels' registers admit three blocks on a
+  // CU in some forms where four, or two backwards, are taken here.)
   const int64_t most = grad ? 512 : 1024, resident = !grad ? 4 : split(p).s == 4 ? 1 : 2;
   const auto chunk = [&](int64_t n) { return n == 0 ? 0. : grad ? 1.8 + 1.5 * (double)n : 0.45 + 0.65 * (double)n; };
   const auto estimate = [&](int64_t segs) {
@@ -1231,8 +1233,8 @@ int lanes(const afc_scan_args *p) {
 template <int DT, int NL>
 void go_step4(const afc_scan_args *p, hipStream_t st) {
   const int64_t tiles = ceil_div(p->width, 256 / NL);
-  // four rows a thread where that leaves four blocks for every CU: 131 x 4096 x 16 bf16 takes 15.6 us with four and 18.3 with
-  // one, 1024 x 256 x 16 f32 9.4 and 9.8; below, one row keeps the chip busier
+  // four rows a thread where that leaves four blocks for every CU: 131 x 4096 x 16 bf16 takes 15.0 us with four and 16.6 with
+  // one, 1024 x 256 x 16 f32 8.5 and 8.7; below, one row keeps the chip busier
   const int rows = tiles * p->batch >= 4096 ? 4 : 1;
   const int64_t n = tiles * ceil_div(p->batch, rows);
   want(n < kMostBlocks, "too many blocks");

@@ -6,7 +6,8 @@ global gradient norm (libafc_ops.so, include/afc_ops.h; no counterpart in the re
     grad_norm, clip_grad_norm                 2-norm over many tensors, clipping (Agent.max_grad_norm)
 
 On a GPU every call runs the hand-written kernels on the current stream of the tensors' own device: nothing is copied to the
-host and nothing waits, so the calls may be captured into a graph.  There is no other GPU path; a missing library raises, and so
+host and nothing waits, so the calls may be captured into a graph (backward passes as everywhere in PyTorch: after a warm-up on the
+capturing stream, with no eager graph of the same leaves alive).  There is no other GPU path; a missing library raises, and so
 does what the kernels do not compute: second derivatives and forward-mode ones (NotImplementedError for a tensor with a tangent).
 A tracer sees no kernel that is called behind PyTorch's back, so calls under torch.jit.trace or make_fx raise NotImplementedError
 (torch.compile breaks its graph around them and runs them as they are).
