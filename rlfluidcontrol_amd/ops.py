@@ -336,10 +336,10 @@ def _plain_scan(x, dt, A, B, C_, D, z, dt_bias, softplus, state, lengths):
     h = state if state is not None else xf.new_zeros(Bn, W, A.shape[1])
     ys = []
     for t in range(L):
-        live = None if lengths is None else (t < lengths)[:, None, None]
-        # (behind a row's end the state stays; a zero step size times an infinite state would be NaN in A's gradient)
-        now = torch.exp(delta[:, t, :, None] * A) * (h if live is None else torch.where(live, h, 0.0)) + (delta[:, t] * xf[:, t])[..., None] * Bf[:, t]
-        h = now if live is None else torch.where(live, now, h)
+        decay = torch.exp(delta[:, t, :, None] * A)
+        if lengths is not None:  # behind a row's end the state stays; zero times an infinite one would be NaN in A's gradient
+            decay = torch.where((t < lengths)[:, None, None], decay, 1.0)
+        h = decay * h + (delta[:, t] * xf[:, t])[..., None] * Bf[:, t]
         ys.append((Cf[:, t] * h).sum(-1))
     y = torch.stack(ys, 1) if ys else xf.new_zeros(Bn, 0, W)
     y = y + D * xf if D is not None else y
