@@ -19,6 +19,7 @@
  * `lengths` (int32 per row, or NULL: all of `length`) are the rows' own lengths in a padded batch; a value outside
  * 0..length counts as the nearer end.  Behind a row's length nothing is read, outputs and gradients are zero, and the
  * final state is the one at the row's length.  batch == 0 and length == 0 are valid.
+ * Refused (AFC_EINVAL), before anything is queued: an axis of 2^30 or more, more than 2^48 elements, work of 2^31 blocks or more.
  * A term whose operand is not given is left out.  Infinite values reach what the formulas let them reach; where they enter a sum
  * (over states, channels or positions) it is infinite or NaN.
  */
